@@ -1070,6 +1070,70 @@ int64_t pegainfer_paged_attention_workspace(int32_t n_tiles, int32_t kv_heads, i
 pegainfer_status_t pegainfer_scale_rows(const void* in, int64_t in_stride, void* out, int64_t out_stride, int32_t cols,
                                         int32_t rows, float factor, int32_t dtype, pegainfer_stream_t stream);
 
+/* ---- a paged key/value cache held in 8 bits ----
+ * A page = 16 tokens; a block = a page's tokens of one kv head.  codes: per page [2: keys, values][kv_heads][16 * dim] bytes, pages code_page_stride bytes apart
+ * (so one layer's part of a page-first pool is a cache of its own); a key block is laid out [dim / 64][16 tokens][64], a value block
+ * [dim / 64][4 quads of tokens][64][4 tokens of the quad].  scales: per page [2][kv_heads], pages scale_page_stride values apart, powers of two: a value is
+ * code * scale.  format E4M3: 1-4-3 bits without infinities (top 448); INT8: two's complement (top 127, -128 unused).  dim 64, 128 or 256; codes and
+ * code_page_stride on 16 bytes.
+ * Entry e owns the rows row0[e] .. row0[e + 1] - 1 of a call (row0 ascending from 0; an entry may have none), its tokens are the slots 0, 1, ... of the pages
+ * page_ids[page_indptr[e]] ..; starts[e] = the tokens it holds in front of the call's rows.  All tables are int32 on the device and may change between the
+ * replays of a captured graph.  A slot without a page in [0, n_pages) is not there: never written, never seen, read as 0.  Rows behind row0[n_entries]
+ * are left alone.  max_rows: about the most rows of an entry, max_len: about the most slots; they shape the grid, results hold for any (0 rows: no call).
+ * At most 65535 entries; storage types as elsewhere: 0 = bf16, 1 = fp32. */
+enum { PEGAINFER_KV8_E4M3 = 0, PEGAINFER_KV8_INT8 = 1 };
+typedef struct {
+  void* codes;
+  float* scales;
+  int64_t code_page_stride, scale_page_stride;
+  int32_t format, n_pages, kv_heads, dim;
+  const int32_t *page_indptr, *page_ids;
+  int32_t n_page_ids, n_entries;
+} pegainfer_kv8_cache;
+/* Rows of k, v [n_rows][kv_heads][dim] (rows of dtype at strides of 16 bytes) into the slots starts[e] ...  A block's scale is the least 2^e (e >= -100) whose
+ * top reaches its largest finite value, and not below that of the tokens that were in the block before starts[e], which are rescaled where it grew; codes are
+ * rounded to nearest, ties to even; infinities become the top, a NaN becomes 0.  Slots of a written block behind the entry's last row become 0.  Two entries
+ * of a call must not write the same page. */
+pegainfer_status_t pegainfer_kv8_append(const pegainfer_kv8_cache* cache, const void* k, const void* v, int64_t k_row_stride, int64_t v_row_stride,
+                                        const int32_t* row0, const int32_t* starts, int32_t n_rows, int32_t max_rows, int32_t dtype, pegainfer_stream_t stream);
+/* The slots starts[e] ... as values, into k, v [n_rows][kv_heads][dim]; exact in both types */
+pegainfer_status_t pegainfer_kv8_read(const pegainfer_kv8_cache* cache, const int32_t* row0, const int32_t* starts, void* k, void* v, int32_t n_rows, int32_t max_rows,
+                                      int32_t dtype, pegainfer_stream_t stream);
+/* Causal softmax attention: row i of entry e sees the slots up to starts[e] + i (its own token is in the cache already), query head h reads kv head
+ * h / (heads / kv_heads);  out[row, h] = sum_j softmax_j(scale q . k_j) v_j, zeros where a row sees nothing.  q, out: rows [heads][dim] of dtype at strides of
+ * 16 bytes.  Scores, softmax state and sums are fp32; bf16: the softmax weights are rounded to bf16 where they enter the matrix cores (their sum is not); fp32:
+ * queries and weights enter as three bf16 parts, nothing is rounded.
+ * mass_out given: mass_out[page][kv head][16] (fp32, pages mass_out_page_stride values apart) = mass_keep * mass + the weight that the call's rows and the kv
+ * head's query heads gave to the token, for every slot of an entry that has rows (mass_out may be mass; mass_keep 0: mass is not read and may be NULL).  Every
+ * sum has one order: results do not change from run to run.
+ * workspace: fp32 scratch of pegainfer_kv8_attention_workspace(...) values, of this call alone until it is done. */
+typedef struct {
+  const void* q;
+  int64_t q_row_stride;
+  void* out;
+  int64_t out_row_stride;
+  const int32_t *row0, *starts;
+  int32_t n_rows, max_rows, max_len, heads;
+  float scale;
+  const float* mass;
+  int64_t mass_page_stride;
+  float* mass_out;
+  int64_t mass_out_page_stride;
+  float mass_keep;
+  float* workspace;
+  int32_t dtype;
+} pegainfer_kv8_attn_desc;
+int64_t pegainfer_kv8_attention_workspace(int32_t n_rows, int32_t heads, int32_t with_mass);
+pegainfer_status_t pegainfer_kv8_attention(const pegainfer_kv8_cache* cache, const pegainfer_kv8_attn_desc* d, pegainfer_stream_t stream);
+/* Entries of lens[e] tokens are cut to `budget`: every kv head by itself keeps its first keep_first, its last keep_last and of those between the ones of the
+ * largest mass (equal: the lowest slots; NaN below everything), in their order, in the pages dst_ids[dst_indptr[e]] .. - pages of their own, none of which the
+ * call reads as a source (a source page may be shared).  Entries of at most `budget` tokens are copied whole.  A written block's scale is the largest of its
+ * tokens' scales; codes of smaller ones are rounded again.  mass moves along; slots of a written block behind the last kept token become 0.
+ * kept [n_entries][kv_heads][budget]: the slots that stayed, ascending, then -1. */
+pegainfer_status_t pegainfer_kv8_evict(const pegainfer_kv8_cache* cache, float* mass, int64_t mass_page_stride, const int32_t* lens, const int32_t* dst_indptr,
+                                       const int32_t* dst_ids, int32_t n_dst_ids, int32_t budget, int32_t keep_first, int32_t keep_last, int32_t max_len, int32_t* kept,
+                                       pegainfer_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

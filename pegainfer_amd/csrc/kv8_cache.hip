@@ -1,0 +1,340 @@
+// The 8-bit paged cache's movers: rows in (append), rows out (read), tokens to fresh pages by what they weigh (evict).
+// All of them move bytes; a wave owns a block's keys, another its values, and keeps them in registers from load to store.
+#include <algorithm>
+
+#include "kv8_host.h"
+
+namespace pk {
+
+// ---- where a lane's 16 bytes of a block come from ----
+// keys: value c * 64 + 16 q .. + 15 of token n;  values: tokens 4 q .. + 3 of the values 64 c + 4 n .. + 3, byte 4 j + t = value j, token t
+__device__ __forceinline__ int unit_at(int side, int chunk, int n, int q) { return chunk * 1024 + (side == 0 ? n * 64 + q * 16 : q * 256 + n * 16); }
+
+// x[16] of a unit from rows of T: row(t) gives the row of the block's token t, or -1
+template <typename T, typename Row>
+__device__ __forceinline__ void unit_rows(const T* base, int64_t stride, int side, int chunk, int n, int q, Row row, float* x) {
+  if (side == 0) {
+    const int r = row(n);
+    if (r >= 0) {
+      const T* p = base + r * stride + chunk * 64 + q * 16;
+      Vec8<T>::load(p, x);
+      Vec8<T>::load(p + 8, x + 8);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] = 0.f;
+    }
+  } else {
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const int r = row(4 * q + t);
+      float y[4] = {0.f, 0.f, 0.f, 0.f};
+      if (r >= 0) ld4(base + r * stride + chunk * 64 + 4 * n, y);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[4 * j + t] = y[j];
+    }
+  }
+}
+// token (of 16) that value i of a unit belongs to
+__device__ __forceinline__ int unit_token(int side, int n, int q, int i) { return side == 0 ? n : 4 * q + (i & 3); }
+
+// Rows into the cache.  One workgroup of two waves a (block, head): the rows' largest value, the exponent it wants (not below that of the tokens in front of
+// them in the block), their codes, and the older tokens' codes again where the exponent grew.  Bound by bytes: the rows are read once.
+template <typename T, int FMT, int D>
+__global__ __launch_bounds__(128) void kv8_append_kernel(Kv8 c, const T* k, const T* v, int64_t k_stride, int64_t v_stride, const int32_t* row0,
+                                                         const int32_t* starts, int n_rows) {
+  const int e = blockIdx.z, head = blockIdx.y, side = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 15, q = lane >> 4;
+  const RowSpan rows = row_span(row0, e, n_rows);
+  const int64_t start = starts[e];
+  if (rows.n == 0 || start < 0 || start + rows.n > INT32_MAX - 32) return;
+  const T* base = (side == 0 ? k : v) + head * D;
+  const int64_t stride = side == 0 ? k_stride : v_stride;
+  const int end = (int)start + rows.n;
+  for (int b = (int)start / kKv8Page + blockIdx.x; b * kKv8Page < end; b += gridDim.x) {
+    const int page = c.page(e, b);
+    if (page < 0) continue;
+    const int low = b * kKv8Page, first = max((int)start - low, 0);   // tokens 0 .. first - 1 of the block were there before
+    auto row = [&](int t) { const int s = low + t; return s >= start && s < end ? rows.first + (s - (int)start) : -1; };
+    float x[D / 64][16], amax = 0.f;
+#pragma unroll
+    for (int ch = 0; ch < D / 64; ++ch) {
+      unit_rows(base, stride, side, ch, n, q, row, x[ch]);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float a = fabsf(x[ch][i]);
+        amax = a <= 3.4028234e38f ? fmaxf(amax, a) : amax;            // finite values alone say how large the block is
+      }
+    }
+    int ex = kv8_exp<FMT>(wave_max(amax));
+    uint8_t* blk = c.block(page, side, head, D);
+    float* scale = c.scale(page, side, head);
+    const int was = first > 0 ? exp_of(*scale) : ex;
+    ex = max(ex, was);
+    const float to = pow2f(-ex), again = pow2f(was - ex);
+#pragma unroll
+    for (int ch = 0; ch < D / 64; ++ch) {
+      uint8_t* at = blk + unit_at(side, ch, n, q);
+      u32x4 old = {0, 0, 0, 0};
+      if (first > 0) old = *reinterpret_cast<const u32x4*>(at);
+      u32x4 out;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        float y[4];
+        if (first > 0) kv8_numbers<FMT>(old[w], y);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] = first > 0 && unit_token(side, n, q, 4 * w + i) < first ? y[i] * again : x[ch][4 * w + i] * to;
+        out[w] = kv8_codes<FMT>(y);
+      }
+      *reinterpret_cast<u32x4*>(at) = out;
+    }
+    if (lane == 0) *scale = pow2f(ex);
+  }
+}
+
+// Tokens out of the cache: code * scale, exact in either type.
+template <typename T, int FMT, int D>
+__global__ __launch_bounds__(128) void kv8_read_kernel(Kv8 c, T* k, T* v, const int32_t* row0, const int32_t* starts, int n_rows) {
+  const int e = blockIdx.z, head = blockIdx.y, side = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 15, q = lane >> 4;
+  const RowSpan rows = row_span(row0, e, n_rows);
+  const int64_t start = starts[e];
+  if (rows.n == 0 || start < 0 || start + rows.n > INT32_MAX - 32) return;
+  const int64_t stride = (int64_t)c.kv_heads * D;
+  T* base = (side == 0 ? k : v) + head * D;
+  const int end = (int)start + rows.n;
+  for (int b = (int)start / kKv8Page + blockIdx.x; b * kKv8Page < end; b += gridDim.x) {
+    const int page = c.page(e, b), low = b * kKv8Page;
+    const float scale = page < 0 ? 0.f : *c.scale(page, side, head);
+#pragma unroll
+    for (int ch = 0; ch < D / 64; ++ch) {
+      u32x4 w = {0, 0, 0, 0};
+      if (page >= 0) w = *reinterpret_cast<const u32x4*>(c.block(page, side, head, D) + unit_at(side, ch, n, q));
+      float x[16];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) kv8_numbers<FMT>(w[i], x + 4 * i);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] *= scale;
+      if (side == 0) {
+        const int s = low + n;
+        if (s >= start && s < end) {
+          T* p = base + (rows.first + (s - start)) * stride + ch * 64 + q * 16;
+          Vec8<T>::store(p, x);
+          Vec8<T>::store(p + 8, x + 8);
+        }
+      } else {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const int s = low + 4 * q + t;
+          if (s < start || s >= end) continue;
+          const float y[4] = {x[t], x[4 + t], x[8 + t], x[12 + t]};
+          st4(base + (rows.first + (s - start)) * stride + ch * 64 + 4 * n, y);
+        }
+      }
+    }
+  }
+}
+
+// ---- eviction ----
+// fp32 as an integer of the same order; NaN below everything
+__device__ __forceinline__ uint32_t order_of(float m) {
+  const uint32_t b = __builtin_bit_cast(uint32_t, m);
+  if (m != m) return 0u;
+  if (m == 0.f) return 0x80000000u;                                   // -0 is 0
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+
+// Which tokens stay: one workgroup an (entry, head).  Four passes of a histogram over eight bits give the weight of the lightest token that stays among those
+// between the first and the last ones, a pass with running counts in slot order writes the slots that stay; of equal weights the lowest slots do.
+constexpr int kPickThreads = 1024;
+__global__ __launch_bounds__(kPickThreads) void kv8_pick_kernel(Kv8 c, const float* mass, int64_t mass_stride, const int32_t* lens, int budget, int keep_first,
+                                                                int keep_last, int32_t* kept) {
+  __shared__ uint32_t hist[256];
+  __shared__ int wave_n[2][kPickThreads / 64];
+  __shared__ uint32_t s_bits;
+  __shared__ int s_left;
+  const int e = blockIdx.y, head = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int len = max(lens[e], 0);
+  int32_t* out = kept + ((int64_t)e * c.kv_heads + head) * budget;
+  if (len <= budget) {
+    for (int i = tid; i < budget; i += kPickThreads) out[i] = i < len ? i : -1;
+    return;
+  }
+  auto weight = [&](int s) {
+    const int page = c.page(e, s / kKv8Page);
+    return page < 0 ? 0u : order_of(mass[page * mass_stride + head * kKv8Page + s % kKv8Page]);
+  };
+  const int lo = keep_first, hi = len - keep_last;
+  uint32_t bits = 0;                       // the weight so far: its upper bits
+  int left = budget - keep_first - keep_last;   // tokens still to be found at or below it
+  if (left > 0) {
+    for (int shift = 24; shift >= 0; shift -= 8) {
+      if (tid < 256) hist[tid] = 0;
+      __syncthreads();
+      const uint32_t mask = shift == 24 ? 0u : 0xFFFFFFFFu << (shift + 8);
+      for (int s = lo + tid; s < hi; s += kPickThreads) {
+        const uint32_t w = weight(s);
+        if ((w & mask) == bits) atomicAdd(&hist[(w >> shift) & 255], 1u);
+      }
+      __syncthreads();
+      if (tid == 0) {
+        int n = left, d = 255;
+        for (; d > 0 && (int)hist[d] < n; --d) n -= (int)hist[d];
+        s_bits = bits | (uint32_t)d << shift;
+        s_left = n;
+      }
+      __syncthreads();
+      bits = s_bits;
+      left = s_left;
+    }
+  }
+  int at = 0, ties = 0;                    // tokens kept, and ties met, in the slots before
+  for (int s0 = 0; s0 < len; s0 += kPickThreads) {
+    const int s = s0 + tid;
+    const bool in = s < len, always = in && (s < lo || s >= hi);
+    const uint32_t w = in && !always ? weight(s) : 0u;
+    const bool tie = in && !always && budget - keep_first - keep_last > 0 && w == bits;
+    const uint64_t tie_mask = __builtin_amdgcn_ballot_w64(tie), below = (1ull << lane) - 1;
+    if (lane == 0) wave_n[0][wave] = __popcll(tie_mask);
+    __syncthreads();
+    int tie_at = ties;
+    for (int i = 0; i < kPickThreads / 64; ++i) {
+      const int n = wave_n[0][i];
+      ties += n;
+      tie_at += i < wave ? n : 0;
+    }
+    tie_at += __popcll(tie_mask & below);
+    const bool stays = always || (in && !always && budget - keep_first - keep_last > 0 && (w > bits || (tie && tie_at < left)));
+    const uint64_t mask = __builtin_amdgcn_ballot_w64(stays);
+    if (lane == 0) wave_n[1][wave] = __popcll(mask);
+    __syncthreads();
+    int to = at;
+    for (int i = 0; i < kPickThreads / 64; ++i) {
+      const int n = wave_n[1][i];
+      at += n;
+      to += i < wave ? n : 0;
+    }
+    to += __popcll(mask & below);
+    if (stays && to < budget) out[to] = s;
+  }
+}
+
+// The kept tokens into fresh pages: a wave a block's keys, another its values.  A block's exponent is the largest of its tokens', whose codes stay as they are.
+template <int FMT, int D>
+__global__ __launch_bounds__(128) void kv8_move_kernel(Kv8 c, const int32_t* dst_indptr, const int32_t* dst_ids, int n_dst_ids, float* mass, int64_t mass_stride,
+                                                       const int32_t* lens, int budget, const int32_t* kept) {
+  const int e = blockIdx.z, head = blockIdx.y, side = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 15, q = lane >> 4;
+  const int len = min(max(lens[e], 0), budget);
+  const int32_t* from = kept + ((int64_t)e * c.kv_heads + head) * budget;
+  Kv8 to = c;
+  to.indptr = dst_indptr;
+  to.ids = dst_ids;
+  to.n_ids = n_dst_ids;
+  for (int b = blockIdx.x; b * kKv8Page < len; b += gridDim.x) {
+    const int dst = to.page(e, b);
+    if (dst < 0) continue;
+    // lane n of every sixteen: where token n comes from
+    const int i = b * kKv8Page + n, slot = i < len ? from[i] : -1, src = slot < 0 ? -1 : c.page(e, slot / kKv8Page), t = slot & 15;
+    const int was = src < 0 ? kKv8LeastExp : exp_of(*c.scale(src, side, head));
+    int ex = was;
+#pragma unroll
+    for (int d = 1; d < 16; d <<= 1) ex = max(ex, __shfl_xor(ex, d, 64));
+    if (side == 0 && q == 0) mass[dst * mass_stride + head * kKv8Page + n] = src < 0 ? 0.f : mass[src * mass_stride + head * kKv8Page + t];
+    uint8_t* blk = to.block(dst, side, head, D);
+    if (lane == 0) *to.scale(dst, side, head) = pow2f(ex);
+    int src4[4], t4[4], was4[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      src4[j] = __shfl(src, 4 * q + j, 64);
+      t4[j] = __shfl(t, 4 * q + j, 64);
+      was4[j] = __shfl(was, 4 * q + j, 64);
+    }
+#pragma unroll
+    for (int ch = 0; ch < D / 64; ++ch) {
+      u32x4 w = {0, 0, 0, 0};
+      if (side == 0) {
+        if (src >= 0) w = *reinterpret_cast<const u32x4*>(c.block(src, 0, head, D) + unit_at(0, ch, t, q));
+        if (was != ex) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            float y[4];
+            kv8_numbers<FMT>(w[k], y);
+#pragma unroll
+            for (int m = 0; m < 4; ++m) y[m] *= pow2f(was - ex);
+            w[k] = kv8_codes<FMT>(y);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (src4[j] < 0) continue;
+          const u32x4 g = *reinterpret_cast<const u32x4*>(c.block(src4[j], 1, head, D) + unit_at(1, ch, n, t4[j] >> 2));
+          uint32_t one = 0;                // this token's byte of each of the four values
+#pragma unroll
+          for (int k = 0; k < 4; ++k) one |= (g[k] >> (8 * (t4[j] & 3)) & 255u) << (8 * k);
+          if (was4[j] != ex) {
+            float y[4];
+            kv8_numbers<FMT>(one, y);
+#pragma unroll
+            for (int m = 0; m < 4; ++m) y[m] *= pow2f(was4[j] - ex);
+            one = kv8_codes<FMT>(y);
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) w[k] |= (one >> (8 * k) & 255u) << (8 * j);
+        }
+      }
+      *reinterpret_cast<u32x4*>(blk + unit_at(side, ch, n, q)) = w;
+    }
+  }
+}
+
+}  // namespace pk
+
+using namespace pk;
+
+extern "C" {
+
+pegainfer_status_t pegainfer_kv8_append(const pegainfer_kv8_cache* cache, const void* k, const void* v, int64_t k_row_stride, int64_t v_row_stride,
+                                        const int32_t* row0, const int32_t* starts, int32_t n_rows, int32_t max_rows, int32_t dtype, pegainfer_stream_t stream) {
+  if (!kv8_ok(cache) || n_rows < 0 || max_rows < 0 || (dtype != kDtBf16 && dtype != kDtF32)) return PK_BAD;
+  if (n_rows == 0 || max_rows == 0 || cache->n_entries == 0) return 0;
+  const int64_t width = (int64_t)cache->kv_heads * cache->dim, unit = dtype == kDtBf16 ? 8 : 4;
+  if (!k || !v || !row0 || !starts || !host_aligned16(k) || !host_aligned16(v) || k_row_stride < width || v_row_stride < width || k_row_stride % unit || v_row_stride % unit)
+    return PK_BAD;
+  const Kv8 c = kv8_of(cache);
+  const dim3 grid(std::min(max_rows, n_rows) / kKv8Page + 2, c.kv_heads, c.entries);
+  kv8_by(dtype, cache->format, cache->dim, [&](auto* t, auto fmt, auto dim) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    kv8_append_kernel<T, fmt(), dim()><<<grid, 128, 0, as_stream(stream)>>>(c, static_cast<const T*>(k), static_cast<const T*>(v), k_row_stride, v_row_stride, row0,
+                                                                            starts, n_rows);
+  });
+  return (pegainfer_status_t)hipGetLastError();
+}
+
+pegainfer_status_t pegainfer_kv8_read(const pegainfer_kv8_cache* cache, const int32_t* row0, const int32_t* starts, void* k, void* v, int32_t n_rows, int32_t max_rows,
+                                      int32_t dtype, pegainfer_stream_t stream) {
+  if (!kv8_ok(cache) || n_rows < 0 || max_rows < 0 || (dtype != kDtBf16 && dtype != kDtF32)) return PK_BAD;
+  if (n_rows == 0 || max_rows == 0 || cache->n_entries == 0) return 0;
+  if (!row0 || !starts || !k || !v || !host_aligned16(k) || !host_aligned16(v)) return PK_BAD;
+  const Kv8 c = kv8_of(cache);
+  const dim3 grid(std::min(max_rows, n_rows) / kKv8Page + 2, c.kv_heads, c.entries);
+  kv8_by(dtype, cache->format, cache->dim, [&](auto* t, auto fmt, auto dim) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    kv8_read_kernel<T, fmt(), dim()><<<grid, 128, 0, as_stream(stream)>>>(c, static_cast<T*>(k), static_cast<T*>(v), row0, starts, n_rows);
+  });
+  return (pegainfer_status_t)hipGetLastError();
+}
+
+pegainfer_status_t pegainfer_kv8_evict(const pegainfer_kv8_cache* cache, float* mass, int64_t mass_page_stride, const int32_t* lens, const int32_t* dst_indptr,
+                                       const int32_t* dst_ids, int32_t n_dst_ids, int32_t budget, int32_t keep_first, int32_t keep_last, int32_t max_len, int32_t* kept,
+                                       pegainfer_stream_t stream) {
+  if (!kv8_ok(cache) || budget < 1 || keep_first < 0 || keep_last < 0 || keep_first > budget - keep_last || n_dst_ids < 0 || max_len < 0) return PK_BAD;
+  if (cache->n_entries == 0) return 0;
+  if (!mass || !lens || !dst_indptr || (!dst_ids && n_dst_ids > 0) || !kept || mass_page_stride < (int64_t)cache->kv_heads * kKv8Page) return PK_BAD;
+  const Kv8 c = kv8_of(cache);
+  kv8_pick_kernel<<<dim3(c.kv_heads, c.entries), kPickThreads, 0, as_stream(stream)>>>(c, mass, mass_page_stride, lens, budget, keep_first, keep_last, kept);
+  const dim3 grid(std::max(1, ceil_div(std::min(budget, max_len), kKv8Page)), c.kv_heads, c.entries);
+  kv8_by(kDtBf16, cache->format, cache->dim, [&](auto*, auto fmt, auto dim) {
+    kv8_move_kernel<fmt(), dim()><<<grid, 128, 0, as_stream(stream)>>>(c, dst_indptr, dst_ids, n_dst_ids, mass, mass_page_stride, lens, budget, kept);
+  });
+  return (pegainfer_status_t)hipGetLastError();
+}
+
+}  // extern "C"

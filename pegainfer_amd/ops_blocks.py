@@ -935,3 +935,131 @@ def recurrent_step(kind, qkv, offs, proj, state, slots, norm_w, heads, kv_heads,
         return q, out
     _chk(ffi.lib().pegainfer_recurrent_step(ctypes.addressof(q), _stream()), "recurrent_step")
     return out
+
+
+# ---- a paged key/value cache held in 8 bits ----
+# codes [pages, 2, kv_heads, 16 * dim] of torch.float8_e4m3fn or torch.int8 (dimension 0 at any stride of 16 bytes: a layer's part of a page-first pool), scales
+# fp32 [pages, 2, kv_heads]; row0 [entries + 1], starts [entries], page_indptr [entries + 1], page_ids: int32 on the device, as include/pegainfer_kernels_blocks.h says
+Kv8Cache = _struct("Kv8Cache", [("p", "codes scales"), ("l", "code_page_stride scale_page_stride"), ("i", "format n_pages kv_heads dim"), ("p", "page_indptr page_ids"),
+                                ("i", "n_page_ids n_entries")])
+Kv8AttnDesc = _struct("Kv8AttnDesc", [("p", "q"), ("l", "q_row_stride"), ("p", "out"), ("l", "out_row_stride"), ("p", "row0 starts"), ("i", "n_rows max_rows max_len heads"),
+                                      ("f", "scale"), ("p", "mass"), ("l", "mass_page_stride"), ("p", "mass_out"), ("l", "mass_out_page_stride"), ("f", "mass_keep"),
+                                      ("p", "workspace"), ("i", "dtype")])
+KV8_FORMATS = {torch.float8_e4m3fn: 0, torch.int8: 1}
+
+
+def _kv8_need(ok, what):
+    if not ok:
+        raise ValueError("kv8: " + what)
+
+
+def _kv8_tables(device, *tables):
+    for t, n, what in tables:
+        _kv8_need(t.dtype == torch.int32 and t.is_contiguous() and t.device == device and (t.numel() == n if n is not None else t.dim() == 1),
+                  "%s: contiguous int32 on the cache's device%s" % (what, "" if n is None else ", %d values" % n))
+
+
+def _kv8_cache(codes, scales, page_indptr, page_ids, entries):
+    """-> (descriptor, kv_heads, dim); refuses what the kernels do not take"""
+    _kv8_need(codes.dtype in KV8_FORMATS, "codes of torch.float8_e4m3fn or torch.int8")
+    _kv8_need(codes.is_cuda and codes.device.index == torch.cuda.current_device(), "a cache on the current device")
+    _kv8_need(codes.dim() == 4 and codes.shape[1] == 2 and codes.shape[3] in (1024, 2048, 4096), "codes [pages, 2, kv_heads, 16 * dim] with dim 64, 128 or 256")
+    pages, _, kv, m = codes.shape
+    _kv8_need(codes.stride()[1:] == (kv * m, m, 1) and codes.stride(0) % 16 == 0 and codes.stride(0) >= 2 * kv * m and codes.data_ptr() % 16 == 0,
+              "codes: a page's values together, pages apart by a multiple of 16 bytes")
+    _kv8_need(scales.dtype == torch.float32 and scales.device == codes.device and scales.shape == (pages, 2, kv) and scales.stride()[1:] == (kv, 1) and
+              scales.stride(0) >= 2 * kv, "scales fp32 [pages, 2, kv_heads] on the cache's device, a page's together")
+    _kv8_need(1 <= kv <= 65535 and entries <= 65535, "at most 65535 kv heads and entries")
+    _kv8_tables(codes.device, (page_indptr, entries + 1, "page_indptr"), (page_ids, None, "page_ids"))
+    return Kv8Cache(codes.data_ptr(), scales.data_ptr(), codes.stride(0), scales.stride(0), KV8_FORMATS[codes.dtype], pages, kv, m // 16, page_indptr.data_ptr(),
+                    page_ids.data_ptr(), page_ids.numel(), entries), kv, m // 16
+
+
+def _kv8_rows(x, heads, dim, device, what):
+    _kv8_need(x.dtype in (torch.bfloat16, torch.float32) and x.device == device, "%s: bf16 or fp32 on the cache's device" % what)
+    _kv8_need(x.dim() == 3 and x.shape[2] == dim and (heads is None or x.shape[1] == heads), "%s: rows of heads of %d values" % (what, dim))
+    _kv8_need(x.stride(2) == 1 and x.stride(1) == dim and (x.stride(0) >= x.shape[1] * dim or x.shape[0] <= 1) and x.stride(0) * x.element_size() % 16 == 0 and x.data_ptr() % 16 == 0,
+              "%s: a row's values together, rows apart by a multiple of 16 bytes" % what)
+    return max(x.stride(0), x.shape[1] * dim)
+
+
+def _kv8_mass(mass, codes, what):
+    _kv8_need(mass.dtype == torch.float32 and mass.device == codes.device and mass.shape == (codes.shape[0], codes.shape[2], 16) and mass.stride()[1:] == (16, 1) and
+              mass.stride(0) >= codes.shape[2] * 16, "%s fp32 [pages, kv_heads, 16] on the cache's device, a page's together" % what)
+    return mass.stride(0)
+
+
+def kv8_append(k, v, codes, scales, row0, starts, page_indptr, page_ids, max_rows=None):
+    """rows k, v [rows, kv_heads, dim] (bf16 or fp32 views, row stride free) into the cache behind the starts[e] tokens of their entry.  max_rows: about the most
+    rows of an entry (None: all)"""
+    entries = row0.numel() - 1
+    cache, kv, dim = _kv8_cache(codes, scales, page_indptr, page_ids, entries)
+    _kv8_tables(codes.device, (row0, entries + 1, "row0"), (starts, entries, "starts"))
+    strides = _kv8_rows(k, kv, dim, codes.device, "k"), _kv8_rows(v, kv, dim, codes.device, "v")
+    _kv8_need(k.dtype == v.dtype and k.shape == v.shape, "k and v of one shape and type")
+    _chk(ffi.lib().pegainfer_kv8_append(ctypes.addressof(cache), k.data_ptr(), v.data_ptr(), *strides, row0.data_ptr(), starts.data_ptr(), k.shape[0],
+                                        k.shape[0] if max_rows is None else int(max_rows), _dt(k), _stream()), "kv8_append")
+
+
+def kv8_read(codes, scales, row0, starts, page_indptr, page_ids, n_rows, dtype=torch.bfloat16, max_rows=None, out=None):
+    """-> k, v [n_rows, kv_heads, dim] of dtype: the slots starts[e] ... of every entry, as many as it has rows.  out: (k, v) to write to; rows behind row0[-1] stay as
+    they are (in a fresh tensor: unset)"""
+    entries = row0.numel() - 1
+    cache, kv, dim = _kv8_cache(codes, scales, page_indptr, page_ids, entries)
+    _kv8_tables(codes.device, (row0, entries + 1, "row0"), (starts, entries, "starts"))
+    _kv8_need(n_rows >= 0 and dtype in (torch.bfloat16, torch.float32), "n_rows >= 0, values in bf16 or fp32")
+    if out is None:
+        out = torch.empty((2, n_rows, kv, dim), dtype=dtype, device=codes.device).unbind(0)
+    k, v = out
+    for x, what in ((k, "k"), (v, "v")):
+        _kv8_need(x.shape == (n_rows, kv, dim) and x.dtype == dtype and x.device == codes.device and x.is_contiguous() and x.data_ptr() % 16 == 0,
+                  "out: contiguous %s [n_rows, kv_heads, dim] of dtype" % what)
+    _chk(ffi.lib().pegainfer_kv8_read(ctypes.addressof(cache), row0.data_ptr(), starts.data_ptr(), k.data_ptr(), v.data_ptr(), int(n_rows),
+                                      int(n_rows if max_rows is None else max_rows), _dt(k), _stream()), "kv8_read")
+    return k, v
+
+
+def kv8_attention(q, codes, scales, row0, starts, page_indptr, page_ids, scale, max_rows=None, max_len=None, out=None, mass=None, mass_out=None, mass_keep=1.0):
+    """-> out [rows, heads, dim]: causal attention of q's rows (their own tokens are in the cache already).  max_rows / max_len: about the most rows / tokens of an
+    entry (None: all rows / all pages).  mass fp32 [pages, kv_heads, 16]: mass_out (None: mass itself) becomes mass_keep * mass + the weight that every token got;
+    mass_out alone with mass_keep 0: the weight of this call."""
+    entries = row0.numel() - 1
+    cache, kv, dim = _kv8_cache(codes, scales, page_indptr, page_ids, entries)
+    _kv8_tables(codes.device, (row0, entries + 1, "row0"), (starts, entries, "starts"))
+    q_stride = _kv8_rows(q, None, dim, codes.device, "q")
+    T, H, _ = q.shape
+    _kv8_need(H > 0 and H % kv == 0, "query heads: a multiple of the kv heads")
+    if out is None:
+        out = torch.empty((T, H, dim), dtype=q.dtype, device=q.device)
+    _kv8_need(out.dtype == q.dtype and out.shape == q.shape, "out like q")
+    out_stride = _kv8_rows(out, H, dim, codes.device, "out")
+    mass_out = mass if mass_out is None else mass_out
+    _kv8_need(mass_out is None or mass is not None or mass_keep == 0, "mass_keep other than 0 needs mass")
+    d = Kv8AttnDesc(q.data_ptr(), q_stride, out.data_ptr(), out_stride, row0.data_ptr(), starts.data_ptr(), T, T if max_rows is None else int(max_rows),
+                    page_ids.numel() * 16 if max_len is None else int(max_len), H, float(scale))
+    if mass_out is not None:
+        if mass is not None:
+            d.mass, d.mass_page_stride = mass.data_ptr(), _kv8_mass(mass, codes, "mass")
+        d.mass_out, d.mass_out_page_stride, d.mass_keep = mass_out.data_ptr(), _kv8_mass(mass_out, codes, "mass_out"), float(mass_keep)
+    d.dtype = _dt(q)
+    n = ffi.lib().pegainfer_kv8_attention_workspace(T, H, int(mass_out is not None))
+    if n > 0:
+        ws = torch.empty(n, dtype=torch.float32, device=q.device)
+        d.workspace = ws.data_ptr()
+    _chk(ffi.lib().pegainfer_kv8_attention(ctypes.addressof(cache), ctypes.addressof(d), _stream()), "kv8_attention")
+    return out
+
+
+def kv8_evict(codes, scales, mass, lens, page_indptr, page_ids, dst_indptr, dst_ids, budget, keep_first=0, keep_last=0, max_len=None):
+    """-> kept int32 [entries, kv_heads, budget]: the slots that stayed, then -1.  Entries of lens[e] tokens are cut to the `budget` heaviest of every kv head (its
+    first keep_first and last keep_last among them) and moved, with their mass, to the pages dst_ids[dst_indptr[e]] ..., which are no source pages of the call."""
+    entries = lens.numel()
+    cache, kv, _ = _kv8_cache(codes, scales, page_indptr, page_ids, entries)
+    _kv8_tables(codes.device, (lens, entries, "lens"), (dst_indptr, entries + 1, "dst_indptr"), (dst_ids, None, "dst_ids"))
+    _kv8_need(budget >= 1 and keep_first >= 0 and keep_last >= 0 and keep_first + keep_last <= budget, "budget of at least 1 token, keep_first + keep_last within it")
+    stride = _kv8_mass(mass, codes, "mass")
+    kept = torch.empty((entries, kv, budget), dtype=torch.int32, device=codes.device)
+    _chk(ffi.lib().pegainfer_kv8_evict(ctypes.addressof(cache), mass.data_ptr(), stride, lens.data_ptr(), dst_indptr.data_ptr(), dst_ids.data_ptr(), dst_ids.numel(),
+                                       int(budget), int(keep_first), int(keep_last), page_ids.numel() * 16 if max_len is None else int(max_len), kept.data_ptr(),
+                                       _stream()), "kv8_evict")
+    return kept

@@ -1,0 +1,387 @@
+"""The 8-bit paged cache on the device against its float64 restatement: movers bit for bit, attention and weights within derived bounds."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import kv8_ref as R
+from pegainfer_amd import ops_blocks as B
+from kv8_common import Cache, TORCH, attention_bound, codes_of, mass_bound
+
+pytestmark = pytest.mark.gpu
+TYPES = {"bf16": torch.bfloat16, "fp32": torch.float32}
+
+
+def rows_of(rng, n, heads, dim, dtype, size=1.0):
+    """values that dtype holds, as numpy float32 and on the device, inside a wider row (a view of a projection)"""
+    x = torch.from_numpy((rng.randn(n, heads, dim) * size).astype(np.float32)).to(dtype)
+    wide = torch.zeros(n, heads * dim + 32, dtype=dtype, device="cuda")
+    view = wide[:, 16:16 + heads * dim].unflatten(1, (heads, dim))
+    view.copy_(x)
+    return x.float().numpy(), view
+
+
+def same(d, c, codes, scales):
+    got = codes_of(d)
+    bad = np.argwhere(got != codes)
+    assert len(bad) == 0, (len(bad), bad[:4], got[tuple(bad[0])], codes[tuple(bad[0])])
+    assert np.array_equal(d.scales.cpu().numpy(), scales)
+
+
+# ---- rows in and out ----
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("kv,dim", [(1, 64), (3, 128), (2, 256)])
+def test_append_and_read(fmt, dtype, kv, dim):
+    c = Cache([0, 5, 16, 31, 40, 7, 0], [1, 1, 33, 1, 0, 9, 17], kv, dim, fmt, seed=dim + kv, layers=2)
+    d = c.device()
+    k, kd = rows_of(c.rng, c.row0[-1] + 2, kv, dim, TYPES[dtype], 3.0)
+    v, vd = rows_of(c.rng, c.row0[-1] + 2, kv, dim, TYPES[dtype], 0.01)
+    codes, scales = c.codes.copy(), c.scales.copy()
+    R.append(k, v, codes, scales, fmt, c.row0, c.starts, c.tables)
+    B.kv8_append(kd, vd, d.codes, d.scales, d.row0, d.starts, d.indptr, d.ids)
+    same(d, c, codes, scales)
+    assert (d.pool[:, 0] == 0).all()                                    # the other layer's part
+    for hint in (None, 1, 33):
+        out = tuple(torch.full((c.row0[-1] + 2, kv, dim), 7.0, dtype=TYPES[dtype], device="cuda") for _ in range(2))
+        got = B.kv8_read(d.codes, d.scales, d.row0, d.starts, d.indptr, d.ids, c.row0[-1] + 2, dtype=TYPES[dtype], max_rows=hint, out=out)
+        for x, y in zip(got, R.read(codes, scales, fmt, dim, c.row0, c.starts, c.tables)):
+            assert np.array_equal(x[:-2].double().cpu().numpy(), y) and (x[-2:] == 7).all()
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+def test_append_values_at_the_ends_of_their_range(fmt):
+    c = Cache([0, 3], [16, 5], 2, 64, fmt, seed=3)
+    d = c.device()
+    k = np.zeros((21, 2, 64), np.float32)
+    k[0, 0, :6] = [np.inf, -np.inf, np.nan, 448, -448.5, 1e-3]
+    k[1, 1, :3] = [np.nan, np.inf, 0.0]                                   # no finite value but 0
+    k[16, 0, :4] = [3.3e38, -3.3e38, 1e38, 1e-38]
+    k[17, 1, :4] = [1e-40, -1e-40, 2.0 ** -126, 0.0]
+    v = -k[::-1].copy()
+    codes, scales = c.codes.copy(), c.scales.copy()
+    R.append(k, v, codes, scales, fmt, c.row0, c.starts, c.tables)
+    B.kv8_append(torch.from_numpy(k).cuda(), torch.from_numpy(v).cuda(), d.codes, d.scales, d.row0, d.starts, d.indptr, d.ids)
+    same(d, c, codes, scales)
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+def test_append_token_by_token(fmt):
+    """a block whose scale grows with every token, then shrinks in the next block"""
+    c = Cache([0], [40], 2, 128, fmt, seed=5)
+    d = c.device()
+    codes, scales = c.codes.copy(), c.scales.copy()
+    for t in range(40):
+        k, kd = rows_of(c.rng, 1, 2, 128, torch.bfloat16, 1.7 ** (t if t < 16 else -t))
+        v, vd = rows_of(c.rng, 1, 2, 128, torch.bfloat16, 1.3 ** t)
+        R.append(k, v, codes, scales, fmt, [0, 1], [t], c.tables)
+        B.kv8_append(kd, vd, d.codes, d.scales, torch.tensor([0, 1], dtype=torch.int32, device="cuda"), torch.tensor([t], dtype=torch.int32, device="cuda"), d.indptr, d.ids)
+        same(d, c, codes, scales)
+
+
+# ---- attention ----
+def attend(c, heads, dtype, weigh=False, keep=1.0, separate=False, hints=(None, None), q_size=1.0, seed=0, d=None):
+    d = d or c.device()
+    n = c.row0[-1]
+    q, qd = rows_of(np.random.RandomState(seed), n + 2, heads, c.dim, dtype, q_size)
+    out = torch.full((n + 2, heads, c.dim), 7.0, dtype=dtype, device="cuda")
+    scale = c.dim ** -0.5
+    kw = {}
+    if weigh:
+        kw = dict(mass=d.mass, mass_keep=keep)
+        if separate:
+            kw["mass_out"] = torch.full_like(d.mass, 5.0)
+    got = B.kv8_attention(qd, d.codes, d.scales, d.row0, d.starts, d.indptr, d.ids, scale, max_rows=hints[0], max_len=hints[1], out=out, **kw)
+    assert (got[n:] == 7).all()
+    want, mass, spread, reach = R.attention(q[:n], c.codes, c.scales, c.fmt, c.row0, c.starts, c.tables, scale)
+    length = max([s + r for s, r in zip(c.starts, c.rows)] + [1])
+    err = np.abs(got[:n].double().cpu().numpy() - want)
+    bound = attention_bound(spread, reach, want, c.dim, length, dtype)
+    assert np.isfinite(err).all() and (err <= bound).all(), (err.max(), (err / bound).max(), np.argwhere(err > bound)[:5])
+    if weigh:
+        end = kw.get("mass_out", d.mass).cpu().numpy().astype(np.float64)
+        full = np.full_like(c.mass, 5.0, dtype=np.float64) if separate else c.mass.astype(np.float64)
+        most, rest = np.zeros_like(full), np.ones(full.shape, bool)
+        for e in range(c.B):
+            for s in range(mass[e].shape[1]):
+                p = R.page_of(c.tables, e, s // 16, c.pages)
+                if p < 0:
+                    continue
+                rest[p, :, s % 16] = False
+                full[p, :, s % 16] = (0 if keep == 0 else keep * c.mass[p, :, s % 16].astype(np.float64)) + mass[e][:, s]
+                most[p, :, s % 16] = mass_bound(mass[e][:, s], reach.max(), c.dim, length, c.rows[e] * heads // c.kv) + 2.0 ** -23 * np.abs(full[p, :, s % 16])
+        assert np.array_equal(end[rest], full[rest], equal_nan=True)     # slots without a token stay as they were
+        off = np.where(rest, 0.0, np.abs(end - full))
+        assert np.isfinite(off).all() and (off <= most).all(), ((off / np.maximum(most, 1e-300)).max(), np.argwhere(off > most)[:5])
+    return d, got
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("kv,group,dim", [(1, 1, 64), (2, 3, 64), (2, 4, 128), (1, 17, 128), (2, 4, 256)])
+def test_attention_of_ragged_batches(fmt, dtype, kv, group, dim):
+    c = Cache([0, 0, 15, 16, 17, 100, 333, 0, 64], [1, 2, 1, 1, 1, 1, 1, 0, 5], kv, dim, fmt, seed=group)
+    attend(c, kv * group, TYPES[dtype])
+    c = Cache([0, 33, 0, 250], [70, 18, 16, 21], kv, dim, fmt, seed=group + 1, layers=2)
+    for hints in [(None, None), (1, 1), (70, 280)]:
+        attend(c, kv * group, TYPES[dtype], hints=hints)
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_attention_over_a_long_cache_and_of_many_rows(fmt, dtype):
+    attend(Cache([3000, 17, 1499], [1, 1, 2], 1, 128, fmt, seed=1), 4, TYPES[dtype])
+    attend(Cache([100, 700], [150, 40], 1, 64, fmt, seed=2), 2, TYPES[dtype])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_attention_with_sharp_and_flat_scores(dtype):
+    for size in (0.0, 30.0):
+        attend(Cache([200, 5], [3, 1], 2, 128, "int8", seed=4), 4, TYPES[dtype], q_size=size)
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("kv,group,dim", [(1, 1, 64), (2, 3, 128), (2, 4, 256), (1, 17, 64)])
+def test_weights_of_cached_tokens(fmt, dtype, kv, group, dim):
+    steps = Cache([0, 15, 16, 100, 333, 0], [1, 1, 1, 1, 1, 0], kv, dim, fmt, seed=group)
+    prompts = Cache([0, 33, 0, 250], [70, 18, 16, 21], kv, dim, fmt, seed=group + 1, layers=2)
+    for c in (steps, prompts):
+        attend(c, kv * group, TYPES[dtype], weigh=True)
+        attend(c, kv * group, TYPES[dtype], weigh=True, keep=0.5, separate=True, hints=(1, 1))
+    c.mass[:] = np.nan
+    attend(c, kv * group, TYPES[dtype], weigh=True, keep=0.0)
+
+
+def test_weights_of_many_rows():
+    attend(Cache([0, 300], [200, 90], 1, 64, "e4m3", seed=9), 4, torch.bfloat16, weigh=True)
+
+
+def test_runs_repeat_bit_for_bit():
+    c = Cache([900, 40, 0], [1, 33, 100], 2, 128, "e4m3", seed=6)
+    d, a = attend(c, 8, torch.bfloat16, weigh=True, keep=0.0)
+    first = d.mass.clone()
+    for _ in range(3):
+        _, b = attend(c, 8, torch.bfloat16, weigh=True, keep=0.0, d=d)
+        assert torch.equal(a, b) and torch.equal(d.mass, first)
+
+
+def test_tables_that_lead_nowhere():
+    """pages out of range, tables that end early, rows out of range, entries that start nowhere: not there, and nothing else is touched"""
+    c = Cache([20, 40, 5, 33, 70], [4, 1, 1, 2, 1], 2, 64, "int8", seed=8)
+    c.ids[c.indptr[0]] = -3
+    c.ids[c.indptr[1] + 1] = c.pages
+    c.ids[c.indptr[2]] = 2 ** 31 - 1                   # all its tokens: zeros
+    c.indptr[5] -= 1                                   # the last entry's last page: its newest token
+    d, out = attend(c, 4, torch.bfloat16, weigh=True)
+    assert (out[5] == 0).all()
+    codes, scales = c.codes.copy(), c.scales.copy()
+    k, kd = rows_of(c.rng, c.row0[-1], 2, 64, torch.float32)
+    R.append(k, k, codes, scales, "int8", c.row0, c.starts, c.tables)
+    B.kv8_append(kd, kd, d.codes, d.scales, d.row0, d.starts, d.indptr, d.ids)
+    same(d, c, codes, scales)
+    for x, y in zip(B.kv8_read(d.codes, d.scales, d.row0, d.starts, d.indptr, d.ids, c.row0[-1]), R.read(codes, scales, "int8", 64, c.row0, c.starts, c.tables)):
+        assert np.array_equal(x.double().cpu().numpy(), y)
+    # an entry that starts before 0, one whose rows lie behind the rows there are
+    d.starts[0] = -1
+    d.row0[5] = 100
+    out = torch.full((9, 4, 64), 7.0, dtype=torch.bfloat16, device="cuda")
+    B.kv8_attention(torch.zeros_like(out), d.codes, d.scales, d.row0, d.starts, d.indptr, d.ids, 1.0, out=out)
+    assert (out[:4] == 7).all() and (out[4:] != 7).all()
+
+
+# ---- eviction ----
+def run_evict(c, lens, budget, first, last, dst_extra=0):
+    """entries of `lens` tokens over c's pages; fresh pages behind c's own"""
+    n = [(min(x, budget) + 15) // 16 + dst_extra for x in lens]
+    free = [p for p in range(c.pages) if p not in c.ids]
+    assert len(free) >= sum(n)
+    dst = [int(x) for x in np.concatenate([[0], np.cumsum(n)])], free[:sum(n)]
+    d = c.device()
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    codes, scales, mass = c.codes.copy(), c.scales.copy(), c.mass.copy()
+    want = R.evict(codes, scales, c.fmt, c.dim, mass, lens, c.tables, dst, budget, first, last)
+    for hint in (None, 1):
+        kept = B.kv8_evict(d.codes, d.scales, d.mass, i32(lens), d.indptr, d.ids, i32(dst[0]), i32(dst[1]), budget, first, last, max_len=hint)
+        assert np.array_equal(kept.cpu().numpy(), want)
+        same(d, c, codes, scales)
+        assert np.array_equal(d.mass.cpu().numpy(), mass, equal_nan=True)
+    return d, kept, dst
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("kv,dim", [(1, 64), (3, 128), (2, 256)])
+@pytest.mark.parametrize("budget,first,last", [(1, 0, 0), (16, 4, 4), (37, 0, 20), (64, 64, 0), (50, 1, 49), (200, 3, 5)])
+def test_evict(fmt, kv, dim, budget, first, last):
+    lens = [0, 1, 16, 37, 150, 200, 201, 64]
+    c = Cache(lens, [0] * 8, kv, dim, fmt, seed=budget, pages=150, dirty=False, layers=2)
+    run_evict(c, lens, budget, first, last)
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+def test_evict_equal_and_odd_weights(fmt):
+    lens = [120, 120, 120]
+    c = Cache(lens, [0] * 3, 2, 64, fmt, seed=1, pages=60, dirty=False)
+    c.mass[:, 0] = np.random.RandomState(0).choice(np.array([0.0, -0.0, 1.0, -1.0], np.float32), c.mass[:, 0].shape)
+    c.mass[:, 1] = np.random.RandomState(1).choice(np.array([np.nan, np.inf, -np.inf, 1e-40, 0.0], np.float32), c.mass[:, 1].shape)
+    run_evict(c, lens, 50, 2, 10)
+    run_evict(c, lens, 100, 0, 0)
+
+
+def test_evict_of_many_tokens_and_of_shared_pages():
+    lens = [2500, 1030, 2500]
+    c = Cache(lens, [0] * 3, 2, 64, "int8", seed=2, pages=700, dirty=False)
+    a, b = c.indptr[0], c.indptr[2]
+    c.ids[b:b + 100] = c.ids[a:a + 100]                # the third entry's first 1600 tokens are the first one's
+    run_evict(c, lens, 1029, 4, 100, dst_extra=1)
+
+
+def test_evict_with_pages_that_are_not_there():
+    lens = [100, 90]
+    c = Cache(lens, [0] * 2, 2, 64, "e4m3", seed=2, pages=60, dirty=False)
+    c.ids[2], c.ids[c.indptr[1] + 1] = -1, 10 ** 6
+    run_evict(c, lens, 40, 20, 5)
+    run_evict(c, lens, 90, 0, 0)
+
+
+# ---- together, as a server uses them ----
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+def test_prompt_steps_eviction_steps(fmt):
+    """prompts in, their weights, steps, a cut to a budget, steps behind it: against the restatement all the way"""
+    kv, H, dim, budget, heads_of = 2, 6, 64, 48, 3
+    c = Cache([0, 0], [90, 37], kv, dim, fmt, seed=11, pages=40, dirty=False, extra=1)
+    d = c.device()
+    free = [p for p in range(c.pages) if p not in c.ids]
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    codes, scales, mass = c.codes.copy(), c.scales.copy(), c.mass.copy()
+    tables, starts, rows = c.tables, [0, 0], [90, 37]
+
+    def step(keep):
+        row0 = [0, rows[0], rows[0] + rows[1]]
+        (k, kd), (v, vd), (q, qd) = (rows_of(c.rng, row0[-1], h, dim, torch.bfloat16) for h in (kv, kv, H))
+        t = i32(row0), i32(starts), i32(tables[0]), i32(tables[1])
+        B.kv8_append(kd, vd, d.codes, d.scales, *t)
+        R.append(k, v, codes, scales, fmt, row0, starts, tables)
+        same(d, c, codes, scales)
+        out = B.kv8_attention(qd, d.codes, d.scales, *t, 0.125, mass=d.mass, mass_keep=keep)
+        want, new, spread, reach = R.attention(q, codes, scales, fmt, row0, starts, tables, 0.125)
+        err = np.abs(out.double().cpu().numpy() - want)
+        assert (err <= attention_bound(spread, reach, want, dim, 128, torch.bfloat16)).all()
+        for e in range(2):
+            for s in range(new[e].shape[1]):
+                p = R.page_of(tables, e, s // 16, c.pages)
+                mass[p, :, s % 16] = (keep * mass[p, :, s % 16] if keep else 0) + new[e][:, s]
+                off = np.abs(d.mass[p, :, s % 16].cpu().numpy() - mass[p, :, s % 16])
+                assert (off <= mass_bound(new[e][:, s], reach.max(), dim, 128, rows[e] * heads_of) + 1e-5 * mass[p, :, s % 16]).all()
+        mass[:] = d.mass.cpu().numpy()                   # from here on the device's own sums
+        starts[:] = [s + r for s, r in zip(starts, rows)]
+
+    step(0.0)
+    rows = [1, 1]
+    for _ in range(3):
+        step(1.0)
+    n = [(min(x, budget) + 15) // 16 + 1 for x in starts]
+    dst = [0, n[0], n[0] + n[1]], free[:sum(n)]
+    kept = B.kv8_evict(d.codes, d.scales, d.mass, i32(starts), i32(tables[0]), i32(tables[1]), i32(dst[0]), i32(dst[1]), budget, 4, 16)
+    assert np.array_equal(kept.cpu().numpy(), R.evict(codes, scales, fmt, dim, mass, list(starts), tables, dst, budget, 4, 16))
+    same(d, c, codes, scales)
+    assert np.array_equal(d.mass.cpu().numpy(), mass)
+    tables, starts[:] = dst, [min(x, budget) for x in starts]
+    for _ in range(4):
+        step(0.9)
+
+
+def test_a_captured_step_replays_with_other_tables():
+    """append, attention with weights: captured once, replayed as the sequences grow, against the same calls outside the graph"""
+    kv, H, dim = 2, 8, 128
+    c = Cache([30, 200, 0], [1, 1, 1], kv, dim, "e4m3", seed=12, pages=60, dirty=False, extra=2)
+    a, b = c.device(), c.device()
+    k, q = torch.randn(3, kv, dim, device="cuda").bfloat16(), torch.randn(3, H, dim, device="cuda").bfloat16()
+    out = torch.zeros_like(q)
+
+    def step(d, out):
+        B.kv8_append(k, k, d.codes, d.scales, d.row0, d.starts, d.indptr, d.ids, max_rows=1)
+        B.kv8_attention(q, d.codes, d.scales, d.row0, d.starts, d.indptr, d.ids, 0.1, max_rows=1, max_len=256, out=out, mass=d.mass)
+
+    warm = c.device()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(warm, out)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(a, out)
+    for i in range(4):
+        k.copy_(torch.randn(3, kv, dim, device="cuda") * (i + 1))
+        q.copy_(torch.randn(3, H, dim, device="cuda"))
+        graph.replay()
+        eager = torch.zeros_like(q)
+        step(b, eager)
+        torch.cuda.synchronize()
+        assert torch.equal(out, eager) and torch.equal(a.pool, b.pool) and torch.equal(a.scales, b.scales) and torch.equal(a.mass, b.mass), i
+        for d in (a, b):
+            d.starts += 1
+
+
+def test_two_streams_at_once():
+    """the same operators on two streams, each with its cache: workspaces are not shared"""
+    c = [Cache([700, 30], [1, 20], 2, 128, f, seed=s) for s, f in enumerate(TORCH)]
+    d = [x.device() for x in c]
+    q = torch.randn(21, 8, 128, device="cuda").bfloat16()
+    run = lambda x: B.kv8_attention(q, x.codes, x.scales, x.row0, x.starts, x.indptr, x.ids, 0.1, mass=x.mass, mass_keep=0.0)  # noqa: E731
+    want = [(run(x).clone(), x.mass.clone()) for x in d]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in d]
+    for _ in range(5):
+        got = []
+        for x, s in zip(d, streams):
+            with torch.cuda.stream(s):
+                got.append(run(x))
+        torch.cuda.synchronize()
+        for x, g, w in zip(d, got, want):
+            assert torch.equal(g, w[0]) and torch.equal(x.mass, w[1])
+
+
+def test_a_cache_that_passes_32_bits():
+    """pages 96 MiB apart: the last ones lie 4.5 GiB behind the first"""
+    kv, dim, pages, apart = 2, 128, 48, 96 << 20
+    c = Cache([200, 100], [1, 3], kv, dim, "int8", seed=13, pages=pages, dirty=False)
+    d = c.device()
+    pool = torch.empty(pages * apart, dtype=torch.int8, device="cuda")
+    codes = pool.as_strided((pages, 2, kv, 16 * dim), (apart, kv * 16 * dim, 16 * dim, 1))
+    codes.copy_(d.codes)
+    d.codes = codes
+    k, kd = rows_of(c.rng, 4, kv, dim, torch.bfloat16)
+    R.append(k, k, c.codes, c.scales, "int8", c.row0, c.starts, c.tables)
+    B.kv8_append(kd, kd, d.codes, d.scales, d.row0, d.starts, d.indptr, d.ids)
+    assert np.array_equal(codes.cpu().numpy().view(np.uint8), c.codes) and np.array_equal(d.scales.cpu().numpy(), c.scales)
+    attend(c, 4, torch.bfloat16, weigh=True, d=d)
+
+
+def test_wrappers_refuse():
+    c = Cache([20], [4], 2, 64, "e4m3")
+    d = c.device()
+    q = torch.zeros(4, 4, 64, dtype=torch.bfloat16, device="cuda")
+    k = torch.zeros(4, 2, 64, dtype=torch.bfloat16, device="cuda")
+    t = (d.row0, d.starts, d.indptr, d.ids)
+    go = lambda **kw: B.kv8_attention(**{**dict(q=q, codes=d.codes, scales=d.scales, row0=d.row0, starts=d.starts, page_indptr=d.indptr, page_ids=d.ids, scale=1.0), **kw})  # noqa: E731
+    assert go().shape == q.shape
+    for kw in [dict(q=q.half()), dict(q=q.float()[..., ::2]), dict(q=q[:, :3]), dict(q=q[..., :32]), dict(q=q.cpu()), dict(q=q.transpose(0, 1)), dict(codes=d.pool[:, -1]),
+               dict(codes=d.codes[..., :1000]), dict(codes=d.codes.cpu()), dict(scales=d.scales[:-1]), dict(scales=d.scales.double()), dict(row0=d.row0.long()), dict(row0=d.row0.cpu()),
+               dict(starts=d.indptr), dict(page_indptr=d.starts), dict(out=q.float()), dict(out=q[:2]), dict(mass=d.mass[..., :8]), dict(mass=d.mass.double()),
+               dict(mass_out=d.mass), dict(page_ids=d.ids[None]), dict(max_rows=-1), dict(max_len=-1)]:
+        with pytest.raises((ValueError, RuntimeError)):
+            go(**kw)
+    with pytest.raises(ValueError):
+        B.kv8_append(k, k.float(), d.codes, d.scales, *t)
+    with pytest.raises(ValueError):
+        B.kv8_append(k[:, :1], k[:, :1], d.codes, d.scales, *t)
+    with pytest.raises(ValueError):
+        B.kv8_read(d.codes, d.scales, *t, 4, dtype=torch.float16)
+    for budget, first, last in [(0, 0, 0), (8, 5, 4), (8, -1, 0)]:
+        with pytest.raises(ValueError):
+            B.kv8_evict(d.codes, d.scales, d.mass, d.lens, d.indptr, d.ids, d.indptr, d.ids, budget, first, last)
+    none = torch.zeros(0, 4, 64, dtype=torch.bfloat16, device="cuda")
+    zero = torch.zeros(1, dtype=torch.int32, device="cuda")
+    assert B.kv8_attention(none, d.codes, d.scales, zero, zero[:0], zero, d.ids, 1.0).shape == (0, 4, 64)      # no entries
