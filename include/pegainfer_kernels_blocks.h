@@ -1100,13 +1100,13 @@ pegainfer_status_t pegainfer_kv8_append(const pegainfer_kv8_cache* cache, const 
 pegainfer_status_t pegainfer_kv8_read(const pegainfer_kv8_cache* cache, const int32_t* row0, const int32_t* starts, void* k, void* v, int32_t n_rows, int32_t max_rows,
                                       int32_t dtype, pegainfer_stream_t stream);
 /* Causal softmax attention: row i of entry e sees the slots up to starts[e] + i (its own token is in the cache already), query head h reads kv head
- * h / (heads / kv_heads);  out[row, h] = sum_j softmax_j(scale q . k_j) v_j, zeros where a row sees nothing.  q, out: rows [heads][dim] of dtype at strides of
+ * h / (heads / kv_heads);  scale >= 0;  out[row, h] = sum_j softmax_j(scale q . k_j) v_j, zeros where a row sees nothing.  q, out: rows [heads][dim] of dtype at strides of
  * 16 bytes.  Scores, softmax state and sums are fp32; bf16: the softmax weights are rounded to bf16 where they enter the matrix cores (their sum is not); fp32:
  * queries and weights enter as three bf16 parts, nothing is rounded.
  * mass_out given: mass_out[page][kv head][16] (fp32, pages mass_out_page_stride values apart) = mass_keep * mass + the weight that the call's rows and the kv
  * head's query heads gave to the token, for every slot of an entry that has rows (mass_out may be mass; mass_keep 0: mass is not read and may be NULL).  Every
  * sum has one order: results do not change from run to run.
- * workspace: fp32 scratch of pegainfer_kv8_attention_workspace(...) values, of this call alone until it is done. */
+ * workspace: fp32 scratch on 16 bytes of pegainfer_kv8_attention_workspace(...) values, of this call alone until it is done (0: NULL). */
 typedef struct {
   const void* q;
   int64_t q_row_stride;
@@ -1123,7 +1123,8 @@ typedef struct {
   float* workspace;
   int32_t dtype;
 } pegainfer_kv8_attn_desc;
-int64_t pegainfer_kv8_attention_workspace(int32_t n_rows, int32_t heads, int32_t with_mass);
+int64_t pegainfer_kv8_attention_workspace(int32_t n_rows, int32_t max_rows, int32_t max_len, int32_t heads, int32_t kv_heads, int32_t dim, int32_t n_entries,
+                                          int32_t with_mass);
 pegainfer_status_t pegainfer_kv8_attention(const pegainfer_kv8_cache* cache, const pegainfer_kv8_attn_desc* d, pegainfer_stream_t stream);
 /* Entries of lens[e] tokens are cut to `budget`: every kv head by itself keeps its first keep_first, its last keep_last and of those between the ones of the
  * largest mass (equal: the lowest slots; NaN below everything), in their order, in the pages dst_ids[dst_indptr[e]] .. - pages of their own, none of which the

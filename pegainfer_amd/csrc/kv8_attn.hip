@@ -19,151 +19,275 @@ struct AttnArgs {
   const void* q;
   int64_t q_stride, out_stride;
   const int32_t *row0, *starts;
-  int n_rows, group, heads;
+  int n_rows, group, heads, n_split, split_blocks;
   float scale_log2;
   void* out;
   float* lse;            // [n_rows][heads], log2 of the sum of exp(scores); NULL: not wanted
+  float *part_o, *part_ml;   // n_split > 1: [n_rows][heads][n_split][D] and [2] (running maximum, sum)
 };
 
-// the queries' rows of a kv head, (token, head of the group) in order; row n of a tile of sixteen is the lane's
-struct QueryRow { int row, head, far; };   // far: the last slot that it sees; -1: no such row
+// the queries' rows of a kv head, (token, head of the group) in order; a row behind the last is the last again
+struct QueryRow { int row, head, far; bool real; };   // far: the last slot that it sees
 __device__ __forceinline__ QueryRow query_row(int rr, int total, int group, const RowSpan& rows, int start, int kv_head) {
-  if (rr >= total) return {rows.first, kv_head * group, -1};
-  const int tok = rr / group;
-  return {rows.first + tok, kv_head * group + rr - tok * group, start + tok};
+  const int r = min(rr, total - 1), tok = r / group;
+  return {rows.first + tok, kv_head * group + r - tok * group, start + tok, rr < total};
 }
 
-// One workgroup of four waves: sixteen query rows of a kv head, the blocks of keys in pairs dealt to the waves, whose states meet in shared memory at the end.
-// Scores are computed transposed (keys x rows), so that a lane holds four keys' scores of one row: exactly what the second product wants from it.
-template <typename T, int FMT, int D>
+// One workgroup of four waves: NT tiles of sixteen query rows of a kv head over a run of key blocks.  The blocks are dealt to the waves KB at a time, whose states
+// meet in shared memory at the end, so that no key is loaded or widened twice in a workgroup.  Scores are computed transposed (keys x rows): a lane then holds four
+// keys' scores of one row, exactly what the second product wants from it.  The next keys are on their way while the weights are made, the next values while
+// the next scores are.
+template <typename T, int FMT, int D, int NT, int KB>
 __global__ __launch_bounds__(256) void kv8_attn_kernel(AttnArgs a) {
   constexpr int NP = kv8_parts<T>(), C = D / 64;
+  constexpr bool kScaled = FMT == kE4m3;   // the conversion takes the block's scale along; int8 scales scores and weights instead
   __shared__ f32x4 s_o[2][D / 16][64];
   __shared__ float s_m[2][16], s_l[2][16];
-  const int e = blockIdx.z, head = blockIdx.y, wave = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+  const int e = blockIdx.z, head = blockIdx.y, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   const RowSpan rows = row_span(a.row0, e, a.n_rows);
   const int start = a.starts[e], total = rows.n * a.group;
-  if (start < 0 || start > INT32_MAX - 32 - rows.n) return;
-  const int len = start + rows.n;
-  for (int tile = blockIdx.x; tile * 16 < total; tile += gridDim.x) {
-    const QueryRow r = query_row(tile * 16 + n, total, a.group, rows, start, head);
-    bf16x8_t qf[C][2][NP];
-    const T* qp = static_cast<const T*>(a.q) + r.row * a.q_stride + (int64_t)r.head * D + g * 16;
+  if (rows.n == 0 || start < 0 || start > INT32_MAX - 2048 - rows.n) return;
+  const int len = start + rows.n, n_tiles = (total + 16 * NT - 1) / (16 * NT), split = blockIdx.x % a.n_split, step = gridDim.x / a.n_split;
+  for (int at = blockIdx.x / a.n_split; at < n_tiles; at += step) {
+    const int tile = n_tiles - 1 - at;     // the rows that see most first
+    QueryRow r[NT];
+    bf16x8_t qf[NT][C][2][NP];
+    float m[NT], l[NT];
+    f32x4 o[NT][D / 16];
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-      kv8_query(qp + c * 64, qf[c][0]);
-      kv8_query(qp + c * 64 + 8, qf[c][1]);
+    for (int t = 0; t < NT; ++t) {
+      r[t] = query_row((tile * NT + t) * 16 + n, total, a.group, rows, start, head);
+      const T* qp = static_cast<const T*>(a.q) + r[t].row * a.q_stride + (int64_t)r[t].head * D + g * 16;
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        kv8_query(qp + c * 64, qf[t][c][0]);
+        kv8_query(qp + c * 64 + 8, qf[t][c][1]);
+      }
+      m[t] = -INFINITY;
+      l[t] = 0.f;
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) o[t][i] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    const int last = min(tile * 16 + 15, total - 1) / a.group + start;   // the last slot that any row of the tile sees
-    const int blocks = last / kKv8Page + 1;
-    float m = -INFINITY, l = 0.f;
-    f32x4 o[D / 16];
+    // slots that every row of the tiles sees, and that any does
+    const int all_see = tile * NT * 16 / a.group + start, any_sees = min((tile + 1) * NT * 16 - 1, total - 1) / a.group + start;
+    const int blocks = any_sees / kKv8Page + 1, per = max(a.split_blocks, (blocks + a.n_split - 1) / a.n_split);
+    const int b_lo = split * per, b_hi = min(blocks, b_lo + per);
+    for (int run = b_lo; run < b_hi; run += 64) {
+      // lane i: the run's block i
+      const int pid = run + lane < b_hi ? a.c.page(e, run + lane) : -1;
+      const float ks = pid < 0 ? 0.f : *a.c.scale(pid, 0, head), vs = pid < 0 ? 0.f : *a.c.scale(pid, 1, head);
+      const uint64_t there = __builtin_amdgcn_ballot_w64(pid >= 0);
+      const int groups = (min(b_hi - run, 64) + KB - 1) / KB;
+      u32x4 kw[KB][C], vw[KB][C];
+      auto load = [&](int side, int i, u32x4 (&w)[KB][C]) {
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int b = 2 * wave; b < blocks; b += 8) {
-      f32x4 s[2];
-      int page[2];
-      float vs[2];
+        for (int h = 0; h < KB; ++h) {
+          const int page = max(__builtin_amdgcn_readlane(pid, i * KB + h), 0);     // one that is not there: page 0's bytes, masked below
+          const uint8_t* p = a.c.block(page, side, head, D) + (side == 0 ? n * 64 + g * 16 : g * 256 + n * 16);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        page[h] = b + h < blocks ? a.c.page(e, b + h) : -1;
-        s[h] = f32x4{0.f, 0.f, 0.f, 0.f};
-        vs[h] = 0.f;
-        if (page[h] >= 0) {
-          const uint8_t* kb = a.c.block(page[h], 0, head, D) + n * 64 + g * 16;
+          for (int c = 0; c < C; ++c) w[h][c] = *reinterpret_cast<const u32x4*>(p + c * 1024);
+        }
+      };
+      auto lane_of = [](float v, int i) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), i)); };
+      if (wave < groups) {
+        load(0, wave, kw);
+        load(1, wave, vw);
+      }
+      for (int i = wave; i < groups; i += 4) {
+        const int slot0 = (run + i * KB) * kKv8Page;
+        f32x4 s[NT][KB];
+#pragma unroll
+        for (int h = 0; h < KB; ++h) {
+#pragma unroll
+          for (int t = 0; t < NT; ++t) s[t][h] = f32x4{0.f, 0.f, 0.f, 0.f};
+          const float kscale = lane_of(ks, i * KB + h);
 #pragma unroll
           for (int c = 0; c < C; ++c) {
-            const u32x4 w = *reinterpret_cast<const u32x4*>(kb + c * 1024);
-            const bf16x8_t k0 = kv8_operand<FMT>(w.x, w.y), k1 = kv8_operand<FMT>(w.z, w.w);
+            const bf16x8_t k0 = kv8_operand<FMT>(kw[h][c].x, kw[h][c].y, kscale), k1 = kv8_operand<FMT>(kw[h][c].z, kw[h][c].w, kscale);
 #pragma unroll
-            for (int p = NP - 1; p >= 0; --p) {
-              s[h] = mfma16(k0, qf[c][0][p], s[h]);
-              s[h] = mfma16(k1, qf[c][1][p], s[h]);
-            }
+            for (int p = NP - 1; p >= 0; --p)
+#pragma unroll
+              for (int t = 0; t < NT; ++t) {
+                s[t][h] = mfma16(k0, qf[t][c][0][p], s[t][h]);
+                s[t][h] = mfma16(k1, qf[t][c][1][p], s[t][h]);
+              }
           }
-          const float ks = *a.c.scale(page[h], 0, head) * a.scale_log2;
-          vs[h] = *a.c.scale(page[h], 1, head);
+          const float f = kScaled ? a.scale_log2 : kscale * a.scale_log2;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) s[h][i] = (b + h) * kKv8Page + 4 * g + i <= r.far ? s[h][i] * ks : -INFINITY;
+          for (int t = 0; t < NT; ++t) s[t][h] *= f;
+        }
+        if (i + 4 < groups) load(0, i + 4, kw);
+        const uint64_t want = ((1ull << KB) - 1) << (i * KB);
+        const bool ragged = slot0 + KB * kKv8Page - 1 > all_see || (there & want) != want;
+        if (ragged) {
+#pragma unroll
+          for (int h = 0; h < KB; ++h) {
+            const int end = there >> (i * KB + h) & 1 ? INT32_MAX : -1, at0 = slot0 + h * kKv8Page + 4 * g;
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) s[t][h][j] = at0 + j <= min(r[t].far, end) ? s[t][h][j] : -INFINITY;
+            // what lies behind the entry's last token may be any bytes, and 0 times one of them a NaN
+            const int here = min(len, end) - at0;
+            const uint32_t bytes = here >= 4 ? 0xFFFFFFFFu : here <= 0 ? 0u : 0xFFFFFFFFu >> (32 - 8 * here);
+#pragma unroll
+            for (int c = 0; c < C; ++c) vw[h][c] &= bytes;
+          }
+        }
+        bf16x8_t pf[NT][KB / 2][NP];
+        float alpha[NT];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          float mx = m[t];
+#pragma unroll
+          for (int h = 0; h < KB; ++h)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) mx = fmaxf(mx, s[t][h][j]);
+          mx = quad_max(mx);
+          const float base = mx == -INFINITY ? 0.f : mx;
+          alpha[t] = exp2_of(m[t] - base);
+          m[t] = mx;
+          l[t] *= alpha[t];
+#pragma unroll
+          for (int h = 0; h < KB; h += 2) {
+            float p[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              p[j] = exp2_of(s[t][h + j / 4][j & 3] - base);
+              l[t] += p[j];
+              if (!kScaled) p[j] *= lane_of(vs, i * KB + h + j / 4);
+            }
+            kv8_split<NP>(p, pf[t][h / 2]);
+          }
+        }
+        // fp32 sums of many keys are added outside the matrix cores, whose accumulation does not round to nearest
+        constexpr bool kOutside = NP > 1;
+        if (!kOutside) {
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+            if (__builtin_amdgcn_ballot_w64(alpha[t] != 1.f))
+#pragma unroll
+              for (int d = 0; d < D / 16; ++d) o[t][d] *= alpha[t];
+        }
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            f32x4 x[NT];
+#pragma unroll
+            for (int t = 0; t < NT; ++t) x[t] = kOutside ? f32x4{0.f, 0.f, 0.f, 0.f} : o[t][4 * c + j];
+#pragma unroll
+            for (int h = 0; h < KB; h += 2) {
+              const bf16x8_t vf = kv8_operand2<FMT>(vw[h][c][j], vw[h + 1][c][j], lane_of(vs, i * KB + h), lane_of(vs, i * KB + h + 1));
+#pragma unroll
+              for (int k = NP - 1; k >= 0; --k)
+#pragma unroll
+                for (int t = 0; t < NT; ++t) x[t] = mfma16(vf, pf[t][h / 2][k], x[t]);
+            }
+#pragma unroll
+            for (int t = 0; t < NT; ++t) o[t][4 * c + j] = kOutside ? o[t][4 * c + j] * alpha[t] + x[t] : x[t];
+          }
+        if (i + 4 < groups) load(1, i + 4, vw);
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      l[t] = quad_sum(l[t]);
+      // four states into one: waves 2, 3 into 0, 1, then 1 into 0
+#pragma unroll
+      for (int half = 2; half >= 1; half >>= 1) {
+        __syncthreads();
+        if (wave >= half && wave < 2 * half) {
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i) s_o[wave - half][i][lane] = o[t][i];
+          if (g == 0) { s_m[wave - half][n] = m[t]; s_l[wave - half][n] = l[t]; }
+        }
+        __syncthreads();
+        if (wave < half) {
+          const float mo = s_m[wave][n], both = fmaxf(m[t], mo), base = both == -INFINITY ? 0.f : both;
+          const float x = exp2_of(m[t] - base), y = exp2_of(mo - base);
+          m[t] = both;
+          l[t] = l[t] * x + s_l[wave][n] * y;
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i) o[t][i] = o[t][i] * x + s_o[wave][i][lane] * y;
+        }
+      }
+      if (wave == 0 && r[t].real) {
+        const bool some = l[t] > 0.f || l[t] != l[t];
+        const float inv = a.n_split > 1 ? 1.f : some ? 1.f / l[t] : 0.f;   // no key: zeros
+        const int64_t rh = (int64_t)r[t].row * a.heads + r[t].head;
+        auto put = [&](auto* op) {
+          using O = std::remove_pointer_t<decltype(op)>;
+#pragma unroll
+          for (int c = 0; c < C; ++c) {
+            float x[16];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) x[4 * i + j] = o[t][4 * c + j][i] * inv;
+            Vec8<O>::store(op + g * 16 + c * 64, x);
+            Vec8<O>::store(op + g * 16 + c * 64 + 8, x + 8);
+          }
+        };
+        if (a.n_split > 1) {
+          if (some) put(a.part_o + (rh * a.n_split + split) * D);
+          if (g == 0) *reinterpret_cast<f32x2*>(a.part_ml + (rh * a.n_split + split) * 2) = f32x2{m[t], l[t]};
         } else {
-          s[h] = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        }
-      }
-      float mx = m;
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[h][i]);
-      mx = quad_max(mx);
-      const float base = mx == -INFINITY ? 0.f : mx, alpha = exp2_of(m - base);
-      m = mx;
-      l *= alpha;
-      float p[8];
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          p[4 * h + i] = exp2_of(s[h][i] - base);
-          l += p[4 * h + i];
-          p[4 * h + i] *= vs[h];
-        }
-      bf16x8_t pf[NP];
-      kv8_split<NP>(p, pf);
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i) o[i] *= alpha;
-#pragma unroll
-      for (int c = 0; c < C; ++c) {
-        u32x4 w[2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          w[h] = u32x4{0, 0, 0, 0};
-          if (page[h] >= 0) w[h] = *reinterpret_cast<const u32x4*>(a.c.block(page[h], 1, head, D) + c * 1024 + g * 256 + n * 16);
-          // what lies behind the entry's last token may be any bytes, and 0 times one of them a NaN
-          const int there = len - ((b + h) * kKv8Page + 4 * g);
-          if (there < 4) w[h] &= there <= 0 ? 0u : 0xFFFFFFFFu >> (32 - 8 * there);
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const bf16x8_t vf = kv8_operand<FMT>(w[0][j], w[1][j]);
-#pragma unroll
-          for (int k = NP - 1; k >= 0; --k) o[4 * c + j] = mfma16(vf, pf[k], o[4 * c + j]);
+          put(static_cast<T*>(a.out) + r[t].row * a.out_stride + (int64_t)r[t].head * D);
+          if (a.lse && g == 0) a.lse[rh] = some ? m[t] + __log2f(l[t]) : INFINITY;
         }
       }
     }
-    l = quad_sum(l);
-    // four states into one: waves 2, 3 into 0, 1, then 1 into 0
+    __syncthreads();
+  }
+}
+
+// The splits' states of a (row, head) into its output: a workgroup each, every wave takes every W-th split.
+template <typename T, int D>
+__global__ __launch_bounds__(512) void kv8_merge_kernel(AttnArgs a) {
+  constexpr int V = D / 64;
+  __shared__ float s_o[8][D], s_l[8];
+  const int e = blockIdx.z, head = blockIdx.y, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, lane = threadIdx.x & 63;
+  const RowSpan rows = row_span(a.row0, e, a.n_rows);
+  const int start = a.starts[e], total = rows.n * a.group;
+  if (rows.n == 0 || start < 0 || start > INT32_MAX - 2048 - rows.n) return;
+  for (int rr = blockIdx.x; rr < total; rr += gridDim.x) {
+    const QueryRow r = query_row(rr, total, a.group, rows, start, head);
+    const int64_t rh = (int64_t)r.row * a.heads + r.head;
+    const f32x2* ml = reinterpret_cast<const f32x2*>(a.part_ml) + rh * a.n_split;
+    float m = -INFINITY;
+    for (int i = lane; i < a.n_split; i += 64) m = fmaxf(m, ml[i].x);
+    m = wave_max(m);
+    const float base = m == -INFINITY ? 0.f : m;
+    float l = 0.f, o[V];
 #pragma unroll
-    for (int half = 2; half >= 1; half >>= 1) {
-      __syncthreads();
-      if (wave >= half && wave < 2 * half) {
+    for (int v = 0; v < V; ++v) o[v] = 0.f;
+#pragma unroll 4
+    for (int i = wave; i < a.n_split; i += waves) {
+      const f32x2 x = ml[i];
+      if (!(x.y > 0.f || x.y != x.y)) continue;             // a split without a key left no sums
+      const float w = exp2_of(x.x - base);
+      l += x.y * w;
+      const float* p = a.part_o + (rh * a.n_split + i) * D + lane * V;
 #pragma unroll
-        for (int i = 0; i < D / 16; ++i) s_o[wave - half][i][lane] = o[i];
-        if (g == 0) { s_m[wave - half][n] = m; s_l[wave - half][n] = l; }
-      }
-      __syncthreads();
-      if (wave < half) {
-        const float mo = s_m[wave][n], both = fmaxf(m, mo), base = both == -INFINITY ? 0.f : both;
-        const float x = exp2_of(m - base), y = exp2_of(mo - base);
-        m = both;
-        l = l * x + s_l[wave][n] * y;
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i) o[i] = o[i] * x + s_o[wave][i][lane] * y;
-      }
+      for (int v = 0; v < V; ++v) o[v] += w * p[v];
     }
-    if (wave == 0 && r.far >= 0) {
-      const float inv = l > 0.f || l != l ? 1.f / l : 0.f;   // no key: zeros
-      T* op = static_cast<T*>(a.out) + r.row * a.out_stride + (int64_t)r.head * D + g * 16;
+    if (lane == 0) s_l[wave] = l;
 #pragma unroll
-      for (int c = 0; c < C; ++c) {
-        float x[16];
+    for (int v = 0; v < V; ++v) s_o[wave][lane * V + v] = o[v];
+    __syncthreads();
+    if (wave == 0) {
+      for (int w = 1; w < waves; ++w) {
+        l += s_l[w];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) x[4 * i + j] = o[4 * c + j][i] * inv;
-        Vec8<T>::store(op + c * 64, x);
-        Vec8<T>::store(op + c * 64 + 8, x + 8);
+        for (int v = 0; v < V; ++v) o[v] += s_o[w][lane * V + v];
       }
-      if (a.lse && g == 0) a.lse[(int64_t)r.row * a.heads + r.head] = l > 0.f || l != l ? m + __log2f(l) : INFINITY;
+      const bool some = l > 0.f || l != l;
+      const float inv = some ? 1.f / l : 0.f;
+      T* op = static_cast<T*>(a.out) + r.row * a.out_stride + (int64_t)r.head * D + lane * V;
+#pragma unroll
+      for (int v = 0; v < V; ++v) st(op + v, o[v] * inv);
+      if (a.lse && lane == 0) a.lse[rh] = some ? m + __log2f(l) : INFINITY;
     }
     __syncthreads();
   }
@@ -177,7 +301,7 @@ __global__ __launch_bounds__(256) void kv8_mass_kernel(AttnArgs a, const float* 
   const int e = blockIdx.z, head = blockIdx.y, wave = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   const RowSpan rows = row_span(a.row0, e, a.n_rows);
   const int start = a.starts[e], total = rows.n * a.group;
-  if (rows.n == 0 || start < 0 || start > INT32_MAX - 32 - rows.n) return;
+  if (rows.n == 0 || start < 0 || start > INT32_MAX - 2048 - rows.n) return;
   const int len = start + rows.n;
   for (int b = blockIdx.x * 4 + wave; b * kKv8Page < len; b += gridDim.x * 4) {
     const int page = a.c.page(e, b);
@@ -210,7 +334,7 @@ __global__ __launch_bounds__(256) void kv8_mass_kernel(AttnArgs a, const float* 
       }
       const float lse = a.lse[(int64_t)r.row * a.heads + r.head];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) sum[i] += b * kKv8Page + 4 * g + i <= r.far ? exp2_of(s[i] * ks - lse) : 0.f;
+      for (int i = 0; i < 4; ++i) sum[i] += r.real && b * kKv8Page + 4 * g + i <= r.far ? exp2_of(s[i] * ks - lse) : 0.f;
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -225,18 +349,37 @@ __global__ __launch_bounds__(256) void kv8_mass_kernel(AttnArgs a, const float* 
   }
 }
 
+// How a call is cut: rows of a workgroup, and splits of the keys where that leaves too few workgroups.
+struct AttnPlan { int tiles, row_tiles, n_split, split_blocks; };
+inline AttnPlan attn_plan(int n_rows, int max_rows, int max_len, int group, int kv_heads, int entries) {
+  AttnPlan p;
+  const int64_t rows = (int64_t)std::min(max_rows, n_rows) * group;
+  p.row_tiles = rows > 16 ? 2 : 1;
+  p.tiles = ceil_div(rows, 16 * p.row_tiles);
+  const int blocks = std::max(1, ceil_div(max_len, kKv8Page));
+  const int64_t groups = (int64_t)p.tiles * kv_heads * entries, want = 8 * device_cus();
+  p.n_split = (int)std::min<int64_t>({(want + groups - 1) / groups, (blocks + 15) / 16, 256});
+  p.split_blocks = ceil_div(blocks, p.n_split);
+  return p;
+}
+
 }  // namespace pk
 
 using namespace pk;
 
 extern "C" {
 
-int64_t pegainfer_kv8_attention_workspace(int32_t n_rows, int32_t heads, int32_t with_mass) {
-  return with_mass ? (int64_t)std::max(n_rows, 0) * std::max(heads, 0) : 0;
+int64_t pegainfer_kv8_attention_workspace(int32_t n_rows, int32_t max_rows, int32_t max_len, int32_t heads, int32_t kv_heads, int32_t dim, int32_t n_entries,
+                                          int32_t with_mass) {
+  if (n_rows <= 0 || max_rows <= 0 || kv_heads < 1 || heads < kv_heads || n_entries <= 0) return 0;
+  const AttnPlan p = attn_plan(n_rows, max_rows, max_len, heads / kv_heads, kv_heads, n_entries);
+  const int64_t rh = (int64_t)n_rows * heads;
+  return (p.n_split > 1 ? rh * p.n_split * (dim + 2) : 0) + (with_mass ? rh : 0);
 }
 
 pegainfer_status_t pegainfer_kv8_attention(const pegainfer_kv8_cache* cache, const pegainfer_kv8_attn_desc* d, pegainfer_stream_t stream) {
-  if (!kv8_ok(cache) || !d || (d->dtype != kDtBf16 && d->dtype != kDtF32) || d->heads < 1 || d->heads % cache->kv_heads || d->n_rows < 0 || d->max_rows < 0 || d->max_len < 0)
+  if (!kv8_ok(cache) || !d || (d->dtype != kDtBf16 && d->dtype != kDtF32) || d->heads < 1 || d->heads % cache->kv_heads || d->n_rows < 0 || d->max_rows < 0 || d->max_len < 0 ||
+      !(d->scale >= 0.f))
     return PK_BAD;
   if (d->n_rows == 0 || d->max_rows == 0 || cache->n_entries == 0) return 0;
   const int64_t width = (int64_t)d->heads * cache->dim, unit = d->dtype == kDtBf16 ? 8 : 4;
@@ -246,19 +389,24 @@ pegainfer_status_t pegainfer_kv8_attention(const pegainfer_kv8_cache* cache, con
   const bool weigh = d->mass_out != nullptr;
   const int64_t mass_width = (int64_t)cache->kv_heads * kKv8Page;
   if (weigh && (d->mass_out_page_stride < mass_width || (d->mass_keep != 0.f && (!d->mass || d->mass_page_stride < mass_width)))) return PK_BAD;
-  if (pegainfer_kv8_attention_workspace(d->n_rows, d->heads, weigh) > 0 && !d->workspace) return PK_BAD;
-  const Kv8 c = kv8_of(cache);
   const int group = d->heads / cache->kv_heads;
-  const AttnArgs a{c, d->q, d->q_row_stride, d->out_row_stride, d->row0, d->starts, d->n_rows, group, d->heads, d->scale * 1.4426950408889634f, d->out,
-                   weigh ? d->workspace : nullptr};
-  const int rows = std::min(d->max_rows, d->n_rows);
-  const dim3 grid(ceil_div((int64_t)rows * group, 16), c.kv_heads, c.entries);
-  const dim3 mass_grid(std::max(1, ceil_div(d->max_len, 4 * kKv8Page)), c.kv_heads, c.entries);
+  const AttnPlan p = attn_plan(d->n_rows, d->max_rows, d->max_len, group, cache->kv_heads, cache->n_entries);
+  if ((weigh || p.n_split > 1) && (!d->workspace || !host_aligned16(d->workspace))) return PK_BAD;
+  const int64_t rh = (int64_t)d->n_rows * d->heads;
+  float* part_ml = d->workspace + (p.n_split > 1 ? rh * p.n_split * cache->dim : 0);
+  const AttnArgs a{kv8_of(cache), d->q, d->q_row_stride, d->out_row_stride, d->row0, d->starts, d->n_rows, group, d->heads, p.n_split, p.split_blocks,
+                   d->scale * 1.4426950408889634f, d->out, weigh ? part_ml + (p.n_split > 1 ? rh * p.n_split * 2 : 0) : nullptr, d->workspace, part_ml};
+  const dim3 grid(p.tiles * p.n_split, cache->kv_heads, cache->n_entries);
+  const dim3 merge_grid(std::min(d->max_rows, d->n_rows) * group, cache->kv_heads, cache->n_entries);
+  const dim3 mass_grid(std::max(1, ceil_div(d->max_len, 4 * kKv8Page)), cache->kv_heads, cache->n_entries);
   kv8_by(d->dtype, cache->format, cache->dim, [&](auto* t, auto fmt, auto dim) {
     using T = std::remove_pointer_t<decltype(t)>;
-    kv8_attn_kernel<T, fmt(), dim()><<<grid, 256, 0, as_stream(stream)>>>(a);
+    constexpr int D = dim(), KB = D == 256 ? 2 : 4;
+    if (p.row_tiles == 1) kv8_attn_kernel<T, fmt(), D, 1, KB><<<grid, 256, 0, as_stream(stream)>>>(a);
+    else kv8_attn_kernel<T, fmt(), D, 2, KB><<<grid, 256, 0, as_stream(stream)>>>(a);
+    if (p.n_split > 1) kv8_merge_kernel<T, D><<<merge_grid, 64 * std::min(8, p.n_split), 0, as_stream(stream)>>>(a);
     if (weigh)
-      kv8_mass_kernel<T, fmt(), dim()><<<mass_grid, 256, 0, as_stream(stream)>>>(a, d->mass, d->mass_page_stride, d->mass_out, d->mass_out_page_stride, d->mass_keep);
+      kv8_mass_kernel<T, fmt(), D><<<mass_grid, 256, 0, as_stream(stream)>>>(a, d->mass, d->mass_page_stride, d->mass_out, d->mass_out_page_stride, d->mass_keep);
   });
   return (pegainfer_status_t)hipGetLastError();
 }

@@ -89,16 +89,16 @@ __device__ __forceinline__ uint32_t kv8_codes(const float* x) {
     return w;
   }
 }
-// eight codes as a bf16 operand (every code is a bf16 number)
+// eight codes as a bf16 operand (every code is a bf16 number): e4m3 times a scale for each four, which the conversion multiplies by on its way; int8 as they are
 template <int FMT>
-__device__ __forceinline__ bf16x8_t kv8_operand(uint32_t lo, uint32_t hi) {
+__device__ __forceinline__ bf16x8_t kv8_operand2(uint32_t lo, uint32_t hi, float scale_lo, float scale_hi) {
   typedef __attribute__((ext_vector_type(4))) uint32_t w4;
   w4 o;
   if constexpr (FMT == kE4m3) {
-    o.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, false));
-    o.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, true));
-    o.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, false));
-    o.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, true));
+    o.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale_lo, false));
+    o.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale_lo, true));
+    o.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale_hi, false));
+    o.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale_hi, true));
   } else {
     float a[4], b[4];
     kv8_numbers<FMT>(lo, a);
@@ -108,6 +108,9 @@ __device__ __forceinline__ bf16x8_t kv8_operand(uint32_t lo, uint32_t hi) {
   }
   return __builtin_bit_cast(bf16x8_t, o);
 }
+
+template <int FMT>
+__device__ __forceinline__ bf16x8_t kv8_operand(uint32_t lo, uint32_t hi, float scale = 1.f) { return kv8_operand2<FMT>(lo, hi, scale, scale); }
 
 // A query or a weight as a sum of bf16 operands: itself where it is bf16 (a weight: rounded to it), in three parts where it is fp32 (24 bits: nothing lost)
 template <typename T> constexpr int kv8_parts() { return sizeof(T) == 2 ? 1 : 3; }

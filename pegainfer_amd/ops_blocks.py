@@ -964,6 +964,7 @@ def _kv8_cache(codes, scales, page_indptr, page_ids, entries):
     _kv8_need(codes.dtype in KV8_FORMATS, "codes of torch.float8_e4m3fn or torch.int8")
     _kv8_need(codes.is_cuda and codes.device.index == torch.cuda.current_device(), "a cache on the current device")
     _kv8_need(codes.dim() == 4 and codes.shape[1] == 2 and codes.shape[3] in (1024, 2048, 4096), "codes [pages, 2, kv_heads, 16 * dim] with dim 64, 128 or 256")
+    _kv8_need(codes.shape[0] >= 1, "at least one page")
     pages, _, kv, m = codes.shape
     _kv8_need(codes.stride()[1:] == (kv * m, m, 1) and codes.stride(0) % 16 == 0 and codes.stride(0) >= 2 * kv * m and codes.data_ptr() % 16 == 0,
               "codes: a page's values together, pages apart by a multiple of 16 bytes")
@@ -1042,7 +1043,7 @@ def kv8_attention(q, codes, scales, row0, starts, page_indptr, page_ids, scale, 
             d.mass, d.mass_page_stride = mass.data_ptr(), _kv8_mass(mass, codes, "mass")
         d.mass_out, d.mass_out_page_stride, d.mass_keep = mass_out.data_ptr(), _kv8_mass(mass_out, codes, "mass_out"), float(mass_keep)
     d.dtype = _dt(q)
-    n = ffi.lib().pegainfer_kv8_attention_workspace(T, H, int(mass_out is not None))
+    n = ffi.lib().pegainfer_kv8_attention_workspace(T, d.max_rows, d.max_len, H, kv, dim, entries, int(mass_out is not None))
     if n > 0:
         ws = torch.empty(n, dtype=torch.float32, device=q.device)
         d.workspace = ws.data_ptr()

@@ -53,7 +53,7 @@ def test_c_entries_refuse(built_libs):
     L, at, bad = ffi.lib(), 1 << 20, 1
     ref = ctypes.addressof
     wrong = [dict(codes=None), dict(codes=at + 8), dict(scales=None), dict(code_page_stride=2 * 2 * 16 * 64 - 16), dict(code_page_stride=2 * 2 * 16 * 64 + 8),
-             dict(scale_page_stride=3), dict(format=2), dict(dim=96), dict(kv_heads=0), dict(n_entries=65536), dict(n_entries=-1), dict(page_indptr=None), dict(page_ids=None)]
+             dict(scale_page_stride=3), dict(format=2), dict(dim=96), dict(kv_heads=0), dict(n_pages=0), dict(n_entries=65536), dict(n_entries=-1), dict(page_indptr=None), dict(page_ids=None)]
     for w in wrong:
         c = _cache(**w)
         assert L.pegainfer_kv8_append(ref(c), at, at, 128, 128, at, at, 4, 4, 0, None) == bad, w
@@ -67,7 +67,7 @@ def test_c_entries_refuse(built_libs):
         assert L.pegainfer_kv8_evict(ref(c), at, 32, at, at, at, 3, budget, first, last, 100, at, None) == bad
     assert L.pegainfer_kv8_evict(ref(c), at, 31, at, at, at, 3, 8, 0, 0, 100, at, None) == bad
     good = dict(q=at, q_row_stride=256, out=at, out_row_stride=256, row0=at, starts=at, n_rows=4, max_rows=4, max_len=9, heads=4, scale=1.0, dtype=0)
-    for w in [dict(q=None), dict(q=at + 4), dict(q_row_stride=255), dict(out_row_stride=260), dict(heads=3), dict(heads=0), dict(n_rows=-1), dict(max_len=-1), dict(dtype=3), dict(row0=None),
+    for w in [dict(q=None), dict(q=at + 4), dict(q_row_stride=255), dict(out_row_stride=260), dict(heads=3), dict(heads=0), dict(scale=-1.0), dict(scale=float('nan')), dict(n_rows=-1), dict(max_len=-1), dict(dtype=3), dict(row0=None),
               dict(mass_out=at, mass_out_page_stride=31, workspace=at), dict(mass_out=at, mass_out_page_stride=32, mass_keep=1.0, workspace=at),
               dict(mass_out=at, mass_out_page_stride=32), dict(n_rows=2 ** 31 - 1, max_rows=1)]:
         d = B.Kv8AttnDesc(**{**good, **w})
