@@ -1123,7 +1123,7 @@ typedef struct {
   float* workspace;
   int32_t dtype;
 } pegainfer_kv8_attn_desc;
-int64_t pegainfer_kv8_attention_workspace(int32_t n_rows, int32_t max_rows, int32_t max_len, int32_t heads, int32_t kv_heads, int32_t dim, int32_t n_entries,
+int64_t pegainfer_kv8_attention_workspace(const pegainfer_kv8_cache* cache, int32_t n_rows, int32_t max_rows, int32_t max_len, int32_t heads, int32_t dtype,
                                           int32_t with_mass);
 pegainfer_status_t pegainfer_kv8_attention(const pegainfer_kv8_cache* cache, const pegainfer_kv8_attn_desc* d, pegainfer_stream_t stream);
 /* Entries of lens[e] tokens are cut to `budget`: every kv head by itself keeps its first keep_first, its last keep_last and of those between the ones of the

@@ -33,13 +33,17 @@ __device__ __forceinline__ QueryRow query_row(int rr, int total, int group, cons
   return {rows.first + tok, kv_head * group + r - tok * group, start + tok, rr < total};
 }
 
+// Blocks a wave takes at a time, and waves of a SIMD: what the registers hold without spilling.  bf16 heads of 128: 189 registers a wave for one row tile, 256 for two.
+template <typename T, int D> constexpr int attn_kb() { return sizeof(T) == 4 || D == 256 ? 2 : 4; }
+template <typename T, int D, int NT> constexpr int attn_waves() { return D * NT * (sizeof(T) == 4 ? 2 : 1) > 256 || (sizeof(T) == 4 && D == 256) ? 1 : 2; }
+
 // One workgroup of four waves: NT tiles of sixteen query rows of a kv head over a run of key blocks.  The blocks are dealt to the waves KB at a time, whose states
 // meet in shared memory at the end, so that no key is loaded or widened twice in a workgroup.  Scores are computed transposed (keys x rows): a lane then holds four
 // keys' scores of one row, exactly what the second product wants from it.  The next keys are on their way while the weights are made, the next values while
 // the next scores are.
-template <typename T, int FMT, int D, int NT, int KB>
-__global__ __launch_bounds__(256) void kv8_attn_kernel(AttnArgs a) {
-  constexpr int NP = kv8_parts<T>(), C = D / 64;
+template <typename T, int FMT, int D, int NT>
+__global__ __launch_bounds__(256, (attn_waves<T, D, NT>())) void kv8_attn_kernel(AttnArgs a) {
+  constexpr int NP = kv8_parts<T>(), C = D / 64, KB = attn_kb<T, D>();
   constexpr bool kScaled = FMT == kE4m3;   // the conversion takes the block's scale along; int8 scales scores and weights instead
   __shared__ f32x4 s_o[2][D / 16][64];
   __shared__ float s_m[2][16], s_l[2][16];
@@ -242,124 +246,180 @@ __global__ __launch_bounds__(256) void kv8_attn_kernel(AttnArgs a) {
   }
 }
 
-// The splits' states of a (row, head) into its output: a workgroup each, every wave takes every W-th split.
+// The splits' states of a (row, head) into its output: a workgroup takes 64 of its values, a wave every W-th split, sixteen of them on their way at a time.
 template <typename T, int D>
 __global__ __launch_bounds__(512) void kv8_merge_kernel(AttnArgs a) {
-  constexpr int V = D / 64;
-  __shared__ float s_o[8][D], s_l[8];
-  const int e = blockIdx.z, head = blockIdx.y, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, lane = threadIdx.x & 63;
+  constexpr int C = D / 64;
+  __shared__ float s_o[8][64], s_l[8];
+  const int e = blockIdx.z, head = blockIdx.y, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6, lane = threadIdx.x & 63, c = blockIdx.x % C;
   const RowSpan rows = row_span(a.row0, e, a.n_rows);
   const int start = a.starts[e], total = rows.n * a.group;
   if (rows.n == 0 || start < 0 || start > INT32_MAX - 2048 - rows.n) return;
-  for (int rr = blockIdx.x; rr < total; rr += gridDim.x) {
+  for (int rr = blockIdx.x / C; rr < total; rr += gridDim.x / C) {
     const QueryRow r = query_row(rr, total, a.group, rows, start, head);
     const int64_t rh = (int64_t)r.row * a.heads + r.head;
     const f32x2* ml = reinterpret_cast<const f32x2*>(a.part_ml) + rh * a.n_split;
+    const float* part = a.part_o + rh * a.n_split * D + c * 64 + lane;
     float m = -INFINITY;
     for (int i = lane; i < a.n_split; i += 64) m = fmaxf(m, ml[i].x);
     m = wave_max(m);
     const float base = m == -INFINITY ? 0.f : m;
-    float l = 0.f, o[V];
+    float l = 0.f, o = 0.f;
+    for (int at = wave; at < a.n_split; at += 16 * waves) {
+      float p[16];
+      f32x2 x[16];
 #pragma unroll
-    for (int v = 0; v < V; ++v) o[v] = 0.f;
-#pragma unroll 4
-    for (int i = wave; i < a.n_split; i += waves) {
-      const f32x2 x = ml[i];
-      if (!(x.y > 0.f || x.y != x.y)) continue;             // a split without a key left no sums
-      const float w = exp2_of(x.x - base);
-      l += x.y * w;
-      const float* p = a.part_o + (rh * a.n_split + i) * D + lane * V;
+      for (int i = 0; i < 16; ++i) {
+        const int z = min(at + i * waves, a.n_split - 1);
+        p[i] = part[(int64_t)z * D];
+        x[i] = ml[z];
+      }
 #pragma unroll
-      for (int v = 0; v < V; ++v) o[v] += w * p[v];
+      for (int i = 0; i < 16; ++i) {
+        // a split without a key left no sums: what is in their place is not looked at
+        const bool some = at + i * waves < a.n_split && (x[i].y > 0.f || x[i].y != x[i].y);
+        const float w = exp2_of(x[i].x - base);
+        l += some ? x[i].y * w : 0.f;
+        o += some ? p[i] * w : 0.f;
+      }
     }
     if (lane == 0) s_l[wave] = l;
-#pragma unroll
-    for (int v = 0; v < V; ++v) s_o[wave][lane * V + v] = o[v];
+    s_o[wave][lane] = o;
     __syncthreads();
     if (wave == 0) {
       for (int w = 1; w < waves; ++w) {
         l += s_l[w];
-#pragma unroll
-        for (int v = 0; v < V; ++v) o[v] += s_o[w][lane * V + v];
+        o += s_o[w][lane];
       }
       const bool some = l > 0.f || l != l;
-      const float inv = some ? 1.f / l : 0.f;
-      T* op = static_cast<T*>(a.out) + r.row * a.out_stride + (int64_t)r.head * D + lane * V;
-#pragma unroll
-      for (int v = 0; v < V; ++v) st(op + v, o[v] * inv);
-      if (a.lse && lane == 0) a.lse[rh] = some ? m + __log2f(l) : INFINITY;
+      st(static_cast<T*>(a.out) + r.row * a.out_stride + (int64_t)r.head * D + c * 64 + lane, some ? o / l : 0.f);
+      if (a.lse && lane == 0 && c == 0) a.lse[rh] = some ? m + __log2f(l) : INFINITY;
     }
     __syncthreads();
   }
 }
 
-// The weights that a step gives to the cached tokens, from the sums that the attention left: a wave a block of keys, which it holds as operands while it walks
-// all rows that see them, so that every token's sum is one wave's, in the rows' order.
+// The weights that a call gives to the cached tokens, from the sums that the attention left.  A wave holds MB blocks of keys as operands while it walks the row tiles
+// that see them (the four waves of a workgroup the same tiles, which then come from the first-level cache), so that a token's sum is one wave's, in the rows' order.
+// n_slice > 1, where that leaves too few workgroups: every slice of the row tiles leaves its sums in part, kv8_mass_sum_kernel adds them in order.
+struct MassArgs {
+  const float* mass;
+  float *out, *part;     // part [n_slice][n_ids][kv_heads][16]
+  int64_t mass_stride, out_stride;
+  float keep;
+  int n_slice;
+};
+__device__ __forceinline__ void put_mass(const MassArgs& w, int page, int at, float x) {
+  // 0 means without what was there, whatever that is
+  w.out[page * w.out_stride + at] = w.keep == 0.f ? x : fmaf(w.keep, w.mass[page * w.mass_stride + at], x);
+}
+
+template <typename T, int D> constexpr int mass_blocks() { return D == 256 ? 2 : 4; }
+
 template <typename T, int FMT, int D>
-__global__ __launch_bounds__(256) void kv8_mass_kernel(AttnArgs a, const float* mass, int64_t mass_stride, float* out, int64_t out_stride, float keep) {
-  constexpr int NP = kv8_parts<T>(), C = D / 64;
-  const int e = blockIdx.z, head = blockIdx.y, wave = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+__global__ __launch_bounds__(256, 2) void kv8_mass_kernel(AttnArgs a, MassArgs w) {
+  constexpr int NP = kv8_parts<T>(), C = D / 64, MB = mass_blocks<T, D>();
+  const int e = blockIdx.z, head = blockIdx.y, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   const RowSpan rows = row_span(a.row0, e, a.n_rows);
   const int start = a.starts[e], total = rows.n * a.group;
   if (rows.n == 0 || start < 0 || start > INT32_MAX - 2048 - rows.n) return;
-  const int len = start + rows.n;
-  for (int b = blockIdx.x * 4 + wave; b * kKv8Page < len; b += gridDim.x * 4) {
-    const int page = a.c.page(e, b);
-    if (page < 0) continue;
-    bf16x8_t kf[C][2];
-    const uint8_t* kb = a.c.block(page, 0, head, D) + n * 64 + g * 16;
+  const int blocks = (start + rows.n + kKv8Page - 1) / kKv8Page, slice = blockIdx.x % w.n_slice, tiles = (total + 15) / 16;
+  for (int b0 = (blockIdx.x / w.n_slice * 4 + wave) * MB; b0 < blocks; b0 += gridDim.x / w.n_slice * 4 * MB) {
+    int page[MB];
+    float ks[MB];
+    bf16x8_t kf[MB][C][2];
+    u32x4 kw[MB][C];
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-      const u32x4 w = *reinterpret_cast<const u32x4*>(kb + c * 1024);
-      kf[c][0] = kv8_operand<FMT>(w.x, w.y);
-      kf[c][1] = kv8_operand<FMT>(w.z, w.w);
+    for (int h = 0; h < MB; ++h) page[h] = b0 + h < blocks ? a.c.page(e, b0 + h) : -1;
+#pragma unroll
+    for (int h = 0; h < MB; ++h) {
+      const uint8_t* kb = a.c.block(max(page[h], 0), 0, head, D) + n * 64 + g * 16;      // one that is not there: page 0's bytes, whose sums are left out
+#pragma unroll
+      for (int c = 0; c < C; ++c) kw[h][c] = *reinterpret_cast<const u32x4*>(kb + c * 1024);
+      ks[h] = *a.c.scale(max(page[h], 0), 0, head) * a.scale_log2;
     }
-    const float ks = *a.c.scale(page, 0, head) * a.scale_log2;
-    float sum[4] = {0.f, 0.f, 0.f, 0.f};
-    const int first = max(b * kKv8Page - start, 0) * a.group / 16;     // the first tile with a row that sees the block
-    for (int tile = first; tile * 16 < total; ++tile) {
-      const QueryRow r = query_row(tile * 16 + n, total, a.group, rows, start, head);
-      const T* qp = static_cast<const T*>(a.q) + r.row * a.q_stride + (int64_t)r.head * D + g * 16;
-      f32x4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int h = 0; h < MB; ++h)
 #pragma unroll
       for (int c = 0; c < C; ++c) {
-        bf16x8_t q0[NP], q1[NP];
-        kv8_query(qp + c * 64, q0);
-        kv8_query(qp + c * 64 + 8, q1);
+        kf[h][c][0] = kv8_operand<FMT>(kw[h][c].x, kw[h][c].y);
+        kf[h][c][1] = kv8_operand<FMT>(kw[h][c].z, kw[h][c].w);
+      }
+    f32x4 sum[MB];
 #pragma unroll
-        for (int p = NP - 1; p >= 0; --p) {
-          s = mfma16(kf[c][0], q0[p], s);
-          s = mfma16(kf[c][1], q1[p], s);
+    for (int h = 0; h < MB; ++h) sum[h] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int slot0 = b0 * kKv8Page, first = (int)((int64_t)max(slot0 - start, 0) * a.group / 16);     // the first tile with a row that sees a block
+    const int per = (tiles - first + w.n_slice - 1) / w.n_slice, last = min(tiles, first + (slice + 1) * per);
+    for (int tile = first + slice * per; tile < last; ++tile) {
+      const QueryRow r = query_row(tile * 16 + n, total, a.group, rows, start, head);
+      const T* qp = static_cast<const T*>(a.q) + r.row * a.q_stride + (int64_t)r.head * D + g * 16;
+      const float lse = r.real ? a.lse[(int64_t)r.row * a.heads + r.head] : INFINITY;      // a row behind the last weighs nothing
+      f32x4 s[MB];
+#pragma unroll
+      for (int h = 0; h < MB; ++h) s[h] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          bf16x8_t q[NP];
+          kv8_query(qp + c * 64 + 8 * k, q);
+#pragma unroll
+          for (int p = NP - 1; p >= 0; --p)
+#pragma unroll
+            for (int h = 0; h < MB; ++h) s[h] = mfma16(kf[h][c][k], q[p], s[h]);
         }
-      }
-      const float lse = a.lse[(int64_t)r.row * a.heads + r.head];
+      const bool all = slot0 + MB * kKv8Page - 1 <= tile * 16 / a.group + start;           // every row of the tile sees every slot
 #pragma unroll
-      for (int i = 0; i < 4; ++i) sum[i] += r.real && b * kKv8Page + 4 * g + i <= r.far ? exp2_of(s[i] * ks - lse) : 0.f;
+      for (int h = 0; h < MB; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float p = exp2_of(fmaf(s[h][i], ks[h], -lse));
+          sum[h][i] += all || slot0 + h * kKv8Page + 4 * g + i <= r.far ? p : 0.f;
+        }
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float x = row16_sum(sum[i]);
-      const int t = 4 * g + i;
-      if (n == i && b * kKv8Page + t < len) {
-        const int64_t at = head * kKv8Page + t;
-        // 0 means without what was there, whatever that is
-        out[page * out_stride + at] = keep == 0.f ? x : fmaf(keep, mass[page * mass_stride + at], x);
+    for (int h = 0; h < MB; ++h)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float x = row16_sum(sum[h][i]);
+        const int t = 4 * g + i, at = head * kKv8Page + t;
+        if (n != i || page[h] < 0 || slot0 + h * kKv8Page + t >= start + rows.n) continue;
+        if (w.n_slice > 1) w.part[((int64_t)slice * a.c.n_ids + a.c.indptr[e] + b0 + h) * a.c.kv_heads * kKv8Page + at] = x;
+        else put_mass(w, page[h], at, x);
       }
-    }
   }
 }
 
-// How a call is cut: rows of a workgroup, and splits of the keys where that leaves too few workgroups.
-struct AttnPlan { int tiles, row_tiles, n_split, split_blocks; };
-inline AttnPlan attn_plan(int n_rows, int max_rows, int max_len, int group, int kv_heads, int entries) {
+// the slices' sums of a block's tokens, in order: a wave four blocks of a head
+__global__ __launch_bounds__(256) void kv8_mass_sum_kernel(AttnArgs a, MassArgs w) {
+  const int e = blockIdx.z, head = blockIdx.y;
+  const RowSpan rows = row_span(a.row0, e, a.n_rows);
+  const int start = a.starts[e];
+  if (rows.n == 0 || start < 0 || start > INT32_MAX - 2048 - rows.n) return;
+  const int len = start + rows.n;
+  for (int slot = blockIdx.x * 256 + threadIdx.x; slot < len; slot += gridDim.x * 256) {
+    const int block = slot / kKv8Page, page = a.c.page(e, block), at = head * kKv8Page + slot % kKv8Page;
+    if (page < 0) continue;
+    float x = 0.f;
+    for (int z = 0; z < w.n_slice; ++z) x += w.part[((int64_t)z * a.c.n_ids + a.c.indptr[e] + block) * a.c.kv_heads * kKv8Page + at];
+    put_mass(w, page, at, x);
+  }
+}
+
+// How a call is cut: rows of a workgroup, splits of the keys and slices of the weights' rows where those leave too few workgroups.
+struct AttnPlan { int tiles, row_tiles, n_split, split_blocks, mass_groups, n_slice; };
+inline AttnPlan attn_plan(const pegainfer_kv8_cache* cache, int n_rows, int max_rows, int max_len, int heads, int dtype) {
   AttnPlan p;
-  const int64_t rows = (int64_t)std::min(max_rows, n_rows) * group;
-  p.row_tiles = rows > 16 ? 2 : 1;
+  const int64_t rows = (int64_t)std::min(max_rows, n_rows) * (heads / cache->kv_heads), pairs = (int64_t)cache->kv_heads * cache->n_entries;
+  p.row_tiles = rows > 16 && !(dtype == kDtF32 && cache->dim == 256) ? 2 : 1;
   p.tiles = ceil_div(rows, 16 * p.row_tiles);
   const int blocks = std::max(1, ceil_div(max_len, kKv8Page));
-  const int64_t groups = (int64_t)p.tiles * kv_heads * entries, want = 8 * device_cus();
-  p.n_split = (int)std::min<int64_t>({(want + groups - 1) / groups, (blocks + 15) / 16, 256});
+  const int64_t want = 2 * device_cus();
+  auto cut = [&](int64_t groups, int64_t most) { return (int)std::max<int64_t>(1, std::min((want + groups - 1) / groups, most)); };
+  p.n_split = cut(p.tiles * pairs, std::min((blocks + 15) / 16, 256));
   p.split_blocks = ceil_div(blocks, p.n_split);
+  p.mass_groups = ceil_div(blocks, 4 * (cache->dim == 256 ? 2 : 4));
+  p.n_slice = cut(p.mass_groups * pairs, std::min<int64_t>((rows + 255) / 256, 16));
   return p;
 }
 
@@ -369,12 +429,13 @@ using namespace pk;
 
 extern "C" {
 
-int64_t pegainfer_kv8_attention_workspace(int32_t n_rows, int32_t max_rows, int32_t max_len, int32_t heads, int32_t kv_heads, int32_t dim, int32_t n_entries,
+int64_t pegainfer_kv8_attention_workspace(const pegainfer_kv8_cache* cache, int32_t n_rows, int32_t max_rows, int32_t max_len, int32_t heads, int32_t dtype,
                                           int32_t with_mass) {
-  if (n_rows <= 0 || max_rows <= 0 || kv_heads < 1 || heads < kv_heads || n_entries <= 0) return 0;
-  const AttnPlan p = attn_plan(n_rows, max_rows, max_len, heads / kv_heads, kv_heads, n_entries);
+  if (!kv8_ok(cache) || n_rows <= 0 || max_rows <= 0 || max_len < 0 || heads < cache->kv_heads || cache->n_entries == 0) return 0;
+  const AttnPlan p = attn_plan(cache, n_rows, max_rows, max_len, heads, dtype);
   const int64_t rh = (int64_t)n_rows * heads;
-  return (p.n_split > 1 ? rh * p.n_split * (dim + 2) : 0) + (with_mass ? rh : 0);
+  return (p.n_split > 1 ? rh * p.n_split * (cache->dim + 2) : 0) + (with_mass ? rh : 0) +
+         (with_mass && p.n_slice > 1 ? (int64_t)p.n_slice * cache->n_page_ids * cache->kv_heads * kKv8Page : 0);
 }
 
 pegainfer_status_t pegainfer_kv8_attention(const pegainfer_kv8_cache* cache, const pegainfer_kv8_attn_desc* d, pegainfer_stream_t stream) {
@@ -390,24 +451,27 @@ pegainfer_status_t pegainfer_kv8_attention(const pegainfer_kv8_cache* cache, con
   const int64_t mass_width = (int64_t)cache->kv_heads * kKv8Page;
   if (weigh && (d->mass_out_page_stride < mass_width || (d->mass_keep != 0.f && (!d->mass || d->mass_page_stride < mass_width)))) return PK_BAD;
   const int group = d->heads / cache->kv_heads;
-  const AttnPlan p = attn_plan(d->n_rows, d->max_rows, d->max_len, group, cache->kv_heads, cache->n_entries);
+  const AttnPlan p = attn_plan(cache, d->n_rows, d->max_rows, d->max_len, d->heads, d->dtype);
   if ((weigh || p.n_split > 1) && (!d->workspace || !host_aligned16(d->workspace))) return PK_BAD;
   const int64_t rh = (int64_t)d->n_rows * d->heads;
   float* part_ml = d->workspace + (p.n_split > 1 ? rh * p.n_split * cache->dim : 0);
   const AttnArgs a{kv8_of(cache), d->q, d->q_row_stride, d->out_row_stride, d->row0, d->starts, d->n_rows, group, d->heads, p.n_split, p.split_blocks,
                    d->scale * 1.4426950408889634f, d->out, weigh ? part_ml + (p.n_split > 1 ? rh * p.n_split * 2 : 0) : nullptr, d->workspace, part_ml};
   const dim3 grid(p.tiles * p.n_split, cache->kv_heads, cache->n_entries);
-  const dim3 merge_grid(std::min(d->max_rows, d->n_rows) * group, cache->kv_heads, cache->n_entries);
-  const dim3 mass_grid(std::max(1, ceil_div(d->max_len, 4 * kKv8Page)), cache->kv_heads, cache->n_entries);
+  const dim3 merge_grid(std::min(d->max_rows, d->n_rows) * group * (cache->dim / 64), cache->kv_heads, cache->n_entries);
+  const dim3 mass_grid(p.mass_groups * p.n_slice, cache->kv_heads, cache->n_entries), sum_grid(std::max(1, ceil_div(d->max_len, 256)), cache->kv_heads, cache->n_entries);
+  const MassArgs w{d->mass, d->mass_out, weigh ? a.lse + rh : nullptr, d->mass_page_stride, d->mass_out_page_stride, d->mass_keep, p.n_slice};
   kv8_by(d->dtype, cache->format, cache->dim, [&](auto* t, auto fmt, auto dim) {
     using T = std::remove_pointer_t<decltype(t)>;
-    constexpr int D = dim(), KB = D == 256 ? 2 : 4;
-    if (p.row_tiles == 1) kv8_attn_kernel<T, fmt(), D, 1, KB><<<grid, 256, 0, as_stream(stream)>>>(a);
-    else kv8_attn_kernel<T, fmt(), D, 2, KB><<<grid, 256, 0, as_stream(stream)>>>(a);
+    constexpr int D = dim();
+    if constexpr (sizeof(T) == 2 || D < 256) {
+      if (p.row_tiles == 2) kv8_attn_kernel<T, fmt(), D, 2><<<grid, 256, 0, as_stream(stream)>>>(a);
+    }
+    if (p.row_tiles == 1) kv8_attn_kernel<T, fmt(), D, 1><<<grid, 256, 0, as_stream(stream)>>>(a);
     if (p.n_split > 1) kv8_merge_kernel<T, D><<<merge_grid, 64 * std::min(8, p.n_split), 0, as_stream(stream)>>>(a);
-    if (weigh)
-      kv8_mass_kernel<T, fmt(), D><<<mass_grid, 256, 0, as_stream(stream)>>>(a, d->mass, d->mass_page_stride, d->mass_out, d->mass_out_page_stride, d->mass_keep);
+    if (weigh) kv8_mass_kernel<T, fmt(), D><<<mass_grid, 256, 0, as_stream(stream)>>>(a, w);
   });
+  if (weigh && p.n_slice > 1) kv8_mass_sum_kernel<<<sum_grid, 256, 0, as_stream(stream)>>>(a, w);
   return (pegainfer_status_t)hipGetLastError();
 }
 

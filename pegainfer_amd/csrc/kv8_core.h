@@ -10,6 +10,8 @@
 // rescaled again and again, one power at a time, is off by half a final step times 1 + 1/2 + 1/4 ...: less than one step.
 #pragma once
 
+#include <type_traits>
+
 #include "typed.h"
 
 namespace pk {
@@ -100,9 +102,20 @@ __device__ __forceinline__ bf16x8_t kv8_operand2(uint32_t lo, uint32_t hi, float
     o.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale_hi, false));
     o.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale_hi, true));
   } else {
-    float a[4], b[4];
-    kv8_numbers<FMT>(lo, a);
-    kv8_numbers<FMT>(hi, b);
+    // a byte to a float in one instruction each; the compiler's own choice takes the byte out first
+    auto at = [](uint32_t w, auto i) {
+      float f;
+      if constexpr (i() == 0) asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_0" : "=v"(f) : "v"(w));
+      else if constexpr (i() == 1) asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_1" : "=v"(f) : "v"(w));
+      else if constexpr (i() == 2) asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_2" : "=v"(f) : "v"(w));
+      else asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_3" : "=v"(f) : "v"(w));
+      return f;
+    };
+    constexpr std::integral_constant<int, 0> i0{};
+    constexpr std::integral_constant<int, 1> i1{};
+    constexpr std::integral_constant<int, 2> i2{};
+    constexpr std::integral_constant<int, 3> i3{};
+    const float a[4] = {at(lo, i0), at(lo, i1), at(lo, i2), at(lo, i3)}, b[4] = {at(hi, i0), at(hi, i1), at(hi, i2), at(hi, i3)};
     auto top = [](float l, float h) { return __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, h), __builtin_bit_cast(uint32_t, l), 0x07060302u); };
     o.x = top(a[0], a[1]); o.y = top(a[2], a[3]); o.z = top(b[0], b[1]); o.w = top(b[2], b[3]);
   }

@@ -953,41 +953,59 @@ def _kv8_need(ok, what):
         raise ValueError("kv8: " + what)
 
 
-def _kv8_tables(device, *tables):
-    for t, n, what in tables:
-        _kv8_need(t.dtype == torch.int32 and t.is_contiguous() and t.device == device and (t.numel() == n if n is not None else t.dim() == 1),
-                  "%s: contiguous int32 on the cache's device%s" % (what, "" if n is None else ", %d values" % n))
+_I32, _F32 = torch.int32, torch.float32
+_KV8_DTYPES = {torch.bfloat16: 0, torch.float32: 1}
+
+
+def _kv8_index(t, n, codes, what):
+    """an index table's address; n values (None: any number)"""
+    if t.dtype is not _I32 or t.dim() != 1 or t.stride(0) != 1 or t.device != codes.device or (n is not None and t.numel() != n):
+        raise ValueError("kv8: %s: contiguous int32 on the cache's device%s" % (what, "" if n is None else ", %d values" % n))
+    return t.data_ptr()
 
 
 def _kv8_cache(codes, scales, page_indptr, page_ids, entries):
     """-> (descriptor, kv_heads, dim); refuses what the kernels do not take"""
-    _kv8_need(codes.dtype in KV8_FORMATS, "codes of torch.float8_e4m3fn or torch.int8")
-    _kv8_need(codes.is_cuda and codes.device.index == torch.cuda.current_device(), "a cache on the current device")
-    _kv8_need(codes.dim() == 4 and codes.shape[1] == 2 and codes.shape[3] in (1024, 2048, 4096), "codes [pages, 2, kv_heads, 16 * dim] with dim 64, 128 or 256")
-    _kv8_need(codes.shape[0] >= 1, "at least one page")
-    pages, _, kv, m = codes.shape
-    _kv8_need(codes.stride()[1:] == (kv * m, m, 1) and codes.stride(0) % 16 == 0 and codes.stride(0) >= 2 * kv * m and codes.data_ptr() % 16 == 0,
+    fmt, shape, stride = KV8_FORMATS.get(codes.dtype), codes.shape, codes.stride()
+    _kv8_need(fmt is not None, "codes of torch.float8_e4m3fn or torch.int8")
+    _kv8_need(codes.is_cuda and codes.get_device() == torch.cuda.current_device(), "a cache on the current device")
+    _kv8_need(len(shape) == 4 and shape[1] == 2 and shape[3] in (1024, 2048, 4096) and shape[0] >= 1, "codes [pages, 2, kv_heads, 16 * dim], a page at least, dim 64, 128 or 256")
+    pages, _, kv, m = shape
+    at = codes.data_ptr()
+    _kv8_need(stride[3] == 1 and stride[2] == m and stride[1] == kv * m and stride[0] >= 2 * kv * m and (stride[0] | at) % 16 == 0,
               "codes: a page's values together, pages apart by a multiple of 16 bytes")
-    _kv8_need(scales.dtype == torch.float32 and scales.device == codes.device and scales.shape == (pages, 2, kv) and scales.stride()[1:] == (kv, 1) and
-              scales.stride(0) >= 2 * kv, "scales fp32 [pages, 2, kv_heads] on the cache's device, a page's together")
+    sstride = scales.stride()
+    _kv8_need(scales.dtype is _F32 and scales.device == codes.device and scales.shape == shape[:3] and sstride[2] == 1 and sstride[1] == kv and sstride[0] >= 2 * kv,
+              "scales fp32 [pages, 2, kv_heads] on the cache's device, a page's together")
     _kv8_need(1 <= kv <= 65535 and entries <= 65535, "at most 65535 kv heads and entries")
-    _kv8_tables(codes.device, (page_indptr, entries + 1, "page_indptr"), (page_ids, None, "page_ids"))
-    return Kv8Cache(codes.data_ptr(), scales.data_ptr(), codes.stride(0), scales.stride(0), KV8_FORMATS[codes.dtype], pages, kv, m // 16, page_indptr.data_ptr(),
-                    page_ids.data_ptr(), page_ids.numel(), entries), kv, m // 16
+    return Kv8Cache(at, scales.data_ptr(), stride[0], sstride[0], fmt, pages, kv, m // 16, _kv8_index(page_indptr, entries + 1, codes, "page_indptr"),
+                    _kv8_index(page_ids, None, codes, "page_ids"), page_ids.numel(), entries), kv, m // 16
 
 
-def _kv8_rows(x, heads, dim, device, what):
-    _kv8_need(x.dtype in (torch.bfloat16, torch.float32) and x.device == device, "%s: bf16 or fp32 on the cache's device" % what)
-    _kv8_need(x.dim() == 3 and x.shape[2] == dim and (heads is None or x.shape[1] == heads), "%s: rows of heads of %d values" % (what, dim))
-    _kv8_need(x.stride(2) == 1 and x.stride(1) == dim and (x.stride(0) >= x.shape[1] * dim or x.shape[0] <= 1) and x.stride(0) * x.element_size() % 16 == 0 and x.data_ptr() % 16 == 0,
-              "%s: a row's values together, rows apart by a multiple of 16 bytes" % what)
-    return max(x.stride(0), x.shape[1] * dim)
+def _kv8_rows(x, heads, dim, codes, what):
+    """row stride of rows of heads"""
+    shape, stride, at = x.shape, x.stride(), x.data_ptr()
+    if x.dtype not in _KV8_DTYPES or x.device != codes.device:
+        raise ValueError("kv8: %s: bf16 or fp32 on the cache's device" % what)
+    if len(shape) != 3 or shape[2] != dim or (heads is not None and shape[1] != heads):
+        raise ValueError("kv8: %s: rows of %s heads of %d values" % (what, "whole" if heads is None else heads, dim))
+    row = shape[1] * dim
+    if shape[0] <= 1:
+        rows = max(row, (stride[0] + 15) // 16 * 16)              # of a single row no stride is used
+    else:
+        rows = stride[0]
+    if stride[2] != 1 or (shape[1] > 1 and stride[1] != dim) or rows < row or (rows * x.element_size() | at) % 16:
+        raise ValueError("kv8: %s: a row's values together, rows apart by a multiple of 16 bytes" % what)
+    return rows
 
 
 def _kv8_mass(mass, codes, what):
-    _kv8_need(mass.dtype == torch.float32 and mass.device == codes.device and mass.shape == (codes.shape[0], codes.shape[2], 16) and mass.stride()[1:] == (16, 1) and
-              mass.stride(0) >= codes.shape[2] * 16, "%s fp32 [pages, kv_heads, 16] on the cache's device, a page's together" % what)
-    return mass.stride(0)
+    """page stride of weights"""
+    stride = mass.stride()
+    if (mass.dtype is not _F32 or mass.device != codes.device or mass.shape != (codes.shape[0], codes.shape[2], 16) or stride[2] != 1 or stride[1] != 16 or
+            stride[0] < codes.shape[2] * 16):
+        raise ValueError("kv8: %s fp32 [pages, kv_heads, 16] on the cache's device, a page's together" % what)
+    return stride[0]
 
 
 def kv8_append(k, v, codes, scales, row0, starts, page_indptr, page_ids, max_rows=None):
@@ -995,11 +1013,11 @@ def kv8_append(k, v, codes, scales, row0, starts, page_indptr, page_ids, max_row
     rows of an entry (None: all)"""
     entries = row0.numel() - 1
     cache, kv, dim = _kv8_cache(codes, scales, page_indptr, page_ids, entries)
-    _kv8_tables(codes.device, (row0, entries + 1, "row0"), (starts, entries, "starts"))
-    strides = _kv8_rows(k, kv, dim, codes.device, "k"), _kv8_rows(v, kv, dim, codes.device, "v")
+    tables = _kv8_index(row0, entries + 1, codes, "row0"), _kv8_index(starts, entries, codes, "starts")
+    strides = _kv8_rows(k, kv, dim, codes, "k"), _kv8_rows(v, kv, dim, codes, "v")
     _kv8_need(k.dtype == v.dtype and k.shape == v.shape, "k and v of one shape and type")
-    _chk(ffi.lib().pegainfer_kv8_append(ctypes.addressof(cache), k.data_ptr(), v.data_ptr(), *strides, row0.data_ptr(), starts.data_ptr(), k.shape[0],
-                                        k.shape[0] if max_rows is None else int(max_rows), _dt(k), _stream()), "kv8_append")
+    _chk(ffi.lib().pegainfer_kv8_append(ctypes.addressof(cache), k.data_ptr(), v.data_ptr(), *strides, *tables, k.shape[0],
+                                        k.shape[0] if max_rows is None else int(max_rows), _KV8_DTYPES[k.dtype], _stream()), "kv8_append")
 
 
 def kv8_read(codes, scales, row0, starts, page_indptr, page_ids, n_rows, dtype=torch.bfloat16, max_rows=None, out=None):
@@ -1007,16 +1025,17 @@ def kv8_read(codes, scales, row0, starts, page_indptr, page_ids, n_rows, dtype=t
     they are (in a fresh tensor: unset)"""
     entries = row0.numel() - 1
     cache, kv, dim = _kv8_cache(codes, scales, page_indptr, page_ids, entries)
-    _kv8_tables(codes.device, (row0, entries + 1, "row0"), (starts, entries, "starts"))
-    _kv8_need(n_rows >= 0 and dtype in (torch.bfloat16, torch.float32), "n_rows >= 0, values in bf16 or fp32")
+    tables = _kv8_index(row0, entries + 1, codes, "row0"), _kv8_index(starts, entries, codes, "starts")
+    _kv8_need(n_rows >= 0 and dtype in _KV8_DTYPES, "n_rows >= 0, values in bf16 or fp32")
     if out is None:
-        out = torch.empty((2, n_rows, kv, dim), dtype=dtype, device=codes.device).unbind(0)
-    k, v = out
-    for x, what in ((k, "k"), (v, "v")):
-        _kv8_need(x.shape == (n_rows, kv, dim) and x.dtype == dtype and x.device == codes.device and x.is_contiguous() and x.data_ptr() % 16 == 0,
-                  "out: contiguous %s [n_rows, kv_heads, dim] of dtype" % what)
-    _chk(ffi.lib().pegainfer_kv8_read(ctypes.addressof(cache), row0.data_ptr(), starts.data_ptr(), k.data_ptr(), v.data_ptr(), int(n_rows),
-                                      int(n_rows if max_rows is None else max_rows), _dt(k), _stream()), "kv8_read")
+        k, v = (torch.empty((n_rows, kv, dim), dtype=dtype, device=codes.device) for _ in range(2))
+    else:
+        k, v = out
+        for x in out:
+            _kv8_need(x.shape == (n_rows, kv, dim) and x.dtype is dtype and x.device == codes.device and x.is_contiguous() and x.data_ptr() % 16 == 0,
+                      "out: two contiguous tensors [n_rows, kv_heads, dim] of dtype")
+    _chk(ffi.lib().pegainfer_kv8_read(ctypes.addressof(cache), *tables, k.data_ptr(), v.data_ptr(), int(n_rows),
+                                      int(n_rows if max_rows is None else max_rows), _KV8_DTYPES[dtype], _stream()), "kv8_read")
     return k, v
 
 
@@ -1026,24 +1045,25 @@ def kv8_attention(q, codes, scales, row0, starts, page_indptr, page_ids, scale, 
     mass_out alone with mass_keep 0: the weight of this call."""
     entries = row0.numel() - 1
     cache, kv, dim = _kv8_cache(codes, scales, page_indptr, page_ids, entries)
-    _kv8_tables(codes.device, (row0, entries + 1, "row0"), (starts, entries, "starts"))
-    q_stride = _kv8_rows(q, None, dim, codes.device, "q")
+    row0_at, starts_at = _kv8_index(row0, entries + 1, codes, "row0"), _kv8_index(starts, entries, codes, "starts")
+    q_stride = _kv8_rows(q, None, dim, codes, "q")
     T, H, _ = q.shape
     _kv8_need(H > 0 and H % kv == 0, "query heads: a multiple of the kv heads")
     if out is None:
-        out = torch.empty((T, H, dim), dtype=q.dtype, device=q.device)
-    _kv8_need(out.dtype == q.dtype and out.shape == q.shape, "out like q")
-    out_stride = _kv8_rows(out, H, dim, codes.device, "out")
+        out, out_stride = torch.empty((T, H, dim), dtype=q.dtype, device=q.device), H * dim
+    else:
+        _kv8_need(out.dtype is q.dtype and out.shape == q.shape, "out like q")
+        out_stride = _kv8_rows(out, H, dim, codes, "out")
     mass_out = mass if mass_out is None else mass_out
     _kv8_need(mass_out is None or mass is not None or mass_keep == 0, "mass_keep other than 0 needs mass")
-    d = Kv8AttnDesc(q.data_ptr(), q_stride, out.data_ptr(), out_stride, row0.data_ptr(), starts.data_ptr(), T, T if max_rows is None else int(max_rows),
+    d = Kv8AttnDesc(q.data_ptr(), q_stride, out.data_ptr(), out_stride, row0_at, starts_at, T, T if max_rows is None else int(max_rows),
                     page_ids.numel() * 16 if max_len is None else int(max_len), H, float(scale))
     if mass_out is not None:
         if mass is not None:
             d.mass, d.mass_page_stride = mass.data_ptr(), _kv8_mass(mass, codes, "mass")
         d.mass_out, d.mass_out_page_stride, d.mass_keep = mass_out.data_ptr(), _kv8_mass(mass_out, codes, "mass_out"), float(mass_keep)
-    d.dtype = _dt(q)
-    n = ffi.lib().pegainfer_kv8_attention_workspace(T, d.max_rows, d.max_len, H, kv, dim, entries, int(mass_out is not None))
+    d.dtype = _KV8_DTYPES[q.dtype]
+    n = ffi.lib().pegainfer_kv8_attention_workspace(ctypes.addressof(cache), T, d.max_rows, d.max_len, H, d.dtype, int(mass_out is not None))
     if n > 0:
         ws = torch.empty(n, dtype=torch.float32, device=q.device)
         d.workspace = ws.data_ptr()
@@ -1056,11 +1076,11 @@ def kv8_evict(codes, scales, mass, lens, page_indptr, page_ids, dst_indptr, dst_
     first keep_first and last keep_last among them) and moved, with their mass, to the pages dst_ids[dst_indptr[e]] ..., which are no source pages of the call."""
     entries = lens.numel()
     cache, kv, _ = _kv8_cache(codes, scales, page_indptr, page_ids, entries)
-    _kv8_tables(codes.device, (lens, entries, "lens"), (dst_indptr, entries + 1, "dst_indptr"), (dst_ids, None, "dst_ids"))
+    tables = _kv8_index(lens, entries, codes, "lens"), _kv8_index(dst_indptr, entries + 1, codes, "dst_indptr"), _kv8_index(dst_ids, None, codes, "dst_ids")
     _kv8_need(budget >= 1 and keep_first >= 0 and keep_last >= 0 and keep_first + keep_last <= budget, "budget of at least 1 token, keep_first + keep_last within it")
     stride = _kv8_mass(mass, codes, "mass")
     kept = torch.empty((entries, kv, budget), dtype=torch.int32, device=codes.device)
-    _chk(ffi.lib().pegainfer_kv8_evict(ctypes.addressof(cache), mass.data_ptr(), stride, lens.data_ptr(), dst_indptr.data_ptr(), dst_ids.data_ptr(), dst_ids.numel(),
+    _chk(ffi.lib().pegainfer_kv8_evict(ctypes.addressof(cache), mass.data_ptr(), stride, *tables, dst_ids.numel(),
                                        int(budget), int(keep_first), int(keep_last), page_ids.numel() * 16 if max_len is None else int(max_len), kept.data_ptr(),
                                        _stream()), "kv8_evict")
     return kept
