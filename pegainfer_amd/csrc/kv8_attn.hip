@@ -24,6 +24,8 @@ struct AttnArgs {
   void* out;
   float* lse;            // [n_rows][heads], log2 of the sum of exp(scores); NULL: not wanted
   float *part_o, *part_ml;   // n_split > 1: [n_rows][heads][n_split][D] and [2] (running maximum, sum)
+  float* scores;         // [n_ids][kv_heads][score_rows][16] of entries of up to score_rows <= 16 query rows a kv head, for the weights; NULL: not wanted
+  int score_rows;
 };
 
 // the queries' rows of a kv head, (token, head of the group) in order; a row behind the last is the last again
@@ -136,6 +138,14 @@ __global__ __launch_bounds__(256, (attn_waves<T, D, NT>())) void kv8_attn_kernel
             const uint32_t bytes = here >= 4 ? 0xFFFFFFFFu : here <= 0 ? 0u : 0xFFFFFFFFu >> (32 - 8 * here);
 #pragma unroll
             for (int c = 0; c < C; ++c) vw[h][c] &= bytes;
+          }
+        }
+        if constexpr (NT == 1) {
+          if (a.scores && total <= a.score_rows && r[0].real) {
+            const int64_t first = a.c.indptr[e] + run + i * KB;
+#pragma unroll
+            for (int h = 0; h < KB; ++h)
+              if (there >> (i * KB + h) & 1) *reinterpret_cast<f32x4*>(a.scores + ((((first + h) * a.c.kv_heads + head) * a.score_rows + n) * kKv8Page + 4 * g)) = s[0][h];
           }
         }
         bf16x8_t pf[NT][KB / 2][NP];
@@ -314,16 +324,57 @@ __device__ __forceinline__ void put_mass(const MassArgs& w, int page, int at, fl
   w.out[page * w.out_stride + at] = w.keep == 0.f ? x : fmaf(w.keep, w.mass[page * w.mass_stride + at], x);
 }
 
-template <typename T, int D> constexpr int mass_blocks() { return D == 256 ? 2 : 4; }
+// a lane's part of a row of queries as loaded
+template <typename T, int C>
+struct RawQuery {
+  typedef __attribute__((ext_vector_type(4))) std::conditional_t<sizeof(T) == 2, uint32_t, float> Words;
+  Words w[C][sizeof(T)];
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T); ++i) w[c][i] = reinterpret_cast<const Words*>(p + c * 64)[i];
+  }
+  __device__ __forceinline__ void part(int c, int k, bf16x8_t* q) const {
+    if constexpr (sizeof(T) == 2) {
+      q[0] = __builtin_bit_cast(bf16x8_t, w[c][k]);
+    } else {
+      float x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = w[c][2 * k + i / 4][i & 3];
+      kv8_split<3>(x, q);
+    }
+  }
+};
+
+// Blocks of keys of a wave: a tile of sixteen rows, 32 D bytes, then feeds 2 D clocks of the matrix cores; eight blocks of 128 values spill (18 to 55 registers).
+constexpr int kMassBlocks = 4;
 
 template <typename T, int FMT, int D>
-__global__ __launch_bounds__(256, 2) void kv8_mass_kernel(AttnArgs a, MassArgs w) {
-  constexpr int NP = kv8_parts<T>(), C = D / 64, MB = mass_blocks<T, D>();
+__global__ __launch_bounds__(256, (sizeof(T) == 2 ? 2 : 1)) void kv8_mass_kernel(AttnArgs a, MassArgs w) {
+  constexpr int NP = kv8_parts<T>(), C = D / 64, MB = kMassBlocks;
   const int e = blockIdx.z, head = blockIdx.y, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   const RowSpan rows = row_span(a.row0, e, a.n_rows);
   const int start = a.starts[e], total = rows.n * a.group;
   if (rows.n == 0 || start < 0 || start > INT32_MAX - 2048 - rows.n) return;
   const int blocks = (start + rows.n + kKv8Page - 1) / kKv8Page, slice = blockIdx.x % w.n_slice, tiles = (total + 15) / 16;
+  if (a.scores && total <= a.score_rows) {
+    // a step: the attention left its scores, 4 bytes a row and token beside D of the keys
+    const int len = start + rows.n;
+    for (int slot = blockIdx.x * 256 + threadIdx.x; slot < len; slot += gridDim.x * 256) {
+      const int block = slot / kKv8Page, page = a.c.page(e, block);
+      if (page < 0) continue;
+      const float* s = a.scores + (((int64_t)a.c.indptr[e] + block) * a.c.kv_heads + head) * a.score_rows * kKv8Page + slot % kKv8Page;
+      float x = 0.f;
+#pragma unroll 4
+      for (int rr = 0; rr < total; ++rr) {
+        const int tok = rr / a.group;
+        x += exp2_of(s[rr * kKv8Page] - a.lse[(int64_t)(rows.first + tok) * a.heads + head * a.group + rr - tok * a.group]);
+      }
+      put_mass(w, page, head * kKv8Page + slot % kKv8Page, x);
+    }
+    return;
+  }
   for (int b0 = (blockIdx.x / w.n_slice * 4 + wave) * MB; b0 < blocks; b0 += gridDim.x / w.n_slice * 4 * MB) {
     int page[MB];
     float ks[MB];
@@ -350,10 +401,18 @@ __global__ __launch_bounds__(256, 2) void kv8_mass_kernel(AttnArgs a, MassArgs w
     for (int h = 0; h < MB; ++h) sum[h] = f32x4{0.f, 0.f, 0.f, 0.f};
     const int slot0 = b0 * kKv8Page, first = (int)((int64_t)max(slot0 - start, 0) * a.group / 16);     // the first tile with a row that sees a block
     const int per = (tiles - first + w.n_slice - 1) / w.n_slice, last = min(tiles, first + (slice + 1) * per);
+    // a row tile's queries and sums are on their way while the tile before is weighed
+    QueryRow r = query_row((first + slice * per) * 16 + n, total, a.group, rows, start, head);
+    RawQuery<T, C> raw, next;
+    float lse, next_lse;
+    auto fetch = [&](const QueryRow& y, RawQuery<T, C>& to, float& sum_of) {
+      to.load(static_cast<const T*>(a.q) + y.row * a.q_stride + (int64_t)y.head * D + g * 16);
+      sum_of = a.lse[(int64_t)y.row * a.heads + y.head];
+    };
+    fetch(r, raw, lse);
     for (int tile = first + slice * per; tile < last; ++tile) {
-      const QueryRow r = query_row(tile * 16 + n, total, a.group, rows, start, head);
-      const T* qp = static_cast<const T*>(a.q) + r.row * a.q_stride + (int64_t)r.head * D + g * 16;
-      const float lse = r.real ? a.lse[(int64_t)r.row * a.heads + r.head] : INFINITY;      // a row behind the last weighs nothing
+      const QueryRow after = query_row((tile + 1) * 16 + n, total, a.group, rows, start, head);
+      fetch(after, next, next_lse);
       f32x4 s[MB];
 #pragma unroll
       for (int h = 0; h < MB; ++h) s[h] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -362,12 +421,13 @@ __global__ __launch_bounds__(256, 2) void kv8_mass_kernel(AttnArgs a, MassArgs w
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           bf16x8_t q[NP];
-          kv8_query(qp + c * 64 + 8 * k, q);
+          raw.part(c, k, q);
 #pragma unroll
           for (int p = NP - 1; p >= 0; --p)
 #pragma unroll
             for (int h = 0; h < MB; ++h) s[h] = mfma16(kf[h][c][k], q[p], s[h]);
         }
+      if (!r.real) lse = INFINITY;      // a row behind the last weighs nothing
       const bool all = slot0 + MB * kKv8Page - 1 <= tile * 16 / a.group + start;           // every row of the tile sees every slot
 #pragma unroll
       for (int h = 0; h < MB; ++h)
@@ -376,6 +436,9 @@ __global__ __launch_bounds__(256, 2) void kv8_mass_kernel(AttnArgs a, MassArgs w
           const float p = exp2_of(fmaf(s[h][i], ks[h], -lse));
           sum[h][i] += all || slot0 + h * kKv8Page + 4 * g + i <= r.far ? p : 0.f;
         }
+      r = after;
+      raw = next;
+      lse = next_lse;
     }
 #pragma unroll
     for (int h = 0; h < MB; ++h)
@@ -407,7 +470,7 @@ __global__ __launch_bounds__(256) void kv8_mass_sum_kernel(AttnArgs a, MassArgs 
 }
 
 // How a call is cut: rows of a workgroup, splits of the keys and slices of the weights' rows where those leave too few workgroups.
-struct AttnPlan { int tiles, row_tiles, n_split, split_blocks, mass_groups, n_slice; };
+struct AttnPlan { int tiles, row_tiles, n_split, split_blocks, mass_groups, n_slice, score_rows; };
 inline AttnPlan attn_plan(const pegainfer_kv8_cache* cache, int n_rows, int max_rows, int max_len, int heads, int dtype) {
   AttnPlan p;
   const int64_t rows = (int64_t)std::min(max_rows, n_rows) * (heads / cache->kv_heads), pairs = (int64_t)cache->kv_heads * cache->n_entries;
@@ -418,10 +481,13 @@ inline AttnPlan attn_plan(const pegainfer_kv8_cache* cache, int n_rows, int max_
   auto cut = [&](int64_t groups, int64_t most) { return (int)std::max<int64_t>(1, std::min((want + groups - 1) / groups, most)); };
   p.n_split = cut(p.tiles * pairs, std::min((blocks + 15) / 16, 256));
   p.split_blocks = ceil_div(blocks, p.n_split);
-  p.mass_groups = ceil_div(blocks, 4 * (cache->dim == 256 ? 2 : 4));
+  p.score_rows = rows <= 16 ? (int)rows : 0;
+  p.mass_groups = p.score_rows ? ceil_div(blocks, 256 / kKv8Page) : ceil_div(blocks, 4 * kMassBlocks);
   p.n_slice = cut(p.mass_groups * pairs, std::min<int64_t>((rows + 255) / 256, 16));
   return p;
 }
+// the splits' sums and states of a workspace, up to 16 bytes
+inline int64_t split_floats(const AttnPlan& p, int64_t row_heads, int dim) { return p.n_split > 1 ? (row_heads * p.n_split * (dim + 2) + 3) / 4 * 4 : 0; }
 
 }  // namespace pk
 
@@ -434,8 +500,9 @@ int64_t pegainfer_kv8_attention_workspace(const pegainfer_kv8_cache* cache, int3
   if (!kv8_ok(cache) || n_rows <= 0 || max_rows <= 0 || max_len < 0 || heads < cache->kv_heads || cache->n_entries == 0) return 0;
   const AttnPlan p = attn_plan(cache, n_rows, max_rows, max_len, heads, dtype);
   const int64_t rh = (int64_t)n_rows * heads;
-  return (p.n_split > 1 ? rh * p.n_split * (cache->dim + 2) : 0) + (with_mass ? rh : 0) +
-         (with_mass && p.n_slice > 1 ? (int64_t)p.n_slice * cache->n_page_ids * cache->kv_heads * kKv8Page : 0);
+  const int64_t slots = (int64_t)cache->n_page_ids * cache->kv_heads * kKv8Page;
+  return split_floats(p, rh, cache->dim) +
+         (with_mass ? (rh + 3) / 4 * 4 + (p.n_slice > 1 ? p.n_slice * slots : 0) + p.score_rows * slots : 0);
 }
 
 pegainfer_status_t pegainfer_kv8_attention(const pegainfer_kv8_cache* cache, const pegainfer_kv8_attn_desc* d, pegainfer_stream_t stream) {
@@ -454,13 +521,16 @@ pegainfer_status_t pegainfer_kv8_attention(const pegainfer_kv8_cache* cache, con
   const AttnPlan p = attn_plan(cache, d->n_rows, d->max_rows, d->max_len, d->heads, d->dtype);
   if ((weigh || p.n_split > 1) && (!d->workspace || !host_aligned16(d->workspace))) return PK_BAD;
   const int64_t rh = (int64_t)d->n_rows * d->heads;
-  float* part_ml = d->workspace + (p.n_split > 1 ? rh * p.n_split * cache->dim : 0);
+  // workspace: the splits' sums and states, the rows' log-sums, then either the slices' sums or the scores (never both: those are of few rows)
+  float* const part_ml = p.n_split > 1 ? d->workspace + rh * p.n_split * cache->dim : nullptr;
+  float* const lse = weigh ? d->workspace + split_floats(p, rh, cache->dim) : nullptr;
+  float* const rest = weigh ? lse + (rh + 3) / 4 * 4 : nullptr;
   const AttnArgs a{kv8_of(cache), d->q, d->q_row_stride, d->out_row_stride, d->row0, d->starts, d->n_rows, group, d->heads, p.n_split, p.split_blocks,
-                   d->scale * 1.4426950408889634f, d->out, weigh ? part_ml + (p.n_split > 1 ? rh * p.n_split * 2 : 0) : nullptr, d->workspace, part_ml};
+                   d->scale * 1.4426950408889634f, d->out, lse, d->workspace, part_ml, p.score_rows ? rest : nullptr, p.score_rows};
   const dim3 grid(p.tiles * p.n_split, cache->kv_heads, cache->n_entries);
   const dim3 merge_grid(std::min(d->max_rows, d->n_rows) * group * (cache->dim / 64), cache->kv_heads, cache->n_entries);
   const dim3 mass_grid(p.mass_groups * p.n_slice, cache->kv_heads, cache->n_entries), sum_grid(std::max(1, ceil_div(d->max_len, 256)), cache->kv_heads, cache->n_entries);
-  const MassArgs w{d->mass, d->mass_out, weigh ? a.lse + rh : nullptr, d->mass_page_stride, d->mass_out_page_stride, d->mass_keep, p.n_slice};
+  const MassArgs w{d->mass, d->mass_out, rest, d->mass_page_stride, d->mass_out_page_stride, d->mass_keep, p.n_slice};
   kv8_by(d->dtype, cache->format, cache->dim, [&](auto* t, auto fmt, auto dim) {
     using T = std::remove_pointer_t<decltype(t)>;
     constexpr int D = dim();

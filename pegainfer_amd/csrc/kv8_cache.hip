@@ -103,29 +103,49 @@ __global__ __launch_bounds__(128) void kv8_read_kernel(Kv8 c, T* k, T* v, const 
   for (int b = (int)start / kKv8Page + blockIdx.x; b * kKv8Page < end; b += gridDim.x) {
     const int page = c.page(e, b), low = b * kKv8Page;
     const float scale = page < 0 ? 0.f : *c.scale(page, side, head);
+    const uint8_t* blk = page < 0 ? nullptr : c.block(page, side, head, D);
+    if (side == 0) {
+      // 16 bytes of a row a lane, so that 64 consecutive values leave together
+      constexpr int N = 16 / sizeof(T), PER = 64 / N;
 #pragma unroll
-    for (int ch = 0; ch < D / 64; ++ch) {
-      u32x4 w = {0, 0, 0, 0};
-      if (page >= 0) w = *reinterpret_cast<const u32x4*>(c.block(page, side, head, D) + unit_at(side, ch, n, q));
-      float x[16];
+      for (int i = 0; i < 16 * D / (64 * N); ++i) {
+        const int u = i * 64 + lane, ch = u / (16 * PER), t = u / PER % 16, at = u % PER * N, s = low + t;
+        uint32_t w[N / 4] = {};
+        if (blk) __builtin_memcpy(w, blk + u * N, N);
+        float x[N];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) kv8_numbers<FMT>(w[i], x + 4 * i);
+        for (int j = 0; j < N / 4; ++j) kv8_numbers<FMT>(w[j], x + 4 * j);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) x[i] *= scale;
-      if (side == 0) {
-        const int s = low + n;
-        if (s >= start && s < end) {
-          T* p = base + (rows.first + (s - start)) * stride + ch * 64 + q * 16;
-          Vec8<T>::store(p, x);
-          Vec8<T>::store(p + 8, x + 8);
-        }
-      } else {
+        for (int j = 0; j < N; ++j) x[j] *= scale;
+        if (s < start || s >= end) continue;
+        T* p = base + (rows.first + (s - start)) * stride + ch * 64 + at;
+        if constexpr (N == 8) Vec8<T>::store(p, x);
+        else st4(p, x);
+      }
+    } else {
+      // a quad's four tokens of 16 bytes of a row a lane
+      constexpr int N = 16 / sizeof(T), PER = 64 / N;
+#pragma unroll
+      for (int i = 0; i < (4 * D / N + 63) / 64; ++i) {
+        const int u = i * 64 + lane, ch = u / (4 * PER), quad = u / PER % 4, at = u % PER * N;
+        if (u >= 4 * D / N) break;
+        u32x4 w[N / 4] = {};
+        if (blk)
+#pragma unroll
+          for (int j = 0; j < N / 4; ++j) w[j] = reinterpret_cast<const u32x4*>(blk + u * N * 4)[j];
+        float x[4 * N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) kv8_numbers<FMT>(w[j / 4][j & 3], x + 4 * j);
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-          const int s = low + 4 * q + t;
+          const int s = low + 4 * quad + t;
           if (s < start || s >= end) continue;
-          const float y[4] = {x[t], x[4 + t], x[8 + t], x[12 + t]};
-          st4(base + (rows.first + (s - start)) * stride + ch * 64 + 4 * n, y);
+          float y[N];
+#pragma unroll
+          for (int j = 0; j < N; ++j) y[j] = x[4 * j + t] * scale;
+          T* p = base + (rows.first + (s - start)) * stride + ch * 64 + at;
+          if constexpr (N == 8) Vec8<T>::store(p, y);
+          else st4(p, y);
         }
       }
     }
@@ -141,13 +161,16 @@ __device__ __forceinline__ uint32_t order_of(float m) {
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-// Which tokens stay: one workgroup an (entry, head).  Four passes of a histogram over eight bits give the weight of the lightest token that stays among those
-// between the first and the last ones, a pass with running counts in slot order writes the slots that stay; of equal weights the lowest slots do.
-constexpr int kPickThreads = 1024;
+// Which tokens stay: one workgroup an (entry, head).  Three histograms over 11, 11 and 10 bits of the weights' order give the lightest weight that stays among those
+// between the first and the last tokens; then every wave counts, and after a barrier writes, the slots that stay of a run of its own, in order: of equal weights the
+// lowest slots.  Bound by the latency of few workgroups, so the weights are fetched once, through their pages, and kept in shared memory where they fit
+// (36 864 tokens; beyond that every pass fetches them).  11 bits reach into the mantissa: weights share few exponents, and counts of one address are taken in turn.
+constexpr int kPickThreads = 1024, kPickWaves = kPickThreads / 64, kPickCached = 36864;
 __global__ __launch_bounds__(kPickThreads) void kv8_pick_kernel(Kv8 c, const float* mass, int64_t mass_stride, const int32_t* lens, int budget, int keep_first,
-                                                                int keep_last, int32_t* kept) {
-  __shared__ uint32_t hist[256];
-  __shared__ int wave_n[2][kPickThreads / 64];
+                                                                int keep_last, int cached, int32_t* kept) {
+  extern __shared__ uint32_t s_order[];
+  __shared__ uint32_t hist[2048];
+  __shared__ int s_sure[kPickWaves], s_ties[kPickWaves], s_sum[kPickWaves];
   __shared__ uint32_t s_bits;
   __shared__ int s_left;
   const int e = blockIdx.y, head = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -157,62 +180,87 @@ __global__ __launch_bounds__(kPickThreads) void kv8_pick_kernel(Kv8 c, const flo
     for (int i = tid; i < budget; i += kPickThreads) out[i] = i < len ? i : -1;
     return;
   }
-  auto weight = [&](int s) {
+  auto fetch = [&](int s) {
     const int page = c.page(e, s / kKv8Page);
     return page < 0 ? 0u : order_of(mass[page * mass_stride + head * kKv8Page + s % kKv8Page]);
   };
-  const int lo = keep_first, hi = len - keep_last;
-  uint32_t bits = 0;                       // the weight so far: its upper bits
-  int left = budget - keep_first - keep_last;   // tokens still to be found at or below it
-  if (left > 0) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      if (tid < 256) hist[tid] = 0;
+  const bool held = len <= cached;
+  if (held) {
+#pragma unroll 8
+    for (int s = tid; s < len; s += kPickThreads) s_order[s] = fetch(s);
+  }
+  auto weight = [&](int s) { return held ? s_order[s] : fetch(s); };
+  const int lo = keep_first, hi = len - keep_last, chosen = budget - keep_first - keep_last;
+  uint32_t bits = 0;                       // of the lightest weight that stays: its upper bits so far
+  int left = chosen;                       // tokens still to be found that have those
+  if (chosen > 0) {
+    for (int done = 0; done < 32; done += 11) {
+      const int width = min(11, 32 - done), shift = 32 - done - width;
+      for (int i = tid; i < 2048; i += kPickThreads) hist[i] = 0;
       __syncthreads();
-      const uint32_t mask = shift == 24 ? 0u : 0xFFFFFFFFu << (shift + 8);
+      const uint32_t mask = done == 0 ? 0u : 0xFFFFFFFFu << (32 - done);
+#pragma unroll 4
       for (int s = lo + tid; s < hi; s += kPickThreads) {
         const uint32_t w = weight(s);
-        if ((w & mask) == bits) atomicAdd(&hist[(w >> shift) & 255], 1u);
+        if ((w & mask) == bits) atomicAdd(&hist[(w >> shift) & 2047 >> (11 - width)], 1u);
       }
       __syncthreads();
-      if (tid == 0) {
-        int n = left, d = 255;
-        for (; d > 0 && (int)hist[d] < n; --d) n -= (int)hist[d];
-        s_bits = bits | (uint32_t)d << shift;
-        s_left = n;
+      // thread t: digits 2047 - 2 t and 2046 - 2 t; how many weights have a larger digit
+      const int a = (int)hist[2047 - 2 * tid], b = (int)hist[2046 - 2 * tid];
+      int sum = a + b;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const int o = __shfl_up(sum, d, 64);
+        if (lane >= d) sum += o;
+      }
+      if (lane == 63) s_sum[wave] = sum;
+      __syncthreads();
+      for (int i = 0; i < wave; ++i) sum += s_sum[i];
+      const int above = sum - a - b;
+      if (above < left && left <= sum) {   // one thread: the counts reach `left` in its two digits
+        const bool second = left > above + a;
+        s_bits = bits | (uint32_t)(2047 - 2 * tid - second) << shift;
+        s_left = left - above - (second ? a : 0);
       }
       __syncthreads();
       bits = s_bits;
       left = s_left;
     }
   }
-  int at = 0, ties = 0;                    // tokens kept, and ties met, in the slots before
-  for (int s0 = 0; s0 < len; s0 += kPickThreads) {
-    const int s = s0 + tid;
-    const bool in = s < len, always = in && (s < lo || s >= hi);
-    const uint32_t w = in && !always ? weight(s) : 0u;
-    const bool tie = in && !always && budget - keep_first - keep_last > 0 && w == bits;
-    const uint64_t tie_mask = __builtin_amdgcn_ballot_w64(tie), below = (1ull << lane) - 1;
-    if (lane == 0) wave_n[0][wave] = __popcll(tie_mask);
-    __syncthreads();
-    int tie_at = ties;
-    for (int i = 0; i < kPickThreads / 64; ++i) {
-      const int n = wave_n[0][i];
-      ties += n;
-      tie_at += i < wave ? n : 0;
-    }
-    tie_at += __popcll(tie_mask & below);
-    const bool stays = always || (in && !always && budget - keep_first - keep_last > 0 && (w > bits || (tie && tie_at < left)));
+  __syncthreads();
+  const int run = (len + kPickThreads - 1) / kPickThreads * 64, from = min(wave * run, len), to = min(from + run, len);
+  auto look = [&](int s, bool& sure, bool& tie) {
+    const bool in = s < to, always = in && (s < lo || s >= hi);
+    const uint32_t w = in && !always && chosen > 0 ? weight(s) : 0u;
+    sure = always || (in && chosen > 0 && w > bits);
+    tie = in && !always && chosen > 0 && w == bits;
+  };
+  int sures = 0, ties = 0;
+  for (int s = from; s < to; s += 64) {
+    bool sure, tie;
+    look(s + lane, sure, tie);
+    sures += __popcll(__builtin_amdgcn_ballot_w64(sure));
+    ties += __popcll(__builtin_amdgcn_ballot_w64(tie));
+  }
+  if (lane == 0) { s_sure[wave] = sures; s_ties[wave] = ties; }
+  __syncthreads();
+  int at = 0, tied = 0;                    // tokens that stay, and ties met, in the slots before
+  for (int i = 0; i < wave; ++i) {
+    at += s_sure[i];
+    tied += s_ties[i];
+  }
+  at += min(tied, left);
+  const uint64_t below = (1ull << lane) - 1;
+  for (int s = from; s < to; s += 64) {
+    bool sure, tie;
+    look(s + lane, sure, tie);
+    const uint64_t tie_mask = __builtin_amdgcn_ballot_w64(tie);
+    const bool stays = sure || (tie && tied + __popcll(tie_mask & below) < left);
     const uint64_t mask = __builtin_amdgcn_ballot_w64(stays);
-    if (lane == 0) wave_n[1][wave] = __popcll(mask);
-    __syncthreads();
-    int to = at;
-    for (int i = 0; i < kPickThreads / 64; ++i) {
-      const int n = wave_n[1][i];
-      at += n;
-      to += i < wave ? n : 0;
-    }
-    to += __popcll(mask & below);
-    if (stays && to < budget) out[to] = s;
+    const int to_at = at + __popcll(mask & below);
+    if (stays && to_at < budget) out[to_at] = s + lane;
+    at += __popcll(mask);
+    tied += __popcll(tie_mask);
   }
 }
 
@@ -329,7 +377,9 @@ pegainfer_status_t pegainfer_kv8_evict(const pegainfer_kv8_cache* cache, float* 
   if (cache->n_entries == 0) return 0;
   if (!mass || !lens || !dst_indptr || (!dst_ids && n_dst_ids > 0) || !kept || mass_page_stride < (int64_t)cache->kv_heads * kKv8Page) return PK_BAD;
   const Kv8 c = kv8_of(cache);
-  kv8_pick_kernel<<<dim3(c.kv_heads, c.entries), kPickThreads, 0, as_stream(stream)>>>(c, mass, mass_page_stride, lens, budget, keep_first, keep_last, kept);
+  const int cached = std::min(max_len, kPickCached);
+  if (hipFuncSetAttribute(reinterpret_cast<const void*>(kv8_pick_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kPickCached * 4) != hipSuccess) return PK_BAD;
+  kv8_pick_kernel<<<dim3(c.kv_heads, c.entries), kPickThreads, cached * 4, as_stream(stream)>>>(c, mass, mass_page_stride, lens, budget, keep_first, keep_last, cached, kept);
   const dim3 grid(std::max(1, ceil_div(std::min(budget, max_len), kKv8Page)), c.kv_heads, c.entries);
   kv8_by(kDtBf16, cache->format, cache->dim, [&](auto*, auto fmt, auto dim) {
     kv8_move_kernel<fmt(), dim()><<<grid, 128, 0, as_stream(stream)>>>(c, dst_indptr, dst_ids, n_dst_ids, mass, mass_page_stride, lens, budget, kept);

@@ -966,18 +966,21 @@ def _kv8_index(t, n, codes, what):
 
 def _kv8_cache(codes, scales, page_indptr, page_ids, entries):
     """-> (descriptor, kv_heads, dim); refuses what the kernels do not take"""
-    fmt, shape, stride = KV8_FORMATS.get(codes.dtype), codes.shape, codes.stride()
-    _kv8_need(fmt is not None, "codes of torch.float8_e4m3fn or torch.int8")
-    _kv8_need(codes.is_cuda and codes.get_device() == torch.cuda.current_device(), "a cache on the current device")
-    _kv8_need(len(shape) == 4 and shape[1] == 2 and shape[3] in (1024, 2048, 4096) and shape[0] >= 1, "codes [pages, 2, kv_heads, 16 * dim], a page at least, dim 64, 128 or 256")
+    fmt, shape, stride, sstride = KV8_FORMATS.get(codes.dtype), codes.shape, codes.stride(), scales.stride()
+    if fmt is None:
+        raise ValueError("kv8: codes of torch.float8_e4m3fn or torch.int8")
+    if not codes.is_cuda or codes.get_device() != torch.cuda.current_device():
+        raise ValueError("kv8: a cache on the current device")
+    if len(shape) != 4 or shape[1] != 2 or shape[3] not in (1024, 2048, 4096) or shape[0] < 1:
+        raise ValueError("kv8: codes [pages, 2, kv_heads, 16 * dim], a page at least, dim 64, 128 or 256")
     pages, _, kv, m = shape
     at = codes.data_ptr()
-    _kv8_need(stride[3] == 1 and stride[2] == m and stride[1] == kv * m and stride[0] >= 2 * kv * m and (stride[0] | at) % 16 == 0,
-              "codes: a page's values together, pages apart by a multiple of 16 bytes")
-    sstride = scales.stride()
-    _kv8_need(scales.dtype is _F32 and scales.device == codes.device and scales.shape == shape[:3] and sstride[2] == 1 and sstride[1] == kv and sstride[0] >= 2 * kv,
-              "scales fp32 [pages, 2, kv_heads] on the cache's device, a page's together")
-    _kv8_need(1 <= kv <= 65535 and entries <= 65535, "at most 65535 kv heads and entries")
+    if stride[3] != 1 or stride[2] != m or stride[1] != kv * m or stride[0] < 2 * kv * m or (stride[0] | at) % 16:
+        raise ValueError("kv8: codes: a page's values together, pages apart by a multiple of 16 bytes")
+    if scales.dtype is not _F32 or scales.device != codes.device or scales.shape != shape[:3] or sstride[2] != 1 or sstride[1] != kv or sstride[0] < 2 * kv:
+        raise ValueError("kv8: scales fp32 [pages, 2, kv_heads] on the cache's device, a page's together")
+    if not 1 <= kv <= 65535 or entries > 65535:
+        raise ValueError("kv8: at most 65535 kv heads and entries")
     return Kv8Cache(at, scales.data_ptr(), stride[0], sstride[0], fmt, pages, kv, m // 16, _kv8_index(page_indptr, entries + 1, codes, "page_indptr"),
                     _kv8_index(page_ids, None, codes, "page_ids"), page_ids.numel(), entries), kv, m // 16
 
