@@ -10,9 +10,28 @@ namespace pk {
 
 __device__ __forceinline__ f32x4 mfma16(const bf16x8_t& a, const bf16x8_t& b, const f32x4& c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float max3(float a, float b, float c) {   // NaN among them does not count
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+// the other half's (of 32) and the other row's (of 16) value, without a trip through shared memory; s_nop: the wait states between a VALU write and the swap.  In
+// assembly because the swap wants two registers, and the builtin given one value twice may be folded to one.
+template <typename Op>
+__device__ __forceinline__ float across_quad(float v, Op op) {
+  float a = v, b = v;
+  asm("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(a), "+v"(b));
+  a = op(a, b);
+  b = a;
+  asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(a), "+v"(b));
+  return op(a, b);
+}
 // over the four lanes that hold a row's scores
-__device__ __forceinline__ float quad_max(float v) { v = fmaxf(v, __shfl_xor(v, 16, 64)); return fmaxf(v, __shfl_xor(v, 32, 64)); }
-__device__ __forceinline__ float quad_sum(float v) { v += __shfl_xor(v, 16, 64); return v + __shfl_xor(v, 32, 64); }
+__device__ __forceinline__ float quad_max(float v) { return across_quad(v, [](float x, float y) { return fmaxf(x, y); }); }
+__device__ __forceinline__ float quad_sum(float v) { return across_quad(v, [](float x, float y) { return x + y; }); }
+// The maximum that a row's weights are taken against moves only when a score passes it by 2^kSlack: weights up to 2^8 round like those up to 1, and most steps
+// need no exchange between lanes and no rescaling.
+constexpr float kSlack = 8.f;
 
 struct AttnArgs {
   Kv8 c;
@@ -33,6 +52,36 @@ struct QueryRow { int row, head, far; bool real; };   // far: the last slot that
 __device__ __forceinline__ QueryRow query_row(int rr, int total, int group, const RowSpan& rows, int start, int kv_head) {
   const int r = min(rr, total - 1), tok = r / group;
   return {rows.first + tok, kv_head * group + r - tok * group, start + tok, rr < total};
+}
+
+constexpr int kPromptRows = 128, kFewSplits = 4;
+
+// a lane's part of a row's result: the output, or what a split leaves of it
+template <typename T, int D>
+__device__ __forceinline__ void put_row(const AttnArgs& a, const QueryRow& r, int split, int g, float m, float l, const f32x4 (&o)[D / 16]) {
+  const bool some = l > 0.f || l != l;
+  const float inv = a.n_split > 1 ? 1.f : some ? 1.f / l : 0.f;   // no key: zeros
+  const int64_t rh = (int64_t)r.row * a.heads + r.head;
+  auto put = [&](auto* op) {
+    using O = std::remove_pointer_t<decltype(op)>;
+#pragma unroll
+    for (int c = 0; c < D / 64; ++c) {
+      float x[16];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[4 * i + j] = o[4 * c + j][i] * inv;
+      Vec8<O>::store(op + g * 16 + c * 64, x);
+      Vec8<O>::store(op + g * 16 + c * 64 + 8, x + 8);
+    }
+  };
+  if (a.n_split > 1) {
+    if (some) put(a.part_o + (rh * a.n_split + split) * D);
+    if (g == 0) *reinterpret_cast<f32x2*>(a.part_ml + (rh * a.n_split + split) * 2) = f32x2{m, l};
+  } else {
+    put(static_cast<T*>(a.out) + r.row * a.out_stride + (int64_t)r.head * D);
+    if (a.lse && g == 0) a.lse[rh] = some ? m + __log2f(l) : INFINITY;
+  }
 }
 
 // Blocks a wave takes at a time, and waves of a SIMD: what the registers hold without spilling.  bf16 heads of 128: 189 registers a wave for one row tile, 256 for two.
@@ -149,19 +198,31 @@ __global__ __launch_bounds__(256, (attn_waves<T, D, NT>())) void kv8_attn_kernel
           }
         }
         bf16x8_t pf[NT][KB / 2][NP];
-        float alpha[NT];
+        float top[NT], alpha[NT];
+        bool moves = false;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-          float mx = m[t];
+          top[t] = s[t][0][0];
 #pragma unroll
-          for (int h = 0; h < KB; ++h)
+          for (int h = 0; h < KB; ++h) top[t] = max3(max3(top[t], s[t][h][0], s[t][h][1]), s[t][h][2], s[t][h][3]);
+          moves |= top[t] > m[t] + kSlack;
+          alpha[t] = 1.f;
+        }
+        if (__builtin_amdgcn_ballot_w64(moves)) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) mx = fmaxf(mx, s[t][h][j]);
-          mx = quad_max(mx);
-          const float base = mx == -INFINITY ? 0.f : mx;
-          alpha[t] = exp2_of(m[t] - base);
-          m[t] = mx;
-          l[t] *= alpha[t];
+          for (int t = 0; t < NT; ++t) {
+            const float mx = quad_max(top[t]), to = mx > m[t] + kSlack ? mx : m[t];
+            alpha[t] = to == -INFINITY ? 1.f : exp2_of(m[t] - to);
+            m[t] = to;
+            l[t] *= alpha[t];
+            if constexpr (NP == 1)
+#pragma unroll
+              for (int d = 0; d < D / 16; ++d) o[t][d] *= alpha[t];
+          }
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          const float base = m[t] == -INFINITY ? 0.f : m[t];
 #pragma unroll
           for (int h = 0; h < KB; h += 2) {
             float p[8];
@@ -176,13 +237,6 @@ __global__ __launch_bounds__(256, (attn_waves<T, D, NT>())) void kv8_attn_kernel
         }
         // fp32 sums of many keys are added outside the matrix cores, whose accumulation does not round to nearest
         constexpr bool kOutside = NP > 1;
-        if (!kOutside) {
-#pragma unroll
-          for (int t = 0; t < NT; ++t)
-            if (__builtin_amdgcn_ballot_w64(alpha[t] != 1.f))
-#pragma unroll
-              for (int d = 0; d < D / 16; ++d) o[t][d] *= alpha[t];
-        }
 #pragma unroll
         for (int c = 0; c < C; ++c)
 #pragma unroll
@@ -226,33 +280,214 @@ __global__ __launch_bounds__(256, (attn_waves<T, D, NT>())) void kv8_attn_kernel
           for (int i = 0; i < D / 16; ++i) o[t][i] = o[t][i] * x + s_o[wave][i][lane] * y;
         }
       }
-      if (wave == 0 && r[t].real) {
-        const bool some = l[t] > 0.f || l[t] != l[t];
-        const float inv = a.n_split > 1 ? 1.f : some ? 1.f / l[t] : 0.f;   // no key: zeros
-        const int64_t rh = (int64_t)r[t].row * a.heads + r[t].head;
-        auto put = [&](auto* op) {
-          using O = std::remove_pointer_t<decltype(op)>;
-#pragma unroll
-          for (int c = 0; c < C; ++c) {
-            float x[16];
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-              for (int j = 0; j < 4; ++j) x[4 * i + j] = o[t][4 * c + j][i] * inv;
-            Vec8<O>::store(op + g * 16 + c * 64, x);
-            Vec8<O>::store(op + g * 16 + c * 64 + 8, x + 8);
-          }
-        };
-        if (a.n_split > 1) {
-          if (some) put(a.part_o + (rh * a.n_split + split) * D);
-          if (g == 0) *reinterpret_cast<f32x2*>(a.part_ml + (rh * a.n_split + split) * 2) = f32x2{m[t], l[t]};
-        } else {
-          put(static_cast<T*>(a.out) + r[t].row * a.out_stride + (int64_t)r[t].head * D);
-          if (a.lse && g == 0) a.lse[rh] = some ? m[t] + __log2f(l[t]) : INFINITY;
-        }
-      }
+      if (wave == 0 && r[t].real) put_row<T, D>(a, r[t], split, g, m[t], l[t], o[t]);
     }
     __syncthreads();
+  }
+}
+
+// Prompts: one workgroup, 128 query rows of a kv head.  Every step's blocks of keys and values (16 KB of codes, 32 KB as operands) are widened once, an equal share by
+// every wave, into one of two buffers of shared memory, while the other is read: a code is widened once for 128 rows and not for 32, and no states are joined at
+// the end.  Operands lie in shared memory as the lanes read them, 16 bytes a lane, without bank conflicts.  Four waves of 32 rows read least (D <= 128: 224 registers);
+// heads of 256 take eight waves of 16 rows, whose outputs and queries fit beside the rest.
+template <int D> constexpr int prompt_blocks() { return 512 / D; }   // of a step
+template <int D> constexpr int prompt_tiles() { return D == 256 ? 1 : 2; }   // of sixteen rows, a wave
+
+template <int FMT, int D>
+__global__ __launch_bounds__(64 * 8 / prompt_tiles<D>(), 2) void kv8_prompt_kernel(AttnArgs a) {
+  typedef uint16_t T;
+  constexpr int C = D / 64, KB = prompt_blocks<D>(), NT = prompt_tiles<D>();
+  // a step is 8 units of keys (a block's 64 values) and 4 of values (a pair of blocks' 64): four waves take two and one, of eight the first four one of values, the others two of keys
+  constexpr bool kRoles = NT == 1;
+  constexpr int kSets = D == 256 ? 2 : 1;   // steps of codes on their way to the registers
+  constexpr bool kScaled = FMT == kE4m3;
+  // keys [block][chunk][half], then values [pair of blocks][chunk][value of the lane's four]
+  __shared__ bf16x8_t s_kv[2][2 * KB * C + 2 * KB * C][64];
+  const int e = blockIdx.z, head = blockIdx.y, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+  const RowSpan rows = row_span(a.row0, e, a.n_rows);
+  const int start = a.starts[e], total = rows.n * a.group;
+  if (rows.n == 0 || start < 0 || start > INT32_MAX - 2048 - rows.n) return;
+  const int len = start + rows.n, n_tiles = (total + kPromptRows - 1) / kPromptRows, split = blockIdx.x % a.n_split, stride = gridDim.x / a.n_split;
+  for (int at = blockIdx.x / a.n_split; at < n_tiles; at += stride) {
+    const int tile = n_tiles - 1 - at;     // the rows that see most first
+    QueryRow r[NT];
+    bf16x8_t qf[NT][C][2];
+    float m[NT], l[NT];
+    f32x4 o[NT][D / 16];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      r[t] = query_row(tile * kPromptRows + (wave * NT + t) * 16 + n, total, a.group, rows, start, head);
+      const T* qp = static_cast<const T*>(a.q) + r[t].row * a.q_stride + (int64_t)r[t].head * D + g * 16;
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        kv8_query(qp + c * 64, &qf[t][c][0]);
+        kv8_query(qp + c * 64 + 8, &qf[t][c][1]);
+      }
+      m[t] = -INFINITY;
+      l[t] = 0.f;
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) o[t][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    const int all_see = tile * kPromptRows / a.group + start, any_sees = min((tile + 1) * kPromptRows - 1, total - 1) / a.group + start;
+    const int blocks = any_sees / kKv8Page + 1, per = (max(a.split_blocks, (blocks + a.n_split - 1) / a.n_split) + KB - 1) / KB * KB;
+    const int b_lo = split * per, b_hi = min(blocks, b_lo + per);
+    auto lane_of = [](float v, int i) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), i)); };
+    for (int run = b_lo; run < b_hi; run += 64) {
+      const int pid = run + lane < b_hi ? a.c.page(e, run + lane) : -1;
+      const float ks = pid < 0 ? 0.f : *a.c.scale(pid, 0, head), vs = pid < 0 ? 0.f : *a.c.scale(pid, 1, head);
+      const uint64_t there = __builtin_amdgcn_ballot_w64(pid >= 0);
+      const int steps = (min(b_hi - run, 64) + KB - 1) / KB;
+      const bool keys = !kRoles || wave >= 4, values = !kRoles || wave < 4;
+      const int k_unit = (kRoles ? wave - 4 : wave) * 2, v_unit = wave;
+      u32x4 kw[kSets][2], vw[kSets][2];    // of a set: two units of keys; the two blocks of a unit of values
+      auto load = [&](int i, auto set) {
+        if (i >= steps) return;
+        if (keys)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const int h = (k_unit + u) / C, c = (k_unit + u) % C;
+            const int page = max(__builtin_amdgcn_readlane(pid, i * KB + h), 0);     // one that is not there: page 0's bytes, masked below
+            kw[set()][u] = *reinterpret_cast<const u32x4*>(a.c.block(page, 0, head, D) + c * 1024 + n * 64 + g * 16);
+          }
+        if (values)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const int h = v_unit / C * 2 + u, c = v_unit % C;
+            const int page = max(__builtin_amdgcn_readlane(pid, i * KB + h), 0);
+            vw[set()][u] = *reinterpret_cast<const u32x4*>(a.c.block(page, 1, head, D) + c * 1024 + g * 256 + n * 16);
+          }
+      };
+      auto widen = [&](int i, auto set) {
+        if (i >= steps) return;
+        bf16x8_t (*to)[64] = s_kv[i & 1];
+        u32x4 (&k)[2] = kw[set()], (&v)[2] = vw[set()];
+        if (keys)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const int unit = k_unit + u;
+            const float x = lane_of(ks, i * KB + unit / C);
+            to[unit * 2][lane] = kv8_operand<FMT>(k[u].x, k[u].y, x);
+            to[unit * 2 + 1][lane] = kv8_operand<FMT>(k[u].z, k[u].w, x);
+          }
+        if (values) {
+          const int h = v_unit / C * 2;
+          const uint64_t want = ((1ull << KB) - 1) << (i * KB);
+          if ((run + (i + 1) * KB) * kKv8Page > len || (there & want) != want) {
+            // what lies behind the entry's last token may be any bytes, and 0 times one of them a NaN
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              const int here = there >> (i * KB + h + u) & 1 ? len - ((run + i * KB + h + u) * kKv8Page + 4 * g) : 0;
+              v[u] &= here >= 4 ? 0xFFFFFFFFu : here <= 0 ? 0u : 0xFFFFFFFFu >> (32 - 8 * here);
+            }
+          }
+          const float x = lane_of(vs, i * KB + h), y = lane_of(vs, i * KB + h + 1);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) to[2 * KB * C + v_unit * 4 + j][lane] = kv8_operand2<FMT>(v[0][j], v[1][j], x, y);
+        }
+      };
+      constexpr std::integral_constant<int, 0> s0{};
+      constexpr std::integral_constant<int, kSets - 1> s1{};
+      load(0, s0);
+      if (kSets == 2) load(1, s1);
+      __syncthreads();                     // the run before has read its last buffer
+      widen(0, s0);
+      load(kSets, s0);
+      auto body = [&](int i, auto set) {   // set: holds step i + 1
+        __syncthreads();
+        bf16x8_t (*from)[64] = s_kv[i & 1];
+        const int slot0 = (run + i * KB) * kKv8Page;
+        f32x4 s[NT][KB];
+#pragma unroll
+        for (int h = 0; h < KB; ++h)
+#pragma unroll
+          for (int t = 0; t < NT; ++t) s[t][h] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int h = 0; h < KB; ++h) {
+              const bf16x8_t kf = from[(h * C + c) * 2 + k][lane];
+#pragma unroll
+              for (int t = 0; t < NT; ++t) s[t][h] = mfma16(kf, qf[t][c][k], s[t][h]);
+            }
+        widen(i + 1, set);
+        load(i + 1 + kSets, set);
+        float f[KB];                       // the scores are scaled as they enter the exponential, but for masked steps: infinity times a factor that underflows is no mask
+#pragma unroll
+        for (int h = 0; h < KB; ++h) f[h] = kScaled ? a.scale_log2 : lane_of(ks, i * KB + h) * a.scale_log2;
+        const uint64_t want = ((1ull << KB) - 1) << (i * KB);
+        if (slot0 + KB * kKv8Page - 1 > all_see || (there & want) != want) {
+#pragma unroll
+          for (int h = 0; h < KB; ++h) {
+            const int end = there >> (i * KB + h) & 1 ? INT32_MAX : -1, at0 = slot0 + h * kKv8Page + 4 * g;
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) s[t][h][j] = at0 + j <= min(r[t].far, end) ? s[t][h][j] * f[h] : -INFINITY;
+            f[h] = 1.f;
+          }
+        }
+        bf16x8_t pf[NT][KB / 2];
+        float top[NT];
+        bool moves = false;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          top[t] = -INFINITY;
+#pragma unroll
+          for (int h = 0; h < KB; ++h) {
+            if constexpr (kScaled) top[t] = max3(max3(top[t], s[t][h][0], s[t][h][1]), s[t][h][2], s[t][h][3]);
+            else top[t] = fmaxf(top[t], max3(max3(s[t][h][0], s[t][h][1], s[t][h][2]), s[t][h][3], s[t][h][3]) * f[h]);
+          }
+          if constexpr (kScaled) top[t] *= f[0];      // one factor for all: the conversion took the blocks' scales along
+          moves |= top[t] > m[t] + kSlack;
+        }
+        if (__builtin_amdgcn_ballot_w64(moves)) {
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            const float mx = quad_max(top[t]), to = mx > m[t] + kSlack ? mx : m[t], alpha = to == -INFINITY ? 1.f : exp2_of(m[t] - to);
+            m[t] = to;
+            l[t] *= alpha;
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d) o[t][d] *= alpha;
+          }
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          const float base = m[t] == -INFINITY ? 0.f : m[t];
+#pragma unroll
+          for (int h = 0; h < KB; h += 2) {
+            float p[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              p[j] = exp2_of(fmaf(s[t][h + j / 4][j & 3], f[h + j / 4], -base));
+              l[t] += p[j];
+              if (!kScaled) p[j] *= lane_of(vs, i * KB + h + j / 4);
+            }
+            kv8_split<1>(p, &pf[t][h / 2]);
+          }
+        }
+#pragma unroll
+        for (int h = 0; h < KB; h += 2)
+#pragma unroll
+          for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const bf16x8_t vf = from[2 * KB * C + (h / 2 * C + c) * 4 + j][lane];
+#pragma unroll
+              for (int t = 0; t < NT; ++t) o[t][4 * c + j] = mfma16(vf, pf[t][h / 2], o[t][4 * c + j]);
+            }
+      };
+      for (int i = 0; i < steps; i += 2) {
+        body(i, s1);
+        if (i + 1 < steps) body(i + 1, s0);
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      l[t] = quad_sum(l[t]);
+      if (r[t].real) put_row<T, D>(a, r[t], split, g, m[t], l[t], o[t]);
+    }
   }
 }
 
@@ -309,9 +544,59 @@ __global__ __launch_bounds__(512) void kv8_merge_kernel(AttnArgs a) {
   }
 }
 
-// The weights that a call gives to the cached tokens, from the sums that the attention left.  A wave holds MB blocks of keys as operands while it walks the row tiles
-// that see them (the four waves of a workgroup the same tiles, which then come from the first-level cache), so that a token's sum is one wave's, in the rows' order.
-// n_slice > 1, where that leaves too few workgroups: every slice of the row tiles leaves its sums in part, kv8_mass_sum_kernel adds them in order.
+// The same for many rows of few splits: a wave each.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void kv8_merge_rows_kernel(AttnArgs a) {
+  constexpr int V = D / 64;
+  const int e = blockIdx.z, head = blockIdx.y, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const RowSpan rows = row_span(a.row0, e, a.n_rows);
+  const int start = a.starts[e], total = rows.n * a.group;
+  if (rows.n == 0 || start < 0 || start > INT32_MAX - 2048 - rows.n) return;
+  for (int rr = blockIdx.x * 4 + wave; rr < total; rr += gridDim.x * 4) {
+    const QueryRow r = query_row(rr, total, a.group, rows, start, head);
+    const int64_t rh = (int64_t)r.row * a.heads + r.head;
+    const f32x2* ml = reinterpret_cast<const f32x2*>(a.part_ml) + rh * a.n_split;
+    const float* part = a.part_o + rh * a.n_split * D + lane * V;
+    f32x2 x[kFewSplits];
+    float m = -INFINITY, l = 0.f, p[kFewSplits][V], o[V];
+#pragma unroll
+    for (int z = 0; z < kFewSplits; ++z) {
+      const int at = min(z, a.n_split - 1);
+      x[z] = ml[at];
+#pragma unroll
+      for (int v = 0; v < V; ++v) p[z][v] = part[(int64_t)at * D + v];
+      m = fmaxf(m, x[z].x);
+    }
+    const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int v = 0; v < V; ++v) o[v] = 0.f;
+#pragma unroll
+    for (int z = 0; z < kFewSplits; ++z) {
+      // a split without a key left no sums: what is in their place is not looked at
+      const bool some = z < a.n_split && (x[z].y > 0.f || x[z].y != x[z].y);
+      const float w = exp2_of(x[z].x - base);
+      l += some ? x[z].y * w : 0.f;
+#pragma unroll
+      for (int v = 0; v < V; ++v) o[v] += some ? p[z][v] * w : 0.f;
+    }
+    const bool some = l > 0.f || l != l;
+    const float inv = some ? 1.f / l : 0.f;
+    T* op = static_cast<T*>(a.out) + r.row * a.out_stride + (int64_t)r.head * D + lane * V;
+    if constexpr (V == 1) st(op, o[0] * inv);
+    else
+#pragma unroll
+      for (int v = 0; v < V; v += 2) {
+        const float y[2] = {o[v] * inv, o[v + 1] * inv};
+        st2(op + v, y);
+      }
+    if (a.lse && lane == 0) a.lse[rh] = some ? m + __log2f(l) : INFINITY;
+  }
+}
+
+// The weights that a call gives to the cached tokens, from the sums that the attention left.  A wave holds four blocks of keys as operands while the workgroup walks
+// the rows that see them, MT tiles of sixteen a step, which its four waves (each with keys of its own) fetch together, two steps ahead, into shared memory: a
+// token's sum is one wave's, in the rows' order.  n_slice > 1, where that leaves too few workgroups: every slice of the rows leaves its sums in part,
+// kv8_mass_sum_kernel adds them in order.
 struct MassArgs {
   const float* mass;
   float *out, *part;     // part [n_slice][n_ids][kv_heads][16]
@@ -324,35 +609,14 @@ __device__ __forceinline__ void put_mass(const MassArgs& w, int page, int at, fl
   w.out[page * w.out_stride + at] = w.keep == 0.f ? x : fmaf(w.keep, w.mass[page * w.mass_stride + at], x);
 }
 
-// a lane's part of a row of queries as loaded
-template <typename T, int C>
-struct RawQuery {
-  typedef __attribute__((ext_vector_type(4))) std::conditional_t<sizeof(T) == 2, uint32_t, float> Words;
-  Words w[C][sizeof(T)];
-  __device__ __forceinline__ void load(const T* p) {
-#pragma unroll
-    for (int c = 0; c < C; ++c)
-#pragma unroll
-      for (int i = 0; i < (int)sizeof(T); ++i) w[c][i] = reinterpret_cast<const Words*>(p + c * 64)[i];
-  }
-  __device__ __forceinline__ void part(int c, int k, bf16x8_t* q) const {
-    if constexpr (sizeof(T) == 2) {
-      q[0] = __builtin_bit_cast(bf16x8_t, w[c][k]);
-    } else {
-      float x[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = w[c][2 * k + i / 4][i & 3];
-      kv8_split<3>(x, q);
-    }
-  }
-};
-
-// Blocks of keys of a wave: a tile of sixteen rows, 32 D bytes, then feeds 2 D clocks of the matrix cores; eight blocks of 128 values spill (18 to 55 registers).
 constexpr int kMassBlocks = 4;
+template <typename T, int D> constexpr int mass_tiles() { return sizeof(T) == 2 && D < 256 ? 2 : 1; }   // fp32: three parts of every query; 256: registers
 
 template <typename T, int FMT, int D>
 __global__ __launch_bounds__(256, (sizeof(T) == 2 ? 2 : 1)) void kv8_mass_kernel(AttnArgs a, MassArgs w) {
-  constexpr int NP = kv8_parts<T>(), C = D / 64, MB = kMassBlocks;
+  constexpr int NP = kv8_parts<T>(), C = D / 64, MB = kMassBlocks, MT = mass_tiles<T, D>(), F = 2 * C * MT / 4;      // F: operands (a tile's rows, 32 values) a wave fetches
+  static_assert(F >= 1 || MT == 1, "an operand a wave at least");
+  __shared__ bf16x8_t s_q[2][2 * C * MT][NP][64];
   const int e = blockIdx.z, head = blockIdx.y, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   const RowSpan rows = row_span(a.row0, e, a.n_rows);
   const int start = a.starts[e], total = rows.n * a.group;
@@ -375,7 +639,8 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? 2 : 1)) void kv8_mass_kernel
     }
     return;
   }
-  for (int b0 = (blockIdx.x / w.n_slice * 4 + wave) * MB; b0 < blocks; b0 += gridDim.x / w.n_slice * 4 * MB) {
+  for (int w0 = blockIdx.x / w.n_slice * 4 * MB; w0 < blocks; w0 += gridDim.x / w.n_slice * 4 * MB) {
+    const int b0 = w0 + wave * MB;
     int page[MB];
     float ks[MB];
     bf16x8_t kf[MB][C][2];
@@ -389,56 +654,106 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? 2 : 1)) void kv8_mass_kernel
       for (int c = 0; c < C; ++c) kw[h][c] = *reinterpret_cast<const u32x4*>(kb + c * 1024);
       ks[h] = *a.c.scale(max(page[h], 0), 0, head) * a.scale_log2;
     }
+    f32x4 sum[MB];
+#pragma unroll
+    for (int h = 0; h < MB; ++h) sum[h] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int slot0 = b0 * kKv8Page, first = (int)((int64_t)max(w0 * kKv8Page - start, 0) * a.group / (16 * MT));   // the first step with a row that sees one of the workgroup's blocks
+    const int steps = (tiles + MT - 1) / MT, per = (steps - first + w.n_slice - 1) / w.n_slice, from = first + slice * per, to = min(steps, from + per);
+    // operand f of a step: tile f / (2 C), values 32 (f % (2 C)); wave w fetches f = w F .. (heads of 64 in fp32: the first two waves one each)
+    T raw[2][F > 0 ? F : 1][8] __attribute__((aligned(16)));
+    float lse[2][MT];
+    constexpr int FW = F > 0 ? F : 1;
+    const bool fetches = F > 0 || wave < 2 * C * MT;
+    auto fetch = [&](int step, auto set) {
+      if (fetches && step < to)
+#pragma unroll
+        for (int f = 0; f < FW; ++f) {
+          const int x = wave * FW + f, t = x / (2 * C), c = x % (2 * C) / 2, k = x & 1;
+          const QueryRow r = query_row((step * MT + t) * 16 + n, total, a.group, rows, start, head);
+          __builtin_memcpy(raw[set()][f], __builtin_assume_aligned(static_cast<const T*>(a.q) + r.row * a.q_stride + (int64_t)r.head * D + g * 16 + c * 64 + 8 * k, 16), 8 * sizeof(T));
+        }
+    };
+    auto leave = [&](int step, auto set) {
+      if (fetches && step < to)
+#pragma unroll
+        for (int f = 0; f < FW; ++f) {
+          bf16x8_t q[NP];
+          kv8_query(raw[set()][f], q);
+#pragma unroll
+          for (int p = 0; p < NP; ++p) s_q[(step - from) & 1][wave * FW + f][p][lane] = q[p];
+        }
+    };
+    auto sums_of = [&](int step, auto set) {
+      if (step < to)
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+          const QueryRow r = query_row((step * MT + t) * 16 + n, total, a.group, rows, start, head);
+          const float x = a.lse[(int64_t)r.row * a.heads + r.head];
+          lse[set()][t] = r.real ? x : INFINITY;                     // a row behind the last weighs nothing
+        }
+    };
+    constexpr std::integral_constant<int, 0> s0{};
+    constexpr std::integral_constant<int, 1> s1{};
 #pragma unroll
     for (int h = 0; h < MB; ++h)
 #pragma unroll
       for (int c = 0; c < C; ++c) {
         kf[h][c][0] = kv8_operand<FMT>(kw[h][c].x, kw[h][c].y);
         kf[h][c][1] = kv8_operand<FMT>(kw[h][c].z, kw[h][c].w);
+        __builtin_amdgcn_sched_barrier(0);                 // one after the other, and before the queries take registers: all floats of the keys at once spill
       }
-    f32x4 sum[MB];
+    fetch(from, s0);
+    sums_of(from, s0);
+    fetch(from + 1, s1);
+    sums_of(from + 1, s1);
+    __syncthreads();                                       // the blocks before have read their last buffer
+    leave(from, s0);
+    fetch(from + 2, s0);
+    auto body = [&](int step, auto set, auto other) {      // set: holds the step's sums, other: the next step's queries
+      const int buffer = (step - from) & 1;
+      __syncthreads();
+      f32x4 s[MT][MB];
 #pragma unroll
-    for (int h = 0; h < MB; ++h) sum[h] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const int slot0 = b0 * kKv8Page, first = (int)((int64_t)max(slot0 - start, 0) * a.group / 16);     // the first tile with a row that sees a block
-    const int per = (tiles - first + w.n_slice - 1) / w.n_slice, last = min(tiles, first + (slice + 1) * per);
-    // a row tile's queries and sums are on their way while the tile before is weighed
-    QueryRow r = query_row((first + slice * per) * 16 + n, total, a.group, rows, start, head);
-    RawQuery<T, C> raw, next;
-    float lse, next_lse;
-    auto fetch = [&](const QueryRow& y, RawQuery<T, C>& to, float& sum_of) {
-      to.load(static_cast<const T*>(a.q) + y.row * a.q_stride + (int64_t)y.head * D + g * 16);
-      sum_of = a.lse[(int64_t)y.row * a.heads + y.head];
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int h = 0; h < MB; ++h) s[t][h] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int p = NP - 1; p >= 0; --p) {
+              const bf16x8_t q = s_q[buffer][(t * C + c) * 2 + k][p][lane];
+#pragma unroll
+              for (int h = 0; h < MB; ++h) s[t][h] = mfma16(kf[h][c][k], q, s[t][h]);
+            }
+      leave(step + 1, other);
+      fetch(step + 3, other);
+      const bool all = slot0 + MB * kKv8Page - 1 <= step * MT * 16 / a.group + start;           // every row of the step sees every slot
+      if (all) {
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+          for (int h = 0; h < MB; ++h)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sum[h][i] += exp2_of(fmaf(s[t][h][i], ks[h], -lse[set()][t]));
+      } else {
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+          const int far = query_row((step * MT + t) * 16 + n, total, a.group, rows, start, head).far;
+#pragma unroll
+          for (int h = 0; h < MB; ++h)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sum[h][i] += slot0 + h * kKv8Page + 4 * g + i <= far ? exp2_of(fmaf(s[t][h][i], ks[h], -lse[set()][t])) : 0.f;
+        }
+      }
+      sums_of(step + 2, set);
     };
-    fetch(r, raw, lse);
-    for (int tile = first + slice * per; tile < last; ++tile) {
-      const QueryRow after = query_row((tile + 1) * 16 + n, total, a.group, rows, start, head);
-      fetch(after, next, next_lse);
-      f32x4 s[MB];
-#pragma unroll
-      for (int h = 0; h < MB; ++h) s[h] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int c = 0; c < C; ++c)
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          bf16x8_t q[NP];
-          raw.part(c, k, q);
-#pragma unroll
-          for (int p = NP - 1; p >= 0; --p)
-#pragma unroll
-            for (int h = 0; h < MB; ++h) s[h] = mfma16(kf[h][c][k], q[p], s[h]);
-        }
-      if (!r.real) lse = INFINITY;      // a row behind the last weighs nothing
-      const bool all = slot0 + MB * kKv8Page - 1 <= tile * 16 / a.group + start;           // every row of the tile sees every slot
-#pragma unroll
-      for (int h = 0; h < MB; ++h)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float p = exp2_of(fmaf(s[h][i], ks[h], -lse));
-          sum[h][i] += all || slot0 + h * kKv8Page + 4 * g + i <= r.far ? p : 0.f;
-        }
-      r = after;
-      raw = next;
-      lse = next_lse;
+    for (int step = from; step < to; step += 2) {
+      body(step, s0, s1);
+      if (step + 1 < to) body(step + 1, s1, s0);
     }
 #pragma unroll
     for (int h = 0; h < MB; ++h)
@@ -470,16 +785,19 @@ __global__ __launch_bounds__(256) void kv8_mass_sum_kernel(AttnArgs a, MassArgs 
 }
 
 // How a call is cut: rows of a workgroup, splits of the keys and slices of the weights' rows where those leave too few workgroups.
-struct AttnPlan { int tiles, row_tiles, n_split, split_blocks, mass_groups, n_slice, score_rows; };
+struct AttnPlan { bool prompt; int tiles, row_tiles, n_split, split_blocks, mass_groups, n_slice, score_rows; };
 inline AttnPlan attn_plan(const pegainfer_kv8_cache* cache, int n_rows, int max_rows, int max_len, int heads, int dtype) {
   AttnPlan p;
   const int64_t rows = (int64_t)std::min(max_rows, n_rows) * (heads / cache->kv_heads), pairs = (int64_t)cache->kv_heads * cache->n_entries;
   p.row_tiles = rows > 16 && !(dtype == kDtF32 && cache->dim == 256) ? 2 : 1;
-  p.tiles = ceil_div(rows, 16 * p.row_tiles);
+  p.prompt = dtype == kDtBf16 && rows >= kPromptRows;
+  p.tiles = ceil_div(rows, p.prompt ? kPromptRows : 16 * p.row_tiles);
   const int blocks = std::max(1, ceil_div(max_len, kKv8Page));
   const int64_t want = 2 * device_cus();
   auto cut = [&](int64_t groups, int64_t most) { return (int)std::max<int64_t>(1, std::min((want + groups - 1) / groups, most)); };
-  p.n_split = cut(p.tiles * pairs, std::min((blocks + 15) / 16, 256));
+  const int64_t groups = p.tiles * pairs;
+  // steps: a workgroup's run is 64 blocks; prompts: 32 at least (a split of 128 rows costs 1 KB a value of the head in sums)
+  p.n_split = p.prompt ? (int)std::max<int64_t>(1, std::min<int64_t>({want / groups, blocks / 32, 256})) : cut(groups, blocks <= 64 ? 1 : std::min((blocks + 15) / 16, 256));
   p.split_blocks = ceil_div(blocks, p.n_split);
   p.score_rows = rows <= 16 ? (int)rows : 0;
   p.mass_groups = p.score_rows ? ceil_div(blocks, 256 / kKv8Page) : ceil_div(blocks, 4 * kMassBlocks);
@@ -529,16 +847,21 @@ pegainfer_status_t pegainfer_kv8_attention(const pegainfer_kv8_cache* cache, con
                    d->scale * 1.4426950408889634f, d->out, lse, d->workspace, part_ml, p.score_rows ? rest : nullptr, p.score_rows};
   const dim3 grid(p.tiles * p.n_split, cache->kv_heads, cache->n_entries);
   const dim3 merge_grid(std::min(d->max_rows, d->n_rows) * group * (cache->dim / 64), cache->kv_heads, cache->n_entries);
+  const dim3 rows_grid(ceil_div((int64_t)std::min(d->max_rows, d->n_rows) * group, 4), cache->kv_heads, cache->n_entries);
   const dim3 mass_grid(p.mass_groups * p.n_slice, cache->kv_heads, cache->n_entries), sum_grid(std::max(1, ceil_div(d->max_len, 256)), cache->kv_heads, cache->n_entries);
   const MassArgs w{d->mass, d->mass_out, rest, d->mass_page_stride, d->mass_out_page_stride, d->mass_keep, p.n_slice};
   kv8_by(d->dtype, cache->format, cache->dim, [&](auto* t, auto fmt, auto dim) {
     using T = std::remove_pointer_t<decltype(t)>;
     constexpr int D = dim();
-    if constexpr (sizeof(T) == 2 || D < 256) {
-      if (p.row_tiles == 2) kv8_attn_kernel<T, fmt(), D, 2><<<grid, 256, 0, as_stream(stream)>>>(a);
+    if constexpr (sizeof(T) == 2) {
+      if (p.prompt) kv8_prompt_kernel<fmt(), D><<<grid, 64 * 8 / prompt_tiles<D>(), 0, as_stream(stream)>>>(a);
     }
-    if (p.row_tiles == 1) kv8_attn_kernel<T, fmt(), D, 1><<<grid, 256, 0, as_stream(stream)>>>(a);
-    if (p.n_split > 1) kv8_merge_kernel<T, D><<<merge_grid, 64 * std::min(8, p.n_split), 0, as_stream(stream)>>>(a);
+    if constexpr (sizeof(T) == 2 || D < 256) {
+      if (!p.prompt && p.row_tiles == 2) kv8_attn_kernel<T, fmt(), D, 2><<<grid, 256, 0, as_stream(stream)>>>(a);
+    }
+    if (!p.prompt && p.row_tiles == 1) kv8_attn_kernel<T, fmt(), D, 1><<<grid, 256, 0, as_stream(stream)>>>(a);
+    if (p.n_split > 1 && p.n_split <= kFewSplits) kv8_merge_rows_kernel<T, D><<<rows_grid, 256, 0, as_stream(stream)>>>(a);
+    if (p.n_split > kFewSplits) kv8_merge_kernel<T, D><<<merge_grid, 64 * std::min(8, p.n_split), 0, as_stream(stream)>>>(a);
     if (weigh) kv8_mass_kernel<T, fmt(), D><<<mass_grid, 256, 0, as_stream(stream)>>>(a, w);
   });
   if (weigh && p.n_slice > 1) kv8_mass_sum_kernel<<<sum_grid, 256, 0, as_stream(stream)>>>(a, w);

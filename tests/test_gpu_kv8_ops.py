@@ -189,6 +189,25 @@ def test_tables_that_lead_nowhere():
     assert (out[:4] == 7).all() and (out[4:] != 7).all()
 
 
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_prompts_over_pages_that_are_not_there(fmt, dim):
+    """many rows: whole blocks missing, at the ends and in the middle; scales that nothing but 0 is left of beside the scores'"""
+    c = Cache([40, 0], [150, 90], 2, dim, fmt, seed=21, layers=2)
+    c.ids[c.indptr[0]], c.ids[c.indptr[0] + 5], c.ids[c.indptr[1] + 2] = -1, c.pages, 2 ** 31 - 1
+    c.indptr[2] -= 1
+    attend(c, 4, torch.bfloat16, weigh=True)
+    c.scales[:] = 2.0 ** -100
+    attend(c, 4, torch.bfloat16, weigh=True)
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+def test_prompts_split_over_a_long_cache(fmt):
+    """a portion of a prompt over more than a run of 64 blocks, few enough rows that the keys are split"""
+    attend(Cache([2300], [40], 1, 128, fmt, seed=22), 4, torch.bfloat16, weigh=True)
+    attend(Cache([1500, 30], [33, 129], 1, 64, fmt, seed=23), 4, torch.bfloat16)
+
+
 # ---- eviction ----
 def run_evict(c, lens, budget, first, last, dst_extra=0):
     """entries of `lens` tokens over c's pages; fresh pages behind c's own"""
