@@ -45,6 +45,7 @@ struct AttnArgs {
   float *part_o, *part_ml;   // n_split > 1: [n_rows][heads][n_split][D] and [2] (running maximum, sum)
   float* scores;         // [n_ids][kv_heads][score_rows][16] of entries of up to score_rows <= 16 query rows a kv head, for the weights; NULL: not wanted
   int score_rows;
+  int round, snake;      // pieces of work of an entry and head that one workgroup a compute unit takes; whether the second round goes from the short to the long
 };
 
 // the queries' rows of a kv head, (token, head of the group) in order; a row behind the last is the last again
@@ -98,13 +99,13 @@ __global__ __launch_bounds__(256, (attn_waves<T, D, NT>())) void kv8_attn_kernel
   constexpr bool kScaled = FMT == kE4m3;   // the conversion takes the block's scale along; int8 scales scores and weights instead
   __shared__ f32x4 s_o[2][D / 16][64];
   __shared__ float s_m[2][16], s_l[2][16];
-  const int e = blockIdx.z, head = blockIdx.y, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+  const int e = (blockIdx.y + blockIdx.z / a.n_split / a.round) % gridDim.y, head = blockIdx.x, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   const RowSpan rows = row_span(a.row0, e, a.n_rows);
   const int start = a.starts[e], total = rows.n * a.group;
   if (rows.n == 0 || start < 0 || start > INT32_MAX - 2048 - rows.n) return;
-  const int len = start + rows.n, n_tiles = (total + 16 * NT - 1) / (16 * NT), split = blockIdx.x % a.n_split, step = gridDim.x / a.n_split;
-  for (int at = blockIdx.x / a.n_split; at < n_tiles; at += step) {
-    const int tile = n_tiles - 1 - at;     // the rows that see most first
+  const int len = start + rows.n, n_tiles = (total + 16 * NT - 1) / (16 * NT), split = blockIdx.z % a.n_split, step = gridDim.z / a.n_split;
+  for (int at = blockIdx.z / a.n_split; at < n_tiles; at += step) {
+    const int tile = a.snake && at >= a.round ? at - a.round : n_tiles - 1 - at;     // the rows that see most first
     QueryRow r[NT];
     bf16x8_t qf[NT][C][2][NP];
     float m[NT], l[NT];
@@ -303,13 +304,13 @@ __global__ __launch_bounds__(64 * 8 / prompt_tiles<D>(), 2) void kv8_prompt_kern
   constexpr bool kScaled = FMT == kE4m3;
   // keys [block][chunk][half], then values [pair of blocks][chunk][value of the lane's four]
   __shared__ bf16x8_t s_kv[2][2 * KB * C + 2 * KB * C][64];
-  const int e = blockIdx.z, head = blockIdx.y, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+  const int e = (blockIdx.y + blockIdx.z / a.n_split / a.round) % gridDim.y, head = blockIdx.x, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   const RowSpan rows = row_span(a.row0, e, a.n_rows);
   const int start = a.starts[e], total = rows.n * a.group;
   if (rows.n == 0 || start < 0 || start > INT32_MAX - 2048 - rows.n) return;
-  const int len = start + rows.n, n_tiles = (total + kPromptRows - 1) / kPromptRows, split = blockIdx.x % a.n_split, stride = gridDim.x / a.n_split;
-  for (int at = blockIdx.x / a.n_split; at < n_tiles; at += stride) {
-    const int tile = n_tiles - 1 - at;     // the rows that see most first
+  const int len = start + rows.n, n_tiles = (total + kPromptRows - 1) / kPromptRows, split = blockIdx.z % a.n_split, stride = gridDim.z / a.n_split;
+  for (int at = blockIdx.z / a.n_split; at < n_tiles; at += stride) {
+    const int tile = a.snake && at >= a.round ? at - a.round : n_tiles - 1 - at;     // the rows that see most first
     QueryRow r[NT];
     bf16x8_t qf[NT][C][2];
     float m[NT], l[NT];
@@ -593,7 +594,7 @@ __global__ __launch_bounds__(256) void kv8_merge_rows_kernel(AttnArgs a) {
   }
 }
 
-// The weights that a call gives to the cached tokens, from the sums that the attention left.  A wave holds four blocks of keys as operands while the workgroup walks
+// The weights that a call gives to the cached tokens, from the sums that the attention left.  A wave holds four blocks of keys (two of 256 values) as operands while the workgroup walks
 // the rows that see them, MT tiles of sixteen a step, which its four waves (each with keys of its own) fetch together, two steps ahead, into shared memory: a
 // token's sum is one wave's, in the rows' order.  n_slice > 1, where that leaves too few workgroups: every slice of the rows leaves its sums in part,
 // kv8_mass_sum_kernel adds them in order.
@@ -609,23 +610,23 @@ __device__ __forceinline__ void put_mass(const MassArgs& w, int page, int at, fl
   w.out[page * w.out_stride + at] = w.keep == 0.f ? x : fmaf(w.keep, w.mass[page * w.mass_stride + at], x);
 }
 
-constexpr int kMassBlocks = 4;
-template <typename T, int D> constexpr int mass_tiles() { return sizeof(T) == 2 && D < 256 ? 2 : 1; }   // fp32: three parts of every query; 256: registers
+template <int D> constexpr int mass_blocks() { return D == 256 ? 2 : 4; }   // of keys, a wave
+template <typename T, int D> constexpr int mass_tiles() { return sizeof(T) == 2 ? 2 : 1; }   // fp32: three parts of every query
 
 template <typename T, int FMT, int D>
 __global__ __launch_bounds__(256, (sizeof(T) == 2 ? 2 : 1)) void kv8_mass_kernel(AttnArgs a, MassArgs w) {
-  constexpr int NP = kv8_parts<T>(), C = D / 64, MB = kMassBlocks, MT = mass_tiles<T, D>(), F = 2 * C * MT / 4;      // F: operands (a tile's rows, 32 values) a wave fetches
+  constexpr int NP = kv8_parts<T>(), C = D / 64, MB = mass_blocks<D>(), MT = mass_tiles<T, D>(), F = 2 * C * MT / 4;      // F: operands (a tile's rows, 32 values) a wave fetches
   static_assert(F >= 1 || MT == 1, "an operand a wave at least");
   __shared__ bf16x8_t s_q[2][2 * C * MT][NP][64];
-  const int e = blockIdx.z, head = blockIdx.y, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+  const int e = (blockIdx.y + blockIdx.z / w.n_slice) % gridDim.y, head = blockIdx.x, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   const RowSpan rows = row_span(a.row0, e, a.n_rows);
   const int start = a.starts[e], total = rows.n * a.group;
   if (rows.n == 0 || start < 0 || start > INT32_MAX - 2048 - rows.n) return;
-  const int blocks = (start + rows.n + kKv8Page - 1) / kKv8Page, slice = blockIdx.x % w.n_slice, tiles = (total + 15) / 16;
+  const int blocks = (start + rows.n + kKv8Page - 1) / kKv8Page, slice = blockIdx.z % w.n_slice, tiles = (total + 15) / 16;
   if (a.scores && total <= a.score_rows) {
     // a step: the attention left its scores, 4 bytes a row and token beside D of the keys
     const int len = start + rows.n;
-    for (int slot = blockIdx.x * 256 + threadIdx.x; slot < len; slot += gridDim.x * 256) {
+    for (int slot = blockIdx.z * 256 + threadIdx.x; slot < len; slot += gridDim.z * 256) {
       const int block = slot / kKv8Page, page = a.c.page(e, block);
       if (page < 0) continue;
       const float* s = a.scores + (((int64_t)a.c.indptr[e] + block) * a.c.kv_heads + head) * a.score_rows * kKv8Page + slot % kKv8Page;
@@ -639,7 +640,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? 2 : 1)) void kv8_mass_kernel
     }
     return;
   }
-  for (int w0 = blockIdx.x / w.n_slice * 4 * MB; w0 < blocks; w0 += gridDim.x / w.n_slice * 4 * MB) {
+  for (int w0 = blockIdx.z / w.n_slice * 4 * MB; w0 < blocks; w0 += gridDim.z / w.n_slice * 4 * MB) {
     const int b0 = w0 + wave * MB;
     int page[MB];
     float ks[MB];
@@ -785,7 +786,7 @@ __global__ __launch_bounds__(256) void kv8_mass_sum_kernel(AttnArgs a, MassArgs 
 }
 
 // How a call is cut: rows of a workgroup, splits of the keys and slices of the weights' rows where those leave too few workgroups.
-struct AttnPlan { bool prompt; int tiles, row_tiles, n_split, split_blocks, mass_groups, n_slice, score_rows; };
+struct AttnPlan { bool prompt; int tiles, row_tiles, n_split, split_blocks, mass_groups, n_slice, score_rows, round, snake; };
 inline AttnPlan attn_plan(const pegainfer_kv8_cache* cache, int n_rows, int max_rows, int max_len, int heads, int dtype) {
   AttnPlan p;
   const int64_t rows = (int64_t)std::min(max_rows, n_rows) * (heads / cache->kv_heads), pairs = (int64_t)cache->kv_heads * cache->n_entries;
@@ -799,11 +800,15 @@ inline AttnPlan attn_plan(const pegainfer_kv8_cache* cache, int n_rows, int max_
   // steps: a workgroup's run is 64 blocks; prompts: 32 at least (a split of 128 rows costs 1 KB a value of the head in sums)
   p.n_split = p.prompt ? (int)std::max<int64_t>(1, std::min<int64_t>({want / groups, blocks / 32, 256})) : cut(groups, blocks <= 64 ? 1 : std::min((blocks + 15) / 16, 256));
   p.split_blocks = ceil_div(blocks, p.n_split);
+  p.round = (int)std::max<int64_t>(1, device_cus() / pairs);
+  p.snake = p.n_split == 1 && p.tiles > p.round && p.tiles <= 2 * p.round;
   p.score_rows = rows <= 16 ? (int)rows : 0;
-  p.mass_groups = p.score_rows ? ceil_div(blocks, 256 / kKv8Page) : ceil_div(blocks, 4 * kMassBlocks);
-  p.n_slice = cut(p.mass_groups * pairs, std::min<int64_t>((rows + 255) / 256, 16));
+  p.mass_groups = p.score_rows ? ceil_div(blocks, 256 / kKv8Page) : ceil_div(blocks, 4 * (cache->dim == 256 ? mass_blocks<256>() : mass_blocks<128>()));
+  p.n_slice = cut((p.mass_groups * pairs + 1) / 2, std::min<int64_t>((rows + 255) / 256, 16));   // the first keys' rows are twice the average's
   return p;
 }
+// workgroups of `items` pieces of work cut `ways`, in whole pieces; kernels walk what a grid cannot hold
+inline int deal(int64_t items, int ways) { return (int)std::min<int64_t>(items, 65535 / ways) * ways; }
 // the splits' sums and states of a workspace, up to 16 bytes
 inline int64_t split_floats(const AttnPlan& p, int64_t row_heads, int dim) { return p.n_split > 1 ? (row_heads * p.n_split * (dim + 2) + 3) / 4 * 4 : 0; }
 
@@ -844,11 +849,15 @@ pegainfer_status_t pegainfer_kv8_attention(const pegainfer_kv8_cache* cache, con
   float* const lse = weigh ? d->workspace + split_floats(p, rh, cache->dim) : nullptr;
   float* const rest = weigh ? lse + (rh + 3) / 4 * 4 : nullptr;
   const AttnArgs a{kv8_of(cache), d->q, d->q_row_stride, d->out_row_stride, d->row0, d->starts, d->n_rows, group, d->heads, p.n_split, p.split_blocks,
-                   d->scale * 1.4426950408889634f, d->out, lse, d->workspace, part_ml, p.score_rows ? rest : nullptr, p.score_rows};
-  const dim3 grid(p.tiles * p.n_split, cache->kv_heads, cache->n_entries);
+                   d->scale * 1.4426950408889634f, d->out, lse, d->workspace, part_ml, p.score_rows ? rest : nullptr, p.score_rows,
+                   p.round, p.snake};
+  // Grid (head, entry, work), the longest work first: heads next to one another meet their cache in their XCD's second level (8 heads: one each), and
+  // the short ones fill the end.  The entries change places from round to round, and where two rounds are all the second starts with the shortest: what shares a
+  // compute unit is a long piece and a short one.
+  const dim3 grid(cache->kv_heads, cache->n_entries, deal(p.tiles, p.n_split)), mass_grid(cache->kv_heads, cache->n_entries, deal(p.mass_groups, p.n_slice));
   const dim3 merge_grid(std::min(d->max_rows, d->n_rows) * group * (cache->dim / 64), cache->kv_heads, cache->n_entries);
   const dim3 rows_grid(ceil_div((int64_t)std::min(d->max_rows, d->n_rows) * group, 4), cache->kv_heads, cache->n_entries);
-  const dim3 mass_grid(p.mass_groups * p.n_slice, cache->kv_heads, cache->n_entries), sum_grid(std::max(1, ceil_div(d->max_len, 256)), cache->kv_heads, cache->n_entries);
+  const dim3 sum_grid(std::max(1, ceil_div(d->max_len, 256)), cache->kv_heads, cache->n_entries);
   const MassArgs w{d->mass, d->mass_out, rest, d->mass_page_stride, d->mass_out_page_stride, d->mass_keep, p.n_slice};
   kv8_by(d->dtype, cache->format, cache->dim, [&](auto* t, auto fmt, auto dim) {
     using T = std::remove_pointer_t<decltype(t)>;
