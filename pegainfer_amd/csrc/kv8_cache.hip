@@ -10,27 +10,25 @@ namespace pk {
 // keys: value c * 64 + 16 q .. + 15 of token n;  values: tokens 4 q .. + 3 of the values 64 c + 4 n .. + 3, byte 4 j + t = value j, token t
 __device__ __forceinline__ int unit_at(int side, int chunk, int n, int q) { return chunk * 1024 + (side == 0 ? n * 64 + q * 16 : q * 256 + n * 16); }
 
-// x[16] of a unit from rows of T: row(t) gives the row of the block's token t, or -1
+// x[16] of a unit from rows of T: row(t) is the row of the block's token t, or -1: zeros.  Such a row's place is read from row `any` and left out, so that no load
+// waits behind a branch.
 template <typename T, typename Row>
-__device__ __forceinline__ void unit_rows(const T* base, int64_t stride, int side, int chunk, int n, int q, Row row, float* x) {
+__device__ __forceinline__ void unit_rows(const T* base, int64_t stride, int side, int chunk, int n, int q, Row row, int any, float* x) {
   if (side == 0) {
     const int r = row(n);
-    if (r >= 0) {
-      const T* p = base + r * stride + chunk * 64 + q * 16;
-      Vec8<T>::load(p, x);
-      Vec8<T>::load(p + 8, x + 8);
-    } else {
+    const T* p = base + (r < 0 ? any : r) * stride + chunk * 64 + q * 16;
+    Vec8<T>::load(p, x);
+    Vec8<T>::load(p + 8, x + 8);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) x[i] = 0.f;
-    }
+    for (int i = 0; i < 16; ++i) x[i] = r < 0 ? 0.f : x[i];
   } else {
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       const int r = row(4 * q + t);
-      float y[4] = {0.f, 0.f, 0.f, 0.f};
-      if (r >= 0) ld4(base + r * stride + chunk * 64 + 4 * n, y);
+      float y[4];
+      ld4(base + (r < 0 ? any : r) * stride + chunk * 64 + 4 * n, y);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) x[4 * j + t] = y[j];
+      for (int j = 0; j < 4; ++j) x[4 * j + t] = r < 0 ? 0.f : y[j];
     }
   }
 }
@@ -56,8 +54,9 @@ __global__ __launch_bounds__(128) void kv8_append_kernel(Kv8 c, const T* k, cons
     auto row = [&](int t) { const int s = low + t; return s >= start && s < end ? rows.first + (s - (int)start) : -1; };
     float x[D / 64][16], amax = 0.f;
 #pragma unroll
+    for (int ch = 0; ch < D / 64; ++ch) unit_rows(base, stride, side, ch, n, q, row, rows.first, x[ch]);
+#pragma unroll
     for (int ch = 0; ch < D / 64; ++ch) {
-      unit_rows(base, stride, side, ch, n, q, row, x[ch]);
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const float a = fabsf(x[ch][i]);
@@ -185,9 +184,28 @@ __global__ __launch_bounds__(kPickThreads) void kv8_pick_kernel(Kv8 c, const flo
     return page < 0 ? 0u : order_of(mass[page * mass_stride + head * kKv8Page + s % kKv8Page]);
   };
   const bool held = len <= cached;
-  if (held) {
-#pragma unroll 8
-    for (int s = tid; s < len; s += kPickThreads) s_order[s] = fetch(s);
+  if (held && c.n_ids > 0) {
+    // sixteen slots a thread at a time, page ids and weights each in one go: what is not there is read from the table's and the cache's first place and left out
+    const int first = c.indptr[e], pages = c.indptr[e + 1] - first;
+    constexpr int N = 16;
+    for (int s0 = tid; s0 < len; s0 += N * kPickThreads) {
+      int page[N];
+      float m[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int block = (s0 + i * kPickThreads) / kKv8Page, at = first + block;
+        const bool there = block < pages && (unsigned)at < (unsigned)c.n_ids;
+        const int id = c.ids[there ? at : 0];
+        page[i] = there && (unsigned)id < (unsigned)c.n_pages ? id : -1;
+      }
+#pragma unroll
+      for (int i = 0; i < N; ++i) m[i] = mass[max(page[i], 0) * mass_stride + head * kKv8Page + (s0 + i * kPickThreads) % kKv8Page];
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (s0 + i * kPickThreads < len) s_order[s0 + i * kPickThreads] = page[i] < 0 ? 0u : order_of(m[i]);
+    }
+  } else if (held) {
+    for (int s = tid; s < len; s += kPickThreads) s_order[s] = 0;
   }
   auto weight = [&](int s) { return held ? s_order[s] : fetch(s); };
   const int lo = keep_first, hi = len - keep_last, chosen = budget - keep_first - keep_last;
@@ -294,29 +312,42 @@ __global__ __launch_bounds__(128) void kv8_move_kernel(Kv8 c, const int32_t* dst
       t4[j] = __shfl(t, 4 * q + j, 64);
       was4[j] = __shfl(was, 4 * q + j, 64);
     }
+    // every load at once; a token that is not there: the first page's bytes, left out
+    if (side == 0) {
+      u32x4 w[D / 64];
 #pragma unroll
-    for (int ch = 0; ch < D / 64; ++ch) {
-      u32x4 w = {0, 0, 0, 0};
-      if (side == 0) {
-        if (src >= 0) w = *reinterpret_cast<const u32x4*>(c.block(src, 0, head, D) + unit_at(0, ch, t, q));
+      for (int ch = 0; ch < D / 64; ++ch) w[ch] = *reinterpret_cast<const u32x4*>(c.block(max(src, 0), 0, head, D) + unit_at(0, ch, t, q));
+      const float by = pow2f(was - ex);
+#pragma unroll
+      for (int ch = 0; ch < D / 64; ++ch) {
+        if (src < 0) w[ch] = u32x4{0, 0, 0, 0};
         if (was != ex) {
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             float y[4];
-            kv8_numbers<FMT>(w[k], y);
+            kv8_numbers<FMT>(w[ch][k], y);
 #pragma unroll
-            for (int m = 0; m < 4; ++m) y[m] *= pow2f(was - ex);
-            w[k] = kv8_codes<FMT>(y);
+            for (int m = 0; m < 4; ++m) y[m] *= by;
+            w[ch][k] = kv8_codes<FMT>(y);
           }
         }
-      } else {
+        *reinterpret_cast<u32x4*>(blk + unit_at(0, ch, n, q)) = w[ch];
+      }
+    } else {
+      u32x4 g[D / 64][4];
+#pragma unroll
+      for (int ch = 0; ch < D / 64; ++ch)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) g[ch][j] = *reinterpret_cast<const u32x4*>(c.block(max(src4[j], 0), 1, head, D) + unit_at(1, ch, n, t4[j] >> 2));
+#pragma unroll
+      for (int ch = 0; ch < D / 64; ++ch) {
+        u32x4 w = {0, 0, 0, 0};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          if (src4[j] < 0) continue;
-          const u32x4 g = *reinterpret_cast<const u32x4*>(c.block(src4[j], 1, head, D) + unit_at(1, ch, n, t4[j] >> 2));
           uint32_t one = 0;                // this token's byte of each of the four values
 #pragma unroll
-          for (int k = 0; k < 4; ++k) one |= (g[k] >> (8 * (t4[j] & 3)) & 255u) << (8 * k);
+          for (int k = 0; k < 4; ++k) one |= (g[ch][j][k] >> (8 * (t4[j] & 3)) & 255u) << (8 * k);
+          if (src4[j] < 0) one = 0;
           if (was4[j] != ex) {
             float y[4];
             kv8_numbers<FMT>(one, y);
@@ -327,8 +358,8 @@ __global__ __launch_bounds__(128) void kv8_move_kernel(Kv8 c, const int32_t* dst
 #pragma unroll
           for (int k = 0; k < 4; ++k) w[k] |= (one >> (8 * k) & 255u) << (8 * j);
         }
+        *reinterpret_cast<u32x4*>(blk + unit_at(1, ch, n, q)) = w;
       }
-      *reinterpret_cast<u32x4*>(blk + unit_at(side, ch, n, q)) = w;
     }
   }
 }
