@@ -55,7 +55,7 @@ __device__ __forceinline__ QueryRow query_row(int rr, int total, int group, cons
   return {rows.first + tok, kv_head * group + r - tok * group, start + tok, rr < total};
 }
 
-constexpr int kPromptRows = 128, kFewSplits = 4;
+constexpr int kPromptRows = 128, kFewSplits = 8;
 
 // a lane's part of a row's result: the output, or what a split leaves of it
 template <typename T, int D>
@@ -93,12 +93,13 @@ template <typename T, int D, int NT> constexpr int attn_waves() { return D * NT 
 // meet in shared memory at the end, so that no key is loaded or widened twice in a workgroup.  Scores are computed transposed (keys x rows): a lane then holds four
 // keys' scores of one row, exactly what the second product wants from it.  The next keys are on their way while the weights are made, the next values while
 // the next scores are.
-template <typename T, int FMT, int D, int NT>
+// ONCE: the rows are one tile, so nobody reads the keys again and they pass the caches by (32 x 8192 tokens int8: 78 -> 70 us, 4.8 TB/s).
+template <typename T, int FMT, int D, int NT, bool ONCE>
 __global__ __launch_bounds__(256, (attn_waves<T, D, NT>())) void kv8_attn_kernel(AttnArgs a) {
-  constexpr int NP = kv8_parts<T>(), C = D / 64, KB = attn_kb<T, D>();
+  constexpr int NP = kv8_parts<T>(), C = D / 64, KB = attn_kb<T, D>(), W = 4;
   constexpr bool kScaled = FMT == kE4m3;   // the conversion takes the block's scale along; int8 scales scores and weights instead
-  __shared__ f32x4 s_o[2][D / 16][64];
-  __shared__ float s_m[2][16], s_l[2][16];
+  __shared__ f32x4 s_o[W / 2][D / 16][64];
+  __shared__ float s_m[W / 2][16], s_l[W / 2][16];
   const int e = (blockIdx.y + blockIdx.z / a.n_split / a.round) % gridDim.y, head = blockIdx.x, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   const RowSpan rows = row_span(a.row0, e, a.n_rows);
   const int start = a.starts[e], total = rows.n * a.group;
@@ -128,28 +129,36 @@ __global__ __launch_bounds__(256, (attn_waves<T, D, NT>())) void kv8_attn_kernel
     const int all_see = tile * NT * 16 / a.group + start, any_sees = min((tile + 1) * NT * 16 - 1, total - 1) / a.group + start;
     const int blocks = any_sees / kKv8Page + 1, per = max(a.split_blocks, (blocks + a.n_split - 1) / a.n_split);
     const int b_lo = split * per, b_hi = min(blocks, b_lo + per);
+    // lane i: block i of a run of 64; the pages of a run are looked up two runs ahead, their scales one
+    auto page_of = [&](int run) { return run + lane < b_hi ? a.c.page(e, run + lane) : -1; };
+    auto scale_of = [&](int page, int side) { return page < 0 ? 0.f : *a.c.scale(page, side, head); };
+    int pid = page_of(b_lo), next = page_of(b_lo + 64);
+    float ks = scale_of(pid, 0), vs = scale_of(pid, 1);
+    u32x4 kw[KB][C], vw[KB][C];
+    auto load = [&](int side, int pages, int i, u32x4 (&w)[KB][C]) {
+#pragma unroll
+      for (int h = 0; h < KB; ++h) {
+        const int page = max(__builtin_amdgcn_readlane(pages, i * KB + h), 0);     // one that is not there: page 0's bytes, masked below
+        const uint8_t* p = a.c.block(page, side, head, D) + (side == 0 ? n * 64 + g * 16 : g * 256 + n * 16);
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+          const u32x4* from = reinterpret_cast<const u32x4*>(p + c * 1024);
+          w[h][c] = ONCE ? __builtin_nontemporal_load(from) : *from;
+        }
+      }
+    };
+    auto lane_of = [](float v, int i) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), i)); };
+    if (wave * KB < b_hi - b_lo) {
+      load(0, pid, wave, kw);
+      load(1, pid, wave, vw);
+    }
     for (int run = b_lo; run < b_hi; run += 64) {
-      // lane i: the run's block i
-      const int pid = run + lane < b_hi ? a.c.page(e, run + lane) : -1;
-      const float ks = pid < 0 ? 0.f : *a.c.scale(pid, 0, head), vs = pid < 0 ? 0.f : *a.c.scale(pid, 1, head);
+      const float next_ks = scale_of(next, 0), next_vs = scale_of(next, 1);
+      const int after = page_of(run + 128);
       const uint64_t there = __builtin_amdgcn_ballot_w64(pid >= 0);
       const int groups = (min(b_hi - run, 64) + KB - 1) / KB;
-      u32x4 kw[KB][C], vw[KB][C];
-      auto load = [&](int side, int i, u32x4 (&w)[KB][C]) {
-#pragma unroll
-        for (int h = 0; h < KB; ++h) {
-          const int page = max(__builtin_amdgcn_readlane(pid, i * KB + h), 0);     // one that is not there: page 0's bytes, masked below
-          const uint8_t* p = a.c.block(page, side, head, D) + (side == 0 ? n * 64 + g * 16 : g * 256 + n * 16);
-#pragma unroll
-          for (int c = 0; c < C; ++c) w[h][c] = *reinterpret_cast<const u32x4*>(p + c * 1024);
-        }
-      };
-      auto lane_of = [](float v, int i) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), i)); };
-      if (wave < groups) {
-        load(0, wave, kw);
-        load(1, wave, vw);
-      }
-      for (int i = wave; i < groups; i += 4) {
+      const bool more = run + 64 + wave * KB < b_hi;     // the wave has a group in the next run
+      for (int i = wave; i < groups; i += W) {
         const int slot0 = (run + i * KB) * kKv8Page;
         f32x4 s[NT][KB];
 #pragma unroll
@@ -172,7 +181,8 @@ __global__ __launch_bounds__(256, (attn_waves<T, D, NT>())) void kv8_attn_kernel
 #pragma unroll
           for (int t = 0; t < NT; ++t) s[t][h] *= f;
         }
-        if (i + 4 < groups) load(0, i + 4, kw);
+        if (i + W < groups) load(0, pid, i + W, kw);
+        else if (more) load(0, next, wave, kw);
         const uint64_t want = ((1ull << KB) - 1) << (i * KB);
         const bool ragged = slot0 + KB * kKv8Page - 1 > all_see || (there & want) != want;
         if (ragged) {
@@ -256,15 +266,20 @@ __global__ __launch_bounds__(256, (attn_waves<T, D, NT>())) void kv8_attn_kernel
 #pragma unroll
             for (int t = 0; t < NT; ++t) o[t][4 * c + j] = kOutside ? o[t][4 * c + j] * alpha[t] + x[t] : x[t];
           }
-        if (i + 4 < groups) load(1, i + 4, vw);
+        if (i + W < groups) load(1, pid, i + W, vw);
+        else if (more) load(1, next, wave, vw);
       }
+      pid = next;
+      next = after;
+      ks = next_ks;
+      vs = next_vs;
     }
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       l[t] = quad_sum(l[t]);
-      // four states into one: waves 2, 3 into 0, 1, then 1 into 0
+      // the waves' states into one: the upper half's into the lower's, and so on
 #pragma unroll
-      for (int half = 2; half >= 1; half >>= 1) {
+      for (int half = W / 2; half >= 1; half >>= 1) {
         __syncthreads();
         if (wave >= half && wave < 2 * half) {
 #pragma unroll
@@ -866,9 +881,12 @@ pegainfer_status_t pegainfer_kv8_attention(const pegainfer_kv8_cache* cache, con
       if (p.prompt) kv8_prompt_kernel<fmt(), D><<<grid, 64 * 8 / prompt_tiles<D>(), 0, as_stream(stream)>>>(a);
     }
     if constexpr (sizeof(T) == 2 || D < 256) {
-      if (!p.prompt && p.row_tiles == 2) kv8_attn_kernel<T, fmt(), D, 2><<<grid, 256, 0, as_stream(stream)>>>(a);
+      if (!p.prompt && p.row_tiles == 2) kv8_attn_kernel<T, fmt(), D, 2, false><<<grid, 256, 0, as_stream(stream)>>>(a);
     }
-    if (!p.prompt && p.row_tiles == 1) kv8_attn_kernel<T, fmt(), D, 1><<<grid, 256, 0, as_stream(stream)>>>(a);
+    if (!p.prompt && p.row_tiles == 1) {
+      if (p.score_rows) kv8_attn_kernel<T, fmt(), D, 1, true><<<grid, 256, 0, as_stream(stream)>>>(a);
+      else if constexpr (sizeof(T) == 4) kv8_attn_kernel<T, fmt(), D, 1, false><<<grid, 256, 0, as_stream(stream)>>>(a);
+    }
     if (p.n_split > 1 && p.n_split <= kFewSplits) kv8_merge_rows_kernel<T, D><<<rows_grid, 256, 0, as_stream(stream)>>>(a);
     if (p.n_split > kFewSplits) kv8_merge_kernel<T, D><<<merge_grid, 64 * std::min(8, p.n_split), 0, as_stream(stream)>>>(a);
     if (weigh) kv8_mass_kernel<T, fmt(), D><<<mass_grid, 256, 0, as_stream(stream)>>>(a, w);
