@@ -954,58 +954,55 @@ def _kv8_need(ok, what):
 
 
 _I32, _F32 = torch.int32, torch.float32
-_KV8_DTYPES = {torch.bfloat16: 0, torch.float32: 1}
+_KV8_DTYPES, _KV8_BLOCKS = {torch.bfloat16: 0, torch.float32: 1}, (1024, 2048, 4096)
 
 
-def _kv8_index(t, n, codes, what):
+def _kv8_index(t, n, device, what):
     """an index table's address; n values (None: any number)"""
-    if t.dtype is not _I32 or t.dim() != 1 or t.stride(0) != 1 or t.device != codes.device or (n is not None and t.numel() != n):
+    if t.dtype is not _I32 or t.dim() != 1 or not t.is_contiguous() or t.get_device() != device or (n is not None and t.numel() != n):
         raise ValueError("kv8: %s: contiguous int32 on the cache's device%s" % (what, "" if n is None else ", %d values" % n))
     return t.data_ptr()
 
 
 def _kv8_cache(codes, scales, page_indptr, page_ids, entries):
-    """-> (descriptor, kv_heads, dim); refuses what the kernels do not take"""
-    fmt, shape, stride, sstride = KV8_FORMATS.get(codes.dtype), codes.shape, codes.stride(), scales.stride()
+    """-> (descriptor, kv_heads, dim, device number); refuses what the kernels do not take"""
+    fmt, device, shape, stride, at = KV8_FORMATS.get(codes.dtype), codes.get_device(), codes.shape, codes.stride(), codes.data_ptr()
     if fmt is None:
         raise ValueError("kv8: codes of torch.float8_e4m3fn or torch.int8")
-    if not codes.is_cuda or codes.get_device() != torch.cuda.current_device():
+    if device < 0 or device != torch.cuda.current_device():
         raise ValueError("kv8: a cache on the current device")
-    if len(shape) != 4 or shape[1] != 2 or shape[3] not in (1024, 2048, 4096) or shape[0] < 1:
-        raise ValueError("kv8: codes [pages, 2, kv_heads, 16 * dim], a page at least, dim 64, 128 or 256")
-    pages, _, kv, m = shape
-    at = codes.data_ptr()
-    if stride[3] != 1 or stride[2] != m or stride[1] != kv * m or stride[0] < 2 * kv * m or (stride[0] | at) % 16:
+    if len(shape) != 4:
+        raise ValueError("kv8: codes [pages, 2, kv_heads, 16 * dim]")
+    pages, two, kv, m = shape
+    if two != 2 or m not in _KV8_BLOCKS or pages < 1 or not 1 <= kv <= 65535 or entries > 65535:
+        raise ValueError("kv8: codes [pages, 2, kv_heads, 16 * dim], a page at least, dim 64, 128 or 256, at most 65535 kv heads and entries")
+    if stride[1:] != (kv * m, m, 1) or stride[0] < 2 * kv * m or (stride[0] | at) % 16:
         raise ValueError("kv8: codes: a page's values together, pages apart by a multiple of 16 bytes")
-    if scales.dtype is not _F32 or scales.device != codes.device or scales.shape != shape[:3] or sstride[2] != 1 or sstride[1] != kv or sstride[0] < 2 * kv:
+    sstride = scales.stride()
+    if scales.dtype is not _F32 or scales.get_device() != device or scales.shape != shape[:3] or sstride[1:] != (kv, 1) or sstride[0] < 2 * kv:
         raise ValueError("kv8: scales fp32 [pages, 2, kv_heads] on the cache's device, a page's together")
-    if not 1 <= kv <= 65535 or entries > 65535:
-        raise ValueError("kv8: at most 65535 kv heads and entries")
-    return Kv8Cache(at, scales.data_ptr(), stride[0], sstride[0], fmt, pages, kv, m // 16, _kv8_index(page_indptr, entries + 1, codes, "page_indptr"),
-                    _kv8_index(page_ids, None, codes, "page_ids"), page_ids.numel(), entries), kv, m // 16
+    return Kv8Cache(at, scales.data_ptr(), stride[0], sstride[0], fmt, pages, kv, m // 16, _kv8_index(page_indptr, entries + 1, device, "page_indptr"),
+                    _kv8_index(page_ids, None, device, "page_ids"), page_ids.numel(), entries), kv, m // 16, device
 
 
-def _kv8_rows(x, heads, dim, codes, what):
-    """row stride of rows of heads"""
-    shape, stride, at = x.shape, x.stride(), x.data_ptr()
-    if x.dtype not in _KV8_DTYPES or x.device != codes.device:
+def _kv8_rows(x, heads, dim, device, what):
+    """-> (rows, heads, row stride, type) of rows of heads"""
+    dtype, shape, stride = _KV8_DTYPES.get(x.dtype), x.shape, x.stride()
+    if dtype is None or x.get_device() != device:
         raise ValueError("kv8: %s: bf16 or fp32 on the cache's device" % what)
     if len(shape) != 3 or shape[2] != dim or (heads is not None and shape[1] != heads):
         raise ValueError("kv8: %s: rows of %s heads of %d values" % (what, "whole" if heads is None else heads, dim))
-    row = shape[1] * dim
-    if shape[0] <= 1:
-        rows = max(row, (stride[0] + 15) // 16 * 16)              # of a single row no stride is used
-    else:
-        rows = stride[0]
-    if stride[2] != 1 or (shape[1] > 1 and stride[1] != dim) or rows < row or (rows * x.element_size() | at) % 16:
+    n, h, _ = shape
+    apart = stride[0] if n > 1 else max(h * dim, (stride[0] + 15) // 16 * 16)     # of a single row no stride is used
+    if stride[2] != 1 or (h > 1 and stride[1] != dim) or apart < h * dim or apart % (4 if dtype else 8) or x.data_ptr() % 16:
         raise ValueError("kv8: %s: a row's values together, rows apart by a multiple of 16 bytes" % what)
-    return rows
+    return n, h, apart, dtype
 
 
 def _kv8_mass(mass, codes, what):
     """page stride of weights"""
     stride = mass.stride()
-    if (mass.dtype is not _F32 or mass.device != codes.device or mass.shape != (codes.shape[0], codes.shape[2], 16) or stride[2] != 1 or stride[1] != 16 or
+    if (mass.dtype is not _F32 or mass.device != codes.device or mass.shape != (codes.shape[0], codes.shape[2], 16) or stride[1:] != (16, 1) or
             stride[0] < codes.shape[2] * 16):
         raise ValueError("kv8: %s fp32 [pages, kv_heads, 16] on the cache's device, a page's together" % what)
     return stride[0]
@@ -1015,23 +1012,24 @@ def kv8_append(k, v, codes, scales, row0, starts, page_indptr, page_ids, max_row
     """rows k, v [rows, kv_heads, dim] (bf16 or fp32 views, row stride free) into the cache behind the starts[e] tokens of their entry.  max_rows: about the most
     rows of an entry (None: all)"""
     entries = row0.numel() - 1
-    cache, kv, dim = _kv8_cache(codes, scales, page_indptr, page_ids, entries)
-    tables = _kv8_index(row0, entries + 1, codes, "row0"), _kv8_index(starts, entries, codes, "starts")
-    strides = _kv8_rows(k, kv, dim, codes, "k"), _kv8_rows(v, kv, dim, codes, "v")
-    _kv8_need(k.dtype == v.dtype and k.shape == v.shape, "k and v of one shape and type")
-    _chk(ffi.lib().pegainfer_kv8_append(ctypes.addressof(cache), k.data_ptr(), v.data_ptr(), *strides, *tables, k.shape[0],
-                                        k.shape[0] if max_rows is None else int(max_rows), _KV8_DTYPES[k.dtype], _stream()), "kv8_append")
+    cache, kv, dim, device = _kv8_cache(codes, scales, page_indptr, page_ids, entries)
+    tables = _kv8_index(row0, entries + 1, device, "row0"), _kv8_index(starts, entries, device, "starts")
+    (n, _, k_apart, dtype), (n_v, _, v_apart, dtype_v) = _kv8_rows(k, kv, dim, device, "k"), _kv8_rows(v, kv, dim, device, "v")
+    _kv8_need(n == n_v and dtype == dtype_v, "k and v of one shape and type")
+    _chk(ffi.lib().pegainfer_kv8_append(ctypes.addressof(cache), k.data_ptr(), v.data_ptr(), k_apart, v_apart, *tables, n, n if max_rows is None else int(max_rows), dtype,
+                                        _stream()), "kv8_append")
 
 
 def kv8_read(codes, scales, row0, starts, page_indptr, page_ids, n_rows, dtype=torch.bfloat16, max_rows=None, out=None):
     """-> k, v [n_rows, kv_heads, dim] of dtype: the slots starts[e] ... of every entry, as many as it has rows.  out: (k, v) to write to; rows behind row0[-1] stay as
     they are (in a fresh tensor: unset)"""
     entries = row0.numel() - 1
-    cache, kv, dim = _kv8_cache(codes, scales, page_indptr, page_ids, entries)
-    tables = _kv8_index(row0, entries + 1, codes, "row0"), _kv8_index(starts, entries, codes, "starts")
+    cache, kv, dim, device = _kv8_cache(codes, scales, page_indptr, page_ids, entries)
+    tables = _kv8_index(row0, entries + 1, device, "row0"), _kv8_index(starts, entries, device, "starts")
     _kv8_need(n_rows >= 0 and dtype in _KV8_DTYPES, "n_rows >= 0, values in bf16 or fp32")
     if out is None:
-        k, v = (torch.empty((n_rows, kv, dim), dtype=dtype, device=codes.device) for _ in range(2))
+        k = torch.empty((n_rows, kv, dim), dtype=dtype, device=codes.device)
+        v = torch.empty_like(k)
     else:
         k, v = out
         for x in out:
@@ -1047,26 +1045,25 @@ def kv8_attention(q, codes, scales, row0, starts, page_indptr, page_ids, scale, 
     entry (None: all rows / all pages).  mass fp32 [pages, kv_heads, 16]: mass_out (None: mass itself) becomes mass_keep * mass + the weight that every token got;
     mass_out alone with mass_keep 0: the weight of this call."""
     entries = row0.numel() - 1
-    cache, kv, dim = _kv8_cache(codes, scales, page_indptr, page_ids, entries)
-    row0_at, starts_at = _kv8_index(row0, entries + 1, codes, "row0"), _kv8_index(starts, entries, codes, "starts")
-    q_stride = _kv8_rows(q, None, dim, codes, "q")
-    T, H, _ = q.shape
+    cache, kv, dim, device = _kv8_cache(codes, scales, page_indptr, page_ids, entries)
+    row0_at, starts_at = _kv8_index(row0, entries + 1, device, "row0"), _kv8_index(starts, entries, device, "starts")
+    T, H, q_apart, dtype = _kv8_rows(q, None, dim, device, "q")
     _kv8_need(H > 0 and H % kv == 0, "query heads: a multiple of the kv heads")
     if out is None:
-        out, out_stride = torch.empty((T, H, dim), dtype=q.dtype, device=q.device), H * dim
+        out, out_apart = torch.empty_like(q, memory_format=torch.contiguous_format), H * dim
     else:
         _kv8_need(out.dtype is q.dtype and out.shape == q.shape, "out like q")
-        out_stride = _kv8_rows(out, H, dim, codes, "out")
+        out_apart = _kv8_rows(out, H, dim, device, "out")[2]
     mass_out = mass if mass_out is None else mass_out
     _kv8_need(mass_out is None or mass is not None or mass_keep == 0, "mass_keep other than 0 needs mass")
-    d = Kv8AttnDesc(q.data_ptr(), q_stride, out.data_ptr(), out_stride, row0_at, starts_at, T, T if max_rows is None else int(max_rows),
-                    page_ids.numel() * 16 if max_len is None else int(max_len), H, float(scale))
+    max_rows, max_len = T if max_rows is None else int(max_rows), page_ids.numel() * 16 if max_len is None else int(max_len)
+    d = Kv8AttnDesc(q.data_ptr(), q_apart, out.data_ptr(), out_apart, row0_at, starts_at, T, max_rows, max_len, H, scale)
+    d.dtype = dtype
     if mass_out is not None:
         if mass is not None:
             d.mass, d.mass_page_stride = mass.data_ptr(), _kv8_mass(mass, codes, "mass")
         d.mass_out, d.mass_out_page_stride, d.mass_keep = mass_out.data_ptr(), _kv8_mass(mass_out, codes, "mass_out"), float(mass_keep)
-    d.dtype = _KV8_DTYPES[q.dtype]
-    n = ffi.lib().pegainfer_kv8_attention_workspace(ctypes.addressof(cache), T, d.max_rows, d.max_len, H, d.dtype, int(mass_out is not None))
+    n = ffi.lib().pegainfer_kv8_attention_workspace(ctypes.addressof(cache), T, max_rows, max_len, H, dtype, mass_out is not None)
     if n > 0:
         ws = torch.empty(n, dtype=torch.float32, device=q.device)
         d.workspace = ws.data_ptr()
@@ -1078,8 +1075,8 @@ def kv8_evict(codes, scales, mass, lens, page_indptr, page_ids, dst_indptr, dst_
     """-> kept int32 [entries, kv_heads, budget]: the slots that stayed, then -1.  Entries of lens[e] tokens are cut to the `budget` heaviest of every kv head (its
     first keep_first and last keep_last among them) and moved, with their mass, to the pages dst_ids[dst_indptr[e]] ..., which are no source pages of the call."""
     entries = lens.numel()
-    cache, kv, _ = _kv8_cache(codes, scales, page_indptr, page_ids, entries)
-    tables = _kv8_index(lens, entries, codes, "lens"), _kv8_index(dst_indptr, entries + 1, codes, "dst_indptr"), _kv8_index(dst_ids, None, codes, "dst_ids")
+    cache, kv, _, device = _kv8_cache(codes, scales, page_indptr, page_ids, entries)
+    tables = _kv8_index(lens, entries, device, "lens"), _kv8_index(dst_indptr, entries + 1, device, "dst_indptr"), _kv8_index(dst_ids, None, device, "dst_ids")
     _kv8_need(budget >= 1 and keep_first >= 0 and keep_last >= 0 and keep_first + keep_last <= budget, "budget of at least 1 token, keep_first + keep_last within it")
     stride = _kv8_mass(mass, codes, "mass")
     kept = torch.empty((entries, kv, budget), dtype=torch.int32, device=codes.device)
