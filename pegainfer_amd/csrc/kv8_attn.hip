@@ -15,6 +15,18 @@ __device__ __forceinline__ float max3(float a, float b, float c) {   // NaN amon
   asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
   return r;
 }
+// Results of matrix instructions that an assembly statement is the first to read: the compiler puts the wait states of that read in front of instructions that it
+// knows, not of assembly (16x16x32: 12 at most), so they stand here, tied to the registers.
+template <int NT, int KB>
+__device__ __forceinline__ void settle(f32x4 (&s)[NT][KB]) {
+  static_assert((NT * KB) % 2 == 0 && (NT * KB <= 2 || (NT * KB) % 8 == 0), "two or eight registers a statement");
+  f32x4* p = &s[0][0];
+  if constexpr (NT * KB == 2) asm("s_nop 15" : "+v"(p[0]), "+v"(p[1]));
+  else
+#pragma unroll
+    for (int i = 0; i < NT * KB; i += 8)
+      asm("s_nop 15" : "+v"(p[i]), "+v"(p[i + 1]), "+v"(p[i + 2]), "+v"(p[i + 3]), "+v"(p[i + 4]), "+v"(p[i + 5]), "+v"(p[i + 6]), "+v"(p[i + 7]));
+}
 // the other half's (of 32) and the other row's (of 16) value, without a trip through shared memory; s_nop: the wait states between a VALU write and the swap.  In
 // assembly because the swap wants two registers, and the builtin given one value twice may be folded to one.
 template <typename Op>
@@ -55,7 +67,7 @@ __device__ __forceinline__ QueryRow query_row(int rr, int total, int group, cons
   return {rows.first + tok, kv_head * group + r - tok * group, start + tok, rr < total};
 }
 
-constexpr int kPromptRows = 128, kFewSplits = 8;
+constexpr int kPromptRows = 128;
 
 // a lane's part of a row's result: the output, or what a split leaves of it
 template <typename T, int D>
@@ -85,9 +97,13 @@ __device__ __forceinline__ void put_row(const AttnArgs& a, const QueryRow& r, in
   }
 }
 
-// Blocks a wave takes at a time, and waves of a SIMD: what the registers hold without spilling.  bf16 heads of 128: 189 registers a wave for one row tile, 256 for two.
-template <typename T, int D> constexpr int attn_kb() { return sizeof(T) == 4 || D == 256 ? 2 : 4; }
-template <typename T, int D, int NT> constexpr int attn_waves() { return D * NT * (sizeof(T) == 4 ? 2 : 1) > 256 || (sizeof(T) == 4 && D == 256) ? 1 : 2; }
+// Blocks a wave takes at a time, and waves of a SIMD: what the registers hold without spilling.  Four blocks of 128 values and two row tiles spill, and are slower by
+// a tenth than two blocks (8 entries of 16 rows over 4000 tokens: 28.2 and 26.4 us); with one tile four are faster over short contexts (1024 tokens: 9.8 and 10.3 us)
+// and two over longer ones of few entries (8 x 4096: 16.2 and 15.2).
+template <typename T, int D, int NT> constexpr int attn_kb() { return D == 64 ? (sizeof(T) == 2 || NT == 1 ? 4 : 2) : D == 128 && sizeof(T) == 2 && NT == 1 ? 4 : 2; }
+template <typename T, int D, int NT> constexpr int attn_waves() {
+  return D == 256 ? (sizeof(T) == 2 && NT == 1 ? 2 : 1) : sizeof(T) == 4 && D * NT == 256 ? 1 : D * NT == 64 && sizeof(T) == 2 ? 3 : 2;
+}
 
 // One workgroup of four waves: NT tiles of sixteen query rows of a kv head over a run of key blocks.  The blocks are dealt to the waves KB at a time, whose states
 // meet in shared memory at the end, so that no key is loaded or widened twice in a workgroup.  Scores are computed transposed (keys x rows): a lane then holds four
@@ -96,7 +112,7 @@ template <typename T, int D, int NT> constexpr int attn_waves() { return D * NT 
 // ONCE: the rows are one tile, so nobody reads the keys again and they pass the caches by (32 x 8192 tokens int8: 78 -> 70 us, 4.8 TB/s).
 template <typename T, int FMT, int D, int NT, bool ONCE>
 __global__ __launch_bounds__(256, (attn_waves<T, D, NT>())) void kv8_attn_kernel(AttnArgs a) {
-  constexpr int NP = kv8_parts<T>(), C = D / 64, KB = attn_kb<T, D>(), W = 4;
+  constexpr int NP = kv8_parts<T>(), C = D / 64, KB = attn_kb<T, D, NT>(), W = 4;
   constexpr bool kScaled = FMT == kE4m3;   // the conversion takes the block's scale along; int8 scales scores and weights instead
   __shared__ f32x4 s_o[W / 2][D / 16][64];
   __shared__ float s_m[W / 2][16], s_l[W / 2][16];
@@ -429,6 +445,7 @@ __global__ __launch_bounds__(64 * 8 / prompt_tiles<D>(), 2) void kv8_prompt_kern
             }
         widen(i + 1, set);
         load(i + 1 + kSets, set);
+        settle<NT, KB>(s);
         float f[KB];                       // the scores are scaled as they enter the exponential, but for masked steps: infinity times a factor that underflows is no mask
 #pragma unroll
         for (int h = 0; h < KB; ++h) f[h] = kScaled ? a.scale_log2 : lane_of(ks, i * KB + h) * a.scale_log2;
@@ -560,10 +577,10 @@ __global__ __launch_bounds__(512) void kv8_merge_kernel(AttnArgs a) {
   }
 }
 
-// The same for many rows of few splits: a wave each.
+// The same for many rows: a wave each, eight splits on their way at a time.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void kv8_merge_rows_kernel(AttnArgs a) {
-  constexpr int V = D / 64;
+  constexpr int V = D / 64, N = 8;
   const int e = blockIdx.z, head = blockIdx.y, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const RowSpan rows = row_span(a.row0, e, a.n_rows);
   const int start = a.starts[e], total = rows.n * a.group;
@@ -573,27 +590,34 @@ __global__ __launch_bounds__(256) void kv8_merge_rows_kernel(AttnArgs a) {
     const int64_t rh = (int64_t)r.row * a.heads + r.head;
     const f32x2* ml = reinterpret_cast<const f32x2*>(a.part_ml) + rh * a.n_split;
     const float* part = a.part_o + rh * a.n_split * D + lane * V;
-    f32x2 x[kFewSplits];
-    float m = -INFINITY, l = 0.f, p[kFewSplits][V], o[V];
-#pragma unroll
-    for (int z = 0; z < kFewSplits; ++z) {
-      const int at = min(z, a.n_split - 1);
-      x[z] = ml[at];
-#pragma unroll
-      for (int v = 0; v < V; ++v) p[z][v] = part[(int64_t)at * D + v];
-      m = fmaxf(m, x[z].x);
-    }
-    const float base = m == -INFINITY ? 0.f : m;
+    float m = -INFINITY, l = 0.f, o[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) o[v] = 0.f;
+    for (int z0 = 0; z0 < a.n_split; z0 += N) {
+      f32x2 x[N];
+      float p[N][V], to = m;
 #pragma unroll
-    for (int z = 0; z < kFewSplits; ++z) {
-      // a split without a key left no sums: what is in their place is not looked at
-      const bool some = z < a.n_split && (x[z].y > 0.f || x[z].y != x[z].y);
-      const float w = exp2_of(x[z].x - base);
-      l += some ? x[z].y * w : 0.f;
+      for (int z = 0; z < N; ++z) {
+        const int at = min(z0 + z, a.n_split - 1);
+        x[z] = ml[at];
 #pragma unroll
-      for (int v = 0; v < V; ++v) o[v] += some ? p[z][v] * w : 0.f;
+        for (int v = 0; v < V; ++v) p[z][v] = part[(int64_t)at * D + v];
+        to = fmaxf(to, x[z].x);
+      }
+      const float base = to == -INFINITY ? 0.f : to, by = exp2_of(m - base);
+      m = to;
+      l *= by;
+#pragma unroll
+      for (int v = 0; v < V; ++v) o[v] *= by;
+#pragma unroll
+      for (int z = 0; z < N; ++z) {
+        // a split without a key left no sums: what is in their place is not looked at
+        const bool some = z0 + z < a.n_split && (x[z].y > 0.f || x[z].y != x[z].y);
+        const float w = exp2_of(x[z].x - base);
+        l += some ? x[z].y * w : 0.f;
+#pragma unroll
+        for (int v = 0; v < V; ++v) o[v] += some ? p[z][v] * w : 0.f;
+      }
     }
     const bool some = l > 0.f || l != l;
     const float inv = some ? 1.f / l : 0.f;
@@ -638,23 +662,6 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? 2 : 1)) void kv8_mass_kernel
   const int start = a.starts[e], total = rows.n * a.group;
   if (rows.n == 0 || start < 0 || start > INT32_MAX - 2048 - rows.n) return;
   const int blocks = (start + rows.n + kKv8Page - 1) / kKv8Page, slice = blockIdx.z % w.n_slice, tiles = (total + 15) / 16;
-  if (a.scores && total <= a.score_rows) {
-    // a step: the attention left its scores, 4 bytes a row and token beside D of the keys
-    const int len = start + rows.n;
-    for (int slot = blockIdx.z * 256 + threadIdx.x; slot < len; slot += gridDim.z * 256) {
-      const int block = slot / kKv8Page, page = a.c.page(e, block);
-      if (page < 0) continue;
-      const float* s = a.scores + (((int64_t)a.c.indptr[e] + block) * a.c.kv_heads + head) * a.score_rows * kKv8Page + slot % kKv8Page;
-      float x = 0.f;
-#pragma unroll 4
-      for (int rr = 0; rr < total; ++rr) {
-        const int tok = rr / a.group;
-        x += exp2_of(s[rr * kKv8Page] - a.lse[(int64_t)(rows.first + tok) * a.heads + head * a.group + rr - tok * a.group]);
-      }
-      put_mass(w, page, head * kKv8Page + slot % kKv8Page, x);
-    }
-    return;
-  }
   for (int w0 = blockIdx.z / w.n_slice * 4 * MB; w0 < blocks; w0 += gridDim.z / w.n_slice * 4 * MB) {
     const int b0 = w0 + wave * MB;
     int page[MB];
@@ -784,6 +791,49 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? 2 : 1)) void kv8_mass_kernel
   }
 }
 
+// The same for steps: a thread a token, whose rows' scores the attention left (4 bytes a row beside D of the keys); an entry with more rows than the call said has
+// none, and its threads take the products themselves.
+template <typename T, int FMT, int D>
+__global__ __launch_bounds__(256) void kv8_step_mass_kernel(AttnArgs a, MassArgs w) {
+  const int e = blockIdx.y, head = blockIdx.x;
+  const RowSpan rows = row_span(a.row0, e, a.n_rows);
+  const int start = a.starts[e], total = rows.n * a.group;
+  if (rows.n == 0 || start < 0 || start > INT32_MAX - 2048 - rows.n) return;
+  const int len = start + rows.n, first_block = a.c.indptr[e];
+  const bool scored = total <= a.score_rows;
+  for (int slot = blockIdx.z * 256 + threadIdx.x; slot < len; slot += gridDim.z * 256) {
+    const int block = slot / kKv8Page, t = slot % kKv8Page, page = a.c.page(e, block);
+    if (page < 0) continue;
+    float x = 0.f;
+    if (scored) {
+      const float* s = a.scores + (((int64_t)first_block + block) * a.c.kv_heads + head) * a.score_rows * kKv8Page + t;
+#pragma unroll 4
+      for (int rr = 0; rr < total; ++rr) {
+        const int tok = rr / a.group;
+        x += exp2_of(s[rr * kKv8Page] - a.lse[(int64_t)(rows.first + tok) * a.heads + head * a.group + rr - tok * a.group]);
+      }
+    } else {
+      const uint8_t* kb = a.c.block(page, 0, head, D) + t * 64;
+      const float ks = *a.c.scale(page, 0, head) * a.scale_log2;
+      for (int tok = max(slot - start, 0); tok < rows.n; ++tok)
+        for (int h = 0; h < a.group; ++h) {
+          const T* q = static_cast<const T*>(a.q) + (rows.first + tok) * a.q_stride + (int64_t)(head * a.group + h) * D;
+          float dot = 0.f;
+#pragma unroll 1
+          for (int d = 0; d < D; d += 4) {
+            float k[4], y[4];
+            kv8_numbers<FMT>(*reinterpret_cast<const uint32_t*>(kb + d / 64 * 1024 + d % 64), k);
+            ld4(q + d, y);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) dot = fmaf(k[i], y[i], dot);
+          }
+          x += exp2_of(fmaf(dot, ks, -a.lse[(int64_t)(rows.first + tok) * a.heads + head * a.group + h]));
+        }
+    }
+    put_mass(w, page, head * kKv8Page + t, x);
+  }
+}
+
 // the slices' sums of a block's tokens, in order: a wave four blocks of a head
 __global__ __launch_bounds__(256) void kv8_mass_sum_kernel(AttnArgs a, MassArgs w) {
   const int e = blockIdx.z, head = blockIdx.y;
@@ -812,14 +862,18 @@ inline AttnPlan attn_plan(const pegainfer_kv8_cache* cache, int n_rows, int max_
   const int64_t want = 2 * device_cus();
   auto cut = [&](int64_t groups, int64_t most) { return (int)std::max<int64_t>(1, std::min((want + groups - 1) / groups, most)); };
   const int64_t groups = p.tiles * pairs;
-  // steps: a workgroup's run is 64 blocks; prompts: 32 at least (a split of 128 rows costs 1 KB a value of the head in sums)
-  p.n_split = p.prompt ? (int)std::max<int64_t>(1, std::min<int64_t>({want / groups, blocks / 32, 256})) : cut(groups, blocks <= 64 ? 1 : std::min((blocks + 15) / 16, 256));
+  // Steps: whole over a run of 64 blocks (1024 tokens: 9.8 us; cut, 8.7 with a merge, whose launch costs the host 4), over more into runs of 16 blocks at least.
+  // Prompts: cut where they leave compute units without one (8 entries of 64 rows over 4000 tokens: 52 us in four, 64 in two), into runs of 32 blocks at least; a
+  // split of 128 rows leaves 1 KB of sums a value of the head (32 entries of 32 rows over 1000 tokens, a workgroup a compute unit: 34 us whole, 46 halved).
+  p.n_split = !p.prompt ? cut(groups, blocks <= 64 ? 1 : std::min((blocks + 15) / 16, 256))
+              : groups >= device_cus() ? 1
+                                       : (int)std::max<int64_t>(1, std::min<int64_t>({want / groups, blocks / 32, 256}));
   p.split_blocks = ceil_div(blocks, p.n_split);
   p.round = (int)std::max<int64_t>(1, device_cus() / pairs);
   p.snake = p.n_split == 1 && p.tiles > p.round && p.tiles <= 2 * p.round;
   p.score_rows = rows <= 16 ? (int)rows : 0;
   p.mass_groups = p.score_rows ? ceil_div(blocks, 256 / kKv8Page) : ceil_div(blocks, 4 * (cache->dim == 256 ? mass_blocks<256>() : mass_blocks<128>()));
-  p.n_slice = cut((p.mass_groups * pairs + 1) / 2, std::min<int64_t>((rows + 255) / 256, 16));   // the first keys' rows are twice the average's
+  p.n_slice = p.score_rows ? 1 : cut((p.mass_groups * pairs + 1) / 2, std::min<int64_t>((rows + 255) / 256, 16));   // the first keys' rows are twice the average's
   return p;
 }
 // workgroups of `items` pieces of work cut `ways`, in whole pieces; kernels walk what a grid cannot hold
@@ -870,6 +924,8 @@ pegainfer_status_t pegainfer_kv8_attention(const pegainfer_kv8_cache* cache, con
   // the short ones fill the end.  The entries change places from round to round, and where two rounds are all the second starts with the shortest: what shares a
   // compute unit is a long piece and a short one.
   const dim3 grid(cache->kv_heads, cache->n_entries, deal(p.tiles, p.n_split)), mass_grid(cache->kv_heads, cache->n_entries, deal(p.mass_groups, p.n_slice));
+  // splits of 2048 rows and heads fill the chip with a wave each; of fewer, a workgroup each shortens the walk over many splits
+  const bool many = p.n_split <= 8 || rh >= 2048;
   const dim3 merge_grid(std::min(d->max_rows, d->n_rows) * group * (cache->dim / 64), cache->kv_heads, cache->n_entries);
   const dim3 rows_grid(ceil_div((int64_t)std::min(d->max_rows, d->n_rows) * group, 4), cache->kv_heads, cache->n_entries);
   const dim3 sum_grid(std::max(1, ceil_div(d->max_len, 256)), cache->kv_heads, cache->n_entries);
@@ -885,11 +941,12 @@ pegainfer_status_t pegainfer_kv8_attention(const pegainfer_kv8_cache* cache, con
     }
     if (!p.prompt && p.row_tiles == 1) {
       if (p.score_rows) kv8_attn_kernel<T, fmt(), D, 1, true><<<grid, 256, 0, as_stream(stream)>>>(a);
-      else if constexpr (sizeof(T) == 4) kv8_attn_kernel<T, fmt(), D, 1, false><<<grid, 256, 0, as_stream(stream)>>>(a);
+      else if constexpr (sizeof(T) == 4 && D == 256) kv8_attn_kernel<T, fmt(), D, 1, false><<<grid, 256, 0, as_stream(stream)>>>(a);
     }
-    if (p.n_split > 1 && p.n_split <= kFewSplits) kv8_merge_rows_kernel<T, D><<<rows_grid, 256, 0, as_stream(stream)>>>(a);
-    if (p.n_split > kFewSplits) kv8_merge_kernel<T, D><<<merge_grid, 64 * std::min(8, p.n_split), 0, as_stream(stream)>>>(a);
-    if (weigh) kv8_mass_kernel<T, fmt(), D><<<mass_grid, 256, 0, as_stream(stream)>>>(a, w);
+    if (p.n_split > 1 && many) kv8_merge_rows_kernel<T, D><<<rows_grid, 256, 0, as_stream(stream)>>>(a);
+    if (p.n_split > 1 && !many) kv8_merge_kernel<T, D><<<merge_grid, 64 * std::min(8, p.n_split), 0, as_stream(stream)>>>(a);
+    if (weigh && p.score_rows) kv8_step_mass_kernel<T, fmt(), D><<<mass_grid, 256, 0, as_stream(stream)>>>(a, w);
+    else if (weigh) kv8_mass_kernel<T, fmt(), D><<<mass_grid, 256, 0, as_stream(stream)>>>(a, w);
   });
   if (weigh && p.n_slice > 1) kv8_mass_sum_kernel<<<sum_grid, 256, 0, as_stream(stream)>>>(a, w);
   return (pegainfer_status_t)hipGetLastError();

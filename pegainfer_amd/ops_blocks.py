@@ -1052,7 +1052,7 @@ def kv8_attention(q, codes, scales, row0, starts, page_indptr, page_ids, scale, 
     if out is None:
         out, out_apart = torch.empty_like(q, memory_format=torch.contiguous_format), H * dim
     else:
-        _kv8_need(out.dtype is q.dtype and out.shape == q.shape, "out like q")
+        _kv8_need(out.dtype is q.dtype and out.shape == q.shape and out.data_ptr() != q.data_ptr(), "out like q, not q itself")
         out_apart = _kv8_rows(out, H, dim, device, "out")[2]
     mass_out = mass if mass_out is None else mass_out
     _kv8_need(mass_out is None or mass is not None or mass_keep == 0, "mass_keep other than 0 needs mass")
