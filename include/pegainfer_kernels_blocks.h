@@ -1102,10 +1102,10 @@ pegainfer_status_t pegainfer_kv8_read(const pegainfer_kv8_cache* cache, const in
 /* Causal softmax attention: row i of entry e sees the slots up to starts[e] + i (its own token is in the cache already), query head h reads kv head
  * h / (heads / kv_heads);  scale >= 0;  out[row, h] = sum_j softmax_j(scale q . k_j) v_j, zeros where a row sees nothing.  q, out: rows [heads][dim] of dtype at strides of
  * 16 bytes.  Scores, softmax state and sums are fp32; bf16: the softmax weights are rounded to bf16 where they enter the matrix cores (their sum is not); fp32:
- * queries and weights enter as three bf16 parts, nothing is rounded.
+ * queries and weights enter as three bf16 parts, nothing is rounded.  Entries may share pages (a common prompt).  out is not q.
  * mass_out given: mass_out[page][kv head][16] (fp32, pages mass_out_page_stride values apart) = mass_keep * mass + the weight that the call's rows and the kv
  * head's query heads gave to the token, for every slot of an entry that has rows (mass_out may be mass; mass_keep 0: mass is not read and may be NULL).  Every
- * sum has one order: results do not change from run to run.
+ * sum has one order: results do not change from run to run.  A page that two entries of such a call shared would be written by both: it is a page of one.
  * workspace: fp32 scratch on 16 bytes of pegainfer_kv8_attention_workspace(...) values, of this call alone until it is done (0: NULL). */
 typedef struct {
   const void* q;

@@ -165,6 +165,46 @@ def test_runs_repeat_bit_for_bit():
         assert torch.equal(a, b) and torch.equal(d.mass, first)
 
 
+@pytest.mark.parametrize("rows", [1, 20, 80])
+def test_a_row_that_is_not_a_number_spoils_itself_alone(rows):
+    c = Cache([50], [rows], 1, 128, "e4m3", seed=30)
+    d = c.device()
+    q = torch.randn(rows, 4, 128, device="cuda").bfloat16()
+    want = B.kv8_attention(q, d.codes, d.scales, d.row0, d.starts, d.indptr, d.ids, 0.1)
+    q[0, 1, 5], q[rows - 1, 2, 7] = float("nan"), float("inf")
+    got = B.kv8_attention(q, d.codes, d.scales, d.row0, d.starts, d.indptr, d.ids, 0.1)
+    spoiled = torch.zeros(rows, 4, dtype=torch.bool)
+    spoiled[0, 1] = spoiled[rows - 1, 2] = True
+    assert torch.equal(got[~spoiled], want[~spoiled]) and torch.isnan(got[0, 1]).all()
+
+
+@pytest.mark.parametrize("entries,kv,group", [(300, 1, 1), (3, 9, 1), (2, 1, 64), (1, 40, 2)])
+def test_attention_of_many_entries_and_heads(entries, kv, group):
+    rng = np.random.RandomState(entries)
+    c = Cache([int(x) for x in rng.randint(0, 90, entries)], [1] * entries, kv, 64, "int8", seed=5)
+    attend(c, kv * group, torch.bfloat16, weigh=True)
+
+
+def test_no_rows_and_no_pages():
+    c = Cache([20, 3], [0, 0], 2, 64, "e4m3")
+    d = c.device()
+    out = torch.full((3, 4, 64), 7.0, device="cuda")
+    mass = d.mass.clone()
+    B.kv8_attention(torch.zeros_like(out), d.codes, d.scales, d.row0, d.starts, d.indptr, d.ids, 1.0, out=out, mass=d.mass)
+    pool = d.pool.clone()
+    B.kv8_append(torch.zeros(3, 2, 64, device="cuda"), torch.zeros(3, 2, 64, device="cuda"), d.codes, d.scales, d.row0, d.starts, d.indptr, d.ids)
+    assert (out == 7).all() and torch.equal(d.mass, mass) and torch.equal(d.pool, pool)
+    # rows of entries that own no pages at all: zeros, nothing written, nothing kept but places
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    row0, starts, none = i32([0, 1, 3]), i32([0, 40]), i32([])
+    B.kv8_append(torch.ones(3, 2, 64, device="cuda"), torch.ones(3, 2, 64, device="cuda"), d.codes, d.scales, row0, starts, i32([0, 0, 0]), none)
+    B.kv8_attention(torch.ones_like(out), d.codes, d.scales, row0, starts, i32([0, 0, 0]), none, 1.0, out=out, mass=d.mass)
+    k, v = B.kv8_read(d.codes, d.scales, row0, starts, i32([0, 0, 0]), none, 3)
+    kept = B.kv8_evict(d.codes, d.scales, d.mass, i32([5, 40]), i32([0, 0, 0]), none, i32([0, 0, 0]), none, 16, 2, 2)
+    assert (out == 0).all() and (k == 0).all() and (v == 0).all() and torch.equal(d.mass, mass) and torch.equal(d.pool, pool)
+    assert kept[0, 0].tolist() == [0, 1, 2, 3, 4] + [-1] * 11 and kept[1, 1].tolist() == list(range(14)) + [38, 39]
+
+
 def test_tables_that_lead_nowhere():
     """pages out of range, tables that end early, rows out of range, entries that start nowhere: not there, and nothing else is touched"""
     c = Cache([20, 40, 5, 33, 70], [4, 1, 1, 2, 1], 2, 64, "int8", seed=8)
@@ -343,6 +383,43 @@ def test_a_captured_step_replays_with_other_tables():
             d.starts += 1
 
 
+def test_a_captured_prompt_and_eviction_replay():
+    """a portion of a prompt with weights, the cut and what is read back, captured once and replayed over other values, with eager work in between"""
+    kv, H, dim, budget = 2, 8, 64, 100
+    c = Cache([40, 0], [150, 60], kv, dim, "int8", seed=31, pages=80, dirty=False)
+    free = [p for p in range(c.pages) if p not in c.ids]
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    dst, ids = i32([0, 7, 14]), i32(free[:14])
+    zeros = i32([0, 0])
+    back0 = i32([0, 100, 160])
+    a, b = c.device(), c.device()
+    k, q = torch.randn(210, kv, dim, device="cuda"), torch.randn(210, H, dim, device="cuda")
+
+    def step(d):
+        t = d.row0, d.starts, d.indptr, d.ids
+        B.kv8_append(k, k, d.codes, d.scales, *t)
+        out = B.kv8_attention(q, d.codes, d.scales, *t, 0.2, mass=d.mass, mass_keep=0.5)
+        kept = B.kv8_evict(d.codes, d.scales, d.mass, d.lens, d.indptr, d.ids, dst, ids, budget, 4, 10)
+        return (out, kept) + B.kv8_read(d.codes, d.scales, back0, zeros, dst, ids, 160)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(c.device())
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(a)
+    for i in range(4):
+        k.copy_(torch.randn_like(k) * (i + 1))
+        q.copy_(torch.randn_like(q))
+        graph.replay()
+        want = step(b)
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(got, want)) and torch.equal(a.mass, b.mass) and torch.equal(a.pool, b.pool) and torch.equal(a.scales, b.scales), i
+
+
 def test_two_streams_at_once():
     """the same operators on two streams, each with its cache: workspaces are not shared"""
     c = [Cache([700, 30], [1, 20], 2, 128, f, seed=s) for s, f in enumerate(TORCH)]
@@ -388,7 +465,7 @@ def test_wrappers_refuse():
     assert go().shape == q.shape
     for kw in [dict(q=q.half()), dict(q=q.float()[..., ::2]), dict(q=q[:, :3]), dict(q=q[..., :32]), dict(q=q.cpu()), dict(q=q.transpose(0, 1)), dict(codes=d.pool[:, -1]),
                dict(codes=d.codes[..., :1000]), dict(codes=d.codes.cpu()), dict(scales=d.scales[:-1]), dict(scales=d.scales.double()), dict(row0=d.row0.long()), dict(row0=d.row0.cpu()),
-               dict(starts=d.indptr), dict(page_indptr=d.starts), dict(out=q.float()), dict(out=q[:2]), dict(mass=d.mass[..., :8]), dict(mass=d.mass.double()),
+               dict(starts=d.indptr), dict(page_indptr=d.starts), dict(out=q.float()), dict(out=q[:2]), dict(out=q), dict(scale=-1.0), dict(scale=float("nan")), dict(mass=d.mass[..., :8]), dict(mass=d.mass.double()),
                dict(mass_out=d.mass), dict(page_ids=d.ids[None]), dict(max_rows=-1), dict(max_len=-1)]:
         with pytest.raises((ValueError, RuntimeError)):
             go(**kw)
