@@ -2,7 +2,8 @@
  * pegainfer_kernels_blocks.h - building blocks of libpegainfer_kernels_hip.so that are not tied to one model family
  * and exist in a bf16 and a true-fp32 instance: Dynamic-Tanh norms over an fp32 residual stream, squared-ReLU and
  * SwiGLU activations, a strided / batched / grouped GEMM, attention over a paged LATENT cache (one compressed key/value
- * vector plus one shared rotated key part per token), and sigmoid-scored grouped top-k expert routing.
+ * vector plus one shared rotated key part per token), sigmoid-scored grouped top-k expert routing, and a paged key/value cache
+ * held in 8 bits.
  *
  * Conventions: device pointers; `dtype` 0 = bf16 bit patterns, 1 = float (storage of activations AND weights of that
  * call); all arithmetic is fp32; stream last; every function only enqueues work and returns hipGetLastError() as int.

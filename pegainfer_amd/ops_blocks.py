@@ -1,7 +1,8 @@
 """Torch-tensor wrappers over include/pegainfer_kernels_blocks.h: the model-independent blocks that exist in a bf16 and a
 true-fp32 instance (Dynamic-Tanh norms over an fp32 stream, activations, the strided / batched / grouped GEMM, attention
 over a paged latent cache, routing; time convolutions with carried tails, grouped output norms with a depth-weighted
-sum, clamp-GLU, recurrent matrix memories over per-request state, attention over a paged key/value cache).  Tensors are torch CUDA tensors used as device memory; the
+sum, clamp-GLU, recurrent matrix memories over per-request state, attention over a paged key/value cache; a paged
+key/value cache held in 8 bits).  Tensors are torch CUDA tensors used as device memory; the
 storage type of a call (bf16 / fp32) is taken from the activation tensor.  Work is enqueued on torch's current stream.
 No CPU fallback: without the HIP library every call raises ImportError.
 """
