@@ -130,6 +130,7 @@ def evict(codes, scales, fmt, dim, mass, lens, tables, dst, budget, first, last)
     kept = np.full((len(lens), kv, budget), -1, np.int32)
     was_codes, was_scales, was_mass = codes.copy(), scales.copy(), mass.copy()
     for e, n in enumerate(lens):
+        n = max(0, min(n, PAGE * min(tables[0][e + 1] - tables[0][e], len(tables[1]))))      # no more tokens than its table has places
         for h in range(kv):
             stay = list(range(n))
             if n > budget:

@@ -143,7 +143,7 @@ __global__ __launch_bounds__(256, (attn_waves<T, D, NT>())) void kv8_attn_kernel
     }
     // slots that every row of the tiles sees, and that any does
     const int all_see = tile * NT * 16 / a.group + start, any_sees = min((tile + 1) * NT * 16 - 1, total - 1) / a.group + start;
-    const int blocks = any_sees / kKv8Page + 1, per = max(a.split_blocks, (blocks + a.n_split - 1) / a.n_split);
+    const int blocks = min(any_sees / kKv8Page + 1, a.c.blocks(e)), per = max(a.split_blocks, (blocks + a.n_split - 1) / a.n_split);
     const int b_lo = split * per, b_hi = min(blocks, b_lo + per);
     // lane i: block i of a run of 64; the pages of a run are looked up two runs ahead, their scales one
     auto page_of = [&](int run) { return run + lane < b_hi ? a.c.page(e, run + lane) : -1; };
@@ -361,7 +361,7 @@ __global__ __launch_bounds__(64 * 8 / prompt_tiles<D>(), 2) void kv8_prompt_kern
       for (int i = 0; i < D / 16; ++i) o[t][i] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
     const int all_see = tile * kPromptRows / a.group + start, any_sees = min((tile + 1) * kPromptRows - 1, total - 1) / a.group + start;
-    const int blocks = any_sees / kKv8Page + 1, per = (max(a.split_blocks, (blocks + a.n_split - 1) / a.n_split) + KB - 1) / KB * KB;
+    const int blocks = min(any_sees / kKv8Page + 1, a.c.blocks(e)), per = (max(a.split_blocks, (blocks + a.n_split - 1) / a.n_split) + KB - 1) / KB * KB;
     const int b_lo = split * per, b_hi = min(blocks, b_lo + per);
     auto lane_of = [](float v, int i) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), i)); };
     for (int run = b_lo; run < b_hi; run += 64) {
@@ -663,7 +663,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? 2 : 1)) void kv8_mass_kernel
   const RowSpan rows = row_span(a.row0, e, a.n_rows);
   const int start = a.starts[e], total = rows.n * a.group;
   if (rows.n == 0 || start < 0 || start > INT32_MAX - 2048 - rows.n) return;
-  const int blocks = (start + rows.n + kKv8Page - 1) / kKv8Page, slice = blockIdx.z % w.n_slice, tiles = (total + 15) / 16;
+  const int blocks = min((start + rows.n + kKv8Page - 1) / kKv8Page, a.c.blocks(e)), slice = blockIdx.z % w.n_slice, tiles = (total + 15) / 16;
   for (int w0 = blockIdx.z / w.n_slice * 4 * MB; w0 < blocks; w0 += gridDim.z / w.n_slice * 4 * MB) {
     const int b0 = w0 + wave * MB;
     int page[MB];
@@ -820,7 +820,7 @@ __global__ __launch_bounds__(256) void kv8_step_finish_kernel(AttnArgs a, MassAr
     for (int rr = blockIdx.z * 4 + wave; rr < total; rr += merges * 4) merge_row<T, D>(a, query_row(rr, total, a.group, rows, start, head), lane);
     return;
   }
-  const int len = start + rows.n, first_block = a.c.indptr[e], z = blockIdx.z - merges;
+  const int len = a.c.tokens(e, start + rows.n), first_block = a.c.indptr[e], z = blockIdx.z - merges;
   if (z * 256 >= len) return;
   const bool scored = total <= a.score_rows;
   auto row_head = [&](int rr) { const QueryRow r = query_row(rr, total, a.group, rows, start, head); return (int64_t)r.row * a.heads + r.head; };
@@ -869,7 +869,7 @@ __global__ __launch_bounds__(256) void kv8_mass_sum_kernel(AttnArgs a, MassArgs 
   const RowSpan rows = row_span(a.row0, e, a.n_rows);
   const int start = a.starts[e];
   if (rows.n == 0 || start < 0 || start > INT32_MAX - 2048 - rows.n) return;
-  const int len = start + rows.n;
+  const int len = a.c.tokens(e, start + rows.n);
   for (int slot = blockIdx.x * 256 + threadIdx.x; slot < len; slot += gridDim.x * 256) {
     const int block = slot / kKv8Page, page = a.c.page(e, block), at = head * kKv8Page + slot % kKv8Page;
     if (page < 0) continue;

@@ -197,7 +197,7 @@ __global__ __launch_bounds__(kPickThreads) void kv8_pick_kernel(Kv8 c, const flo
   __shared__ uint32_t s_bits;
   __shared__ int s_left;
   const int e = blockIdx.y, head = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int len = max(lens[e], 0);
+  const int len = c.tokens(e, lens[e]);
   int32_t* out = kept + ((int64_t)e * c.kv_heads + head) * budget;
   if (len <= budget) {
     for (int i = tid; i < budget; i += kPickThreads) out[i] = i < len ? i : -1;
@@ -208,6 +208,9 @@ __global__ __launch_bounds__(kPickThreads) void kv8_pick_kernel(Kv8 c, const flo
     return page < 0 ? 0u : order_of(mass[page * mass_stride + head * kKv8Page + s % kKv8Page]);
   };
   const bool held = len <= cached;
+  const int lo = keep_first, hi = len - keep_last, chosen = budget - keep_first - keep_last;
+  for (int i = tid; i < 2048; i += kPickThreads) hist[i] = 0;
+  __syncthreads();
   if (held && c.n_ids > 0) {
     // sixteen slots a thread at a time, page ids and weights each in one go: what is not there is read from the table's and the cache's first place and left out
     const int first = c.indptr[e], pages = c.indptr[e + 1] - first;
@@ -225,26 +228,34 @@ __global__ __launch_bounds__(kPickThreads) void kv8_pick_kernel(Kv8 c, const flo
 #pragma unroll
       for (int i = 0; i < N; ++i) m[i] = mass[max(page[i], 0) * mass_stride + head * kKv8Page + (s0 + i * kPickThreads) % kKv8Page];
 #pragma unroll
-      for (int i = 0; i < N; ++i)
-        if (s0 + i * kPickThreads < len) s_order[s0 + i * kPickThreads] = page[i] < 0 ? 0u : order_of(m[i]);
+      for (int i = 0; i < N; ++i) {
+        const int s = s0 + i * kPickThreads;
+        const uint32_t w = page[i] < 0 ? 0u : order_of(m[i]);
+        if (s < len) s_order[s] = w;
+        if (s >= lo && s < hi) atomicAdd(&hist[w >> 21], 1u);
+      }
     }
   } else if (held) {
     for (int s = tid; s < len; s += kPickThreads) s_order[s] = 0;
+    if (tid == 0 && hi > lo) hist[0] = hi - lo;
   }
   auto weight = [&](int s) { return held ? s_order[s] : fetch(s); };
-  const int lo = keep_first, hi = len - keep_last, chosen = budget - keep_first - keep_last;
   uint32_t bits = 0;                       // of the lightest weight that stays: its upper bits so far
   int left = chosen;                       // tokens still to be found that have those
   if (chosen > 0) {
     for (int done = 0; done < 32; done += 11) {
       const int width = min(11, 32 - done), shift = 32 - done - width;
-      for (int i = tid; i < 2048; i += kPickThreads) hist[i] = 0;
-      __syncthreads();
+      if (done > 0) {
+        for (int i = tid; i < 2048; i += kPickThreads) hist[i] = 0;
+        __syncthreads();
+      }
       const uint32_t mask = done == 0 ? 0u : 0xFFFFFFFFu << (32 - done);
+      if (done > 0 || !held) {             // the first is counted as the weights arrive
 #pragma unroll 4
-      for (int s = lo + tid; s < hi; s += kPickThreads) {
-        const uint32_t w = weight(s);
-        if ((w & mask) == bits) atomicAdd(&hist[(w >> shift) & 2047 >> (11 - width)], 1u);
+        for (int s = lo + tid; s < hi; s += kPickThreads) {
+          const uint32_t w = weight(s);
+          if ((w & mask) == bits) atomicAdd(&hist[(w >> shift) & 2047 >> (11 - width)], 1u);
+        }
       }
       __syncthreads();
       // thread t: digits 2047 - 2 t and 2046 - 2 t; how many weights have a larger digit
@@ -311,7 +322,7 @@ template <int FMT, int D>
 __global__ __launch_bounds__(128) void kv8_move_kernel(Kv8 c, const int32_t* dst_indptr, const int32_t* dst_ids, int n_dst_ids, float* mass, int64_t mass_stride,
                                                        const int32_t* lens, int budget, const int32_t* kept) {
   const int e = blockIdx.z, head = blockIdx.y, side = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 15, q = lane >> 4;
-  const int len = min(max(lens[e], 0), budget);
+  const int len = min(c.tokens(e, lens[e]), budget);
   const int32_t* from = kept + ((int64_t)e * c.kv_heads + head) * budget;
   Kv8 to = c;
   to.indptr = dst_indptr;

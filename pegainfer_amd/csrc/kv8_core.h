@@ -34,6 +34,10 @@ struct Kv8 {
     const int id = ids[at];
     return (unsigned)id < (unsigned)n_pages ? id : -1;
   }
+  // blocks that an entry's table has: no length, whatever its table holds, makes a walk longer than this
+  __device__ __forceinline__ int blocks(int e) const { return max(0, min(indptr[e + 1] - indptr[e], n_ids)); }
+  // tokens of an entry said to have n
+  __device__ __forceinline__ int tokens(int e, int n) const { return (int)max((int64_t)0, min((int64_t)n, (int64_t)blocks(e) * kKv8Page)); }
   __device__ __forceinline__ uint8_t* block(int page, int side, int head, int dim) const {
     return codes + page * code_stride + (int64_t)(side * kv_heads + head) * (kKv8Page * dim);
   }

@@ -1009,15 +1009,20 @@ def _kv8_mass(mass, codes, what):
     return stride[0]
 
 
+def _kv8_most(given, total, entries):
+    """a hint of the most of an entry: as given, or the average"""
+    return int(given) if given is not None else -(-total // max(entries, 1))
+
+
 def kv8_append(k, v, codes, scales, row0, starts, page_indptr, page_ids, max_rows=None):
     """rows k, v [rows, kv_heads, dim] (bf16 or fp32 views, row stride free) into the cache behind the starts[e] tokens of their entry.  max_rows: about the most
-    rows of an entry (None: all)"""
+    rows of an entry (None: the average); it shapes the grid, the results are those of any"""
     entries = row0.numel() - 1
     cache, kv, dim, device = _kv8_cache(codes, scales, page_indptr, page_ids, entries)
     tables = _kv8_index(row0, entries + 1, device, "row0"), _kv8_index(starts, entries, device, "starts")
     (n, _, k_apart, dtype), (n_v, _, v_apart, dtype_v) = _kv8_rows(k, kv, dim, device, "k"), _kv8_rows(v, kv, dim, device, "v")
     _kv8_need(n == n_v and dtype == dtype_v, "k and v of one shape and type")
-    _chk(ffi.lib().pegainfer_kv8_append(ctypes.addressof(cache), k.data_ptr(), v.data_ptr(), k_apart, v_apart, *tables, n, n if max_rows is None else int(max_rows), dtype,
+    _chk(ffi.lib().pegainfer_kv8_append(ctypes.addressof(cache), k.data_ptr(), v.data_ptr(), k_apart, v_apart, *tables, n, _kv8_most(max_rows, n, entries), dtype,
                                         _stream()), "kv8_append")
 
 
@@ -1037,13 +1042,13 @@ def kv8_read(codes, scales, row0, starts, page_indptr, page_ids, n_rows, dtype=t
             _kv8_need(x.shape == (n_rows, kv, dim) and x.dtype is dtype and x.device == codes.device and x.is_contiguous() and x.data_ptr() % 16 == 0,
                       "out: two contiguous tensors [n_rows, kv_heads, dim] of dtype")
     _chk(ffi.lib().pegainfer_kv8_read(ctypes.addressof(cache), *tables, k.data_ptr(), v.data_ptr(), int(n_rows),
-                                      int(n_rows if max_rows is None else max_rows), _KV8_DTYPES[dtype], _stream()), "kv8_read")
+                                      _kv8_most(max_rows, n_rows, entries), _KV8_DTYPES[dtype], _stream()), "kv8_read")
     return k, v
 
 
 def kv8_attention(q, codes, scales, row0, starts, page_indptr, page_ids, scale, max_rows=None, max_len=None, out=None, mass=None, mass_out=None, mass_keep=1.0):
     """-> out [rows, heads, dim]: causal attention of q's rows (their own tokens are in the cache already).  max_rows / max_len: about the most rows / tokens of an
-    entry (None: all rows / all pages).  mass fp32 [pages, kv_heads, 16]: mass_out (None: mass itself) becomes mass_keep * mass + the weight that every token got;
+    entry (None: the average of the rows, twice that of the pages); they choose how the call is cut, results are right for any.  mass fp32 [pages, kv_heads, 16]: mass_out (None: mass itself) becomes mass_keep * mass + the weight that every token got;
     mass_out alone with mass_keep 0: the weight of this call."""
     entries = row0.numel() - 1
     cache, kv, dim, device = _kv8_cache(codes, scales, page_indptr, page_ids, entries)
@@ -1057,7 +1062,7 @@ def kv8_attention(q, codes, scales, row0, starts, page_indptr, page_ids, scale, 
         out_apart = _kv8_rows(out, H, dim, device, "out")[2]
     mass_out = mass if mass_out is None else mass_out
     _kv8_need(mass_out is None or mass is not None or mass_keep == 0, "mass_keep other than 0 needs mass")
-    max_rows, max_len = T if max_rows is None else int(max_rows), page_ids.numel() * 16 if max_len is None else int(max_len)
+    max_rows, max_len = _kv8_most(max_rows, T, entries), _kv8_most(max_len, page_ids.numel() * 32, entries)
     d = Kv8AttnDesc(q.data_ptr(), q_apart, out.data_ptr(), out_apart, row0_at, starts_at, T, max_rows, max_len, H, scale)
     d.dtype = dtype
     if mass_out is not None:
@@ -1082,6 +1087,6 @@ def kv8_evict(codes, scales, mass, lens, page_indptr, page_ids, dst_indptr, dst_
     stride = _kv8_mass(mass, codes, "mass")
     kept = torch.empty((entries, kv, budget), dtype=torch.int32, device=codes.device)
     _chk(ffi.lib().pegainfer_kv8_evict(ctypes.addressof(cache), mass.data_ptr(), stride, *tables, dst_ids.numel(),
-                                       int(budget), int(keep_first), int(keep_last), page_ids.numel() * 16 if max_len is None else int(max_len), kept.data_ptr(),
+                                       int(budget), int(keep_first), int(keep_last), _kv8_most(max_len, page_ids.numel() * 32, entries), kept.data_ptr(),
                                        _stream()), "kv8_evict")
     return kept

@@ -194,7 +194,7 @@ def test_no_rows_and_no_pages():
     pool = d.pool.clone()
     B.kv8_append(torch.zeros(3, 2, 64, device="cuda"), torch.zeros(3, 2, 64, device="cuda"), d.codes, d.scales, d.row0, d.starts, d.indptr, d.ids)
     assert (out == 7).all() and torch.equal(d.mass, mass) and torch.equal(d.pool, pool)
-    # rows of entries that own no pages at all: zeros, nothing written, nothing kept but places
+    # rows of entries that own no pages at all: zeros, nothing written, nothing kept
     i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
     row0, starts, none = i32([0, 1, 3]), i32([0, 40]), i32([])
     B.kv8_append(torch.ones(3, 2, 64, device="cuda"), torch.ones(3, 2, 64, device="cuda"), d.codes, d.scales, row0, starts, i32([0, 0, 0]), none)
@@ -202,7 +202,30 @@ def test_no_rows_and_no_pages():
     k, v = B.kv8_read(d.codes, d.scales, row0, starts, i32([0, 0, 0]), none, 3)
     kept = B.kv8_evict(d.codes, d.scales, d.mass, i32([5, 40]), i32([0, 0, 0]), none, i32([0, 0, 0]), none, 16, 2, 2)
     assert (out == 0).all() and (k == 0).all() and (v == 0).all() and torch.equal(d.mass, mass) and torch.equal(d.pool, pool)
-    assert kept[0, 0].tolist() == [0, 1, 2, 3, 4] + [-1] * 11 and kept[1, 1].tolist() == list(range(14)) + [38, 39]
+    assert (kept == -1).all()
+
+
+def test_lengths_and_starts_of_any_size_end():
+    """what a table says of a length goes no further than the entry's pages: these calls end at once, and give what the pages hold"""
+    c = Cache([31, 15], [1, 1], 2, 64, "int8", seed=33)
+    d = c.device()
+    q = torch.randn(2, 4, 64, device="cuda").bfloat16()
+    want = B.kv8_attention(q, d.codes, d.scales, d.row0, d.starts, d.indptr, d.ids, 0.1)
+    weights = torch.zeros_like(d.mass)
+    B.kv8_attention(q, d.codes, d.scales, d.row0, d.starts, d.indptr, d.ids, 0.1, mass_out=weights, mass_keep=0.0)
+    far = torch.tensor([2 ** 31 - 5000, 2 ** 30], dtype=torch.int32, device="cuda")           # every slot of the pages lies before them
+    for row0, rows in ((d.row0, q), (torch.tensor([0, 100, 200], dtype=torch.int32, device="cuda"), torch.randn(200, 4, 64, device="cuda").bfloat16())):
+        again = torch.zeros_like(d.mass)
+        got = B.kv8_attention(rows, d.codes, d.scales, row0, far, d.indptr, d.ids, 0.1, mass_out=again, mass_keep=0.0)
+        assert torch.isfinite(got).all()
+        if rows is q:
+            assert torch.equal(got, want) and torch.equal(again, weights)
+    free = [p for p in range(c.pages) if p not in c.ids]
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    for lens in ([2 ** 31 - 1, -5], [2 ** 30, 2 ** 31 - 1]):
+        kept = B.kv8_evict(d.codes, d.scales, d.mass, i32(lens), d.indptr, d.ids, i32([0, 1, 2]), i32(free[:2]), 10, 2, 3)
+        assert kept[0, :, :2].tolist() == [[0, 1]] * 2 and kept[0, :, -3:].tolist() == [[29, 30, 31]] * 2
+        assert (kept[1] == -1).all() if lens[1] < 0 else kept[1, :, -3:].tolist() == [[13, 14, 15]] * 2
 
 
 def test_tables_that_lead_nowhere():
