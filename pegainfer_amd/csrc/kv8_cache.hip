@@ -282,19 +282,28 @@ __global__ __launch_bounds__(kPickThreads) void kv8_pick_kernel(Kv8 c, const flo
   }
   __syncthreads();
   const int run = (len + kPickThreads - 1) / kPickThreads * 64, from = min(wave * run, len), to = min(from + run, len);
-  auto look = [&](int s, bool& sure, bool& tie) {
-    const bool in = s < to, always = in && (s < lo || s >= hi);
-    const uint32_t w = in && !always && chosen > 0 ? weight(s) : 0u;
-    sure = always || (in && chosen > 0 && w > bits);
-    tie = in && !always && chosen > 0 && w == bits;
+  // four slots a lane at a time, so that their reads do not wait for one another
+  constexpr int U = 4;
+  auto look = [&](int s0, auto&& each) {
+    uint32_t w[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int s = min(s0 + u * 64 + lane, len - 1);
+      w[u] = held ? s_order[s] : chosen > 0 ? fetch(s) : 0u;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int s = s0 + u * 64 + lane;
+      const bool in = s < to, always = in && (s < lo || s >= hi), between = in && !always && chosen > 0;
+      each(s, always || (between && w[u] > bits), between && w[u] == bits);
+    }
   };
   int sures = 0, ties = 0;
-  for (int s = from; s < to; s += 64) {
-    bool sure, tie;
-    look(s + lane, sure, tie);
-    sures += __popcll(__builtin_amdgcn_ballot_w64(sure));
-    ties += __popcll(__builtin_amdgcn_ballot_w64(tie));
-  }
+  for (int s0 = from; s0 < to; s0 += 64 * U)
+    look(s0, [&](int, bool sure, bool tie) {
+      sures += __popcll(__builtin_amdgcn_ballot_w64(sure));
+      ties += __popcll(__builtin_amdgcn_ballot_w64(tie));
+    });
   if (lane == 0) { s_sure[wave] = sures; s_ties[wave] = ties; }
   __syncthreads();
   int at = 0, tied = 0;                    // tokens that stay, and ties met, in the slots before
@@ -304,17 +313,16 @@ __global__ __launch_bounds__(kPickThreads) void kv8_pick_kernel(Kv8 c, const flo
   }
   at += min(tied, left);
   const uint64_t below = (1ull << lane) - 1;
-  for (int s = from; s < to; s += 64) {
-    bool sure, tie;
-    look(s + lane, sure, tie);
-    const uint64_t tie_mask = __builtin_amdgcn_ballot_w64(tie);
-    const bool stays = sure || (tie && tied + __popcll(tie_mask & below) < left);
-    const uint64_t mask = __builtin_amdgcn_ballot_w64(stays);
-    const int to_at = at + __popcll(mask & below);
-    if (stays && to_at < budget) out[to_at] = s + lane;
-    at += __popcll(mask);
-    tied += __popcll(tie_mask);
-  }
+  for (int s0 = from; s0 < to; s0 += 64 * U)
+    look(s0, [&](int s, bool sure, bool tie) {
+      const uint64_t tie_mask = __builtin_amdgcn_ballot_w64(tie);
+      const bool stays = sure || (tie && tied + __popcll(tie_mask & below) < left);
+      const uint64_t mask = __builtin_amdgcn_ballot_w64(stays);
+      const int to_at = at + __popcll(mask & below);
+      if (stays && to_at < budget) out[to_at] = s;
+      at += __popcll(mask);
+      tied += __popcll(tie_mask);
+    });
 }
 
 // The kept tokens into fresh pages: a wave a block's keys, another its values.  A block's exponent is the largest of its tokens', whose codes stay as they are.
