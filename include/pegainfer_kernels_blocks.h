@@ -1084,6 +1084,8 @@ pegainfer_status_t pegainfer_scale_rows(const void* in, int64_t in_stride, void*
  * are left alone.  max_rows: about the most rows of an entry, max_len: about the most slots; they shape the grid, results hold for any (0 rows: no call).
  * At most 65535 entries; storage types as elsewhere: 0 = bf16, 1 = fp32. */
 enum { PEGAINFER_KV8_E4M3 = 0, PEGAINFER_KV8_INT8 = 1 };
+/* keys of as many tokens (max_len) are not cut: without weights the attention then needs no workspace */
+enum { PEGAINFER_KV8_WHOLE = 1024 };
 typedef struct {
   void* codes;
   float* scales;

@@ -879,6 +879,8 @@ __global__ __launch_bounds__(256) void kv8_mass_sum_kernel(AttnArgs a, MassArgs 
   }
 }
 
+constexpr int kWholeBlocks = PEGAINFER_KV8_WHOLE / kKv8Page;
+
 // How a call is cut: rows of a workgroup, splits of the keys and slices of the weights' rows where those leave too few workgroups.
 struct AttnPlan { bool prompt; int tiles, row_tiles, n_split, split_blocks, mass_groups, n_slice, score_rows, round, snake; };
 inline AttnPlan attn_plan(const pegainfer_kv8_cache* cache, int n_rows, int max_rows, int max_len, int heads, int dtype) {
@@ -891,10 +893,11 @@ inline AttnPlan attn_plan(const pegainfer_kv8_cache* cache, int n_rows, int max_
   const int64_t want = 2 * device_cus();
   auto cut = [&](int64_t groups, int64_t most) { return (int)std::max<int64_t>(1, std::min((want + groups - 1) / groups, most)); };
   const int64_t groups = p.tiles * pairs;
-  // Steps: whole over a run of 64 blocks (1024 tokens: 9.8 us; cut, 8.7 with a merge, whose launch costs the host 4), over more into runs of 16 blocks at least.
+  // Whole over a run of 64 blocks (a step over 1024 tokens: 9.8 us; cut, 8.7 with a merge, whose launch costs the host 4).  Steps over more: runs of 16 blocks at least.
   // Prompts: cut where they leave compute units without one (8 entries of 64 rows over 4000 tokens: 52 us in four, 64 in two), into runs of 32 blocks at least; a
   // split of 128 rows leaves 1 KB of sums a value of the head (32 entries of 32 rows over 1000 tokens, a workgroup a compute unit: 34 us whole, 46 halved).
-  p.n_split = !p.prompt ? cut(groups, blocks <= 64 ? 1 : std::min((blocks + 15) / 16, 256))
+  p.n_split = blocks <= kWholeBlocks ? 1
+              : !p.prompt            ? cut(groups, std::min((blocks + 15) / 16, 256))
               : groups >= device_cus() ? 1
                                        : (int)std::max<int64_t>(1, std::min<int64_t>({want / groups, blocks / 32, 256}));
   p.split_blocks = ceil_div(blocks, p.n_split);

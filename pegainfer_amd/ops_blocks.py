@@ -947,6 +947,7 @@ Kv8AttnDesc = _struct("Kv8AttnDesc", [("p", "q"), ("l", "q_row_stride"), ("p", "
                                       ("f", "scale"), ("p", "mass"), ("l", "mass_page_stride"), ("p", "mass_out"), ("l", "mass_out_page_stride"), ("f", "mass_keep"),
                                       ("p", "workspace"), ("i", "dtype")])
 KV8_FORMATS = {torch.float8_e4m3fn: 0, torch.int8: 1}
+KV8_WHOLE = 1024      # PEGAINFER_KV8_WHOLE: over as many tokens no call is cut, so one without weights needs no workspace
 
 
 def _kv8_need(ok, what):
@@ -954,7 +955,7 @@ def _kv8_need(ok, what):
         raise ValueError("kv8: " + what)
 
 
-_I32, _F32 = torch.int32, torch.float32
+_I32, _F32, _current_device, _raw_stream = torch.int32, torch.float32, torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 _KV8_DTYPES, _KV8_BLOCKS = {torch.bfloat16: 0, torch.float32: 1}, (1024, 2048, 4096)
 
 
@@ -967,23 +968,23 @@ def _kv8_index(t, n, device, what):
 
 def _kv8_cache(codes, scales, page_indptr, page_ids, entries):
     """-> (descriptor, kv_heads, dim, device number); refuses what the kernels do not take"""
-    fmt, device, shape, stride, at = KV8_FORMATS.get(codes.dtype), codes.get_device(), codes.shape, codes.stride(), codes.data_ptr()
-    if fmt is None:
-        raise ValueError("kv8: codes of torch.float8_e4m3fn or torch.int8")
-    if device < 0 or device != torch.cuda.current_device():
+    fmt, device = KV8_FORMATS.get(codes.dtype), codes.get_device()
+    if fmt is None or codes.dim() != 4:
+        raise ValueError("kv8: codes [pages, 2, kv_heads, 16 * dim] of torch.float8_e4m3fn or torch.int8")
+    if device < 0 or device != _current_device():
         raise ValueError("kv8: a cache on the current device")
-    if len(shape) != 4:
-        raise ValueError("kv8: codes [pages, 2, kv_heads, 16 * dim]")
-    pages, two, kv, m = shape
+    pages, two, kv, m = codes.shape
     if two != 2 or m not in _KV8_BLOCKS or pages < 1 or not 1 <= kv <= 65535 or entries > 65535:
         raise ValueError("kv8: codes [pages, 2, kv_heads, 16 * dim], a page at least, dim 64, 128 or 256, at most 65535 kv heads and entries")
-    if stride[1:] != (kv * m, m, 1) or stride[0] < 2 * kv * m or (stride[0] | at) % 16:
+    apart, by_side, by_head, one = codes.stride()
+    at = codes.data_ptr()
+    if one != 1 or by_head != m or by_side != kv * m or apart < 2 * kv * m or (apart | at) % 16:
         raise ValueError("kv8: codes: a page's values together, pages apart by a multiple of 16 bytes")
-    sstride = scales.stride()
-    if scales.dtype is not _F32 or scales.get_device() != device or scales.shape != shape[:3] or sstride[1:] != (kv, 1) or sstride[0] < 2 * kv:
+    stride = scales.stride()
+    if scales.dtype is not _F32 or scales.get_device() != device or scales.shape != (pages, 2, kv) or stride[2] != 1 or stride[1] != kv or stride[0] < 2 * kv:
         raise ValueError("kv8: scales fp32 [pages, 2, kv_heads] on the cache's device, a page's together")
-    return Kv8Cache(at, scales.data_ptr(), stride[0], sstride[0], fmt, pages, kv, m // 16, _kv8_index(page_indptr, entries + 1, device, "page_indptr"),
-                    _kv8_index(page_ids, None, device, "page_ids"), page_ids.numel(), entries), kv, m // 16, device
+    return Kv8Cache(at, scales.data_ptr(), apart, stride[0], fmt, pages, kv, m >> 4, _kv8_index(page_indptr, entries + 1, device, "page_indptr"),
+                    _kv8_index(page_ids, None, device, "page_ids"), page_ids.numel(), entries), kv, m >> 4, device
 
 
 def _kv8_rows(x, heads, dim, device, what):
@@ -1023,7 +1024,7 @@ def kv8_append(k, v, codes, scales, row0, starts, page_indptr, page_ids, max_row
     (n, _, k_apart, dtype), (n_v, _, v_apart, dtype_v) = _kv8_rows(k, kv, dim, device, "k"), _kv8_rows(v, kv, dim, device, "v")
     _kv8_need(n == n_v and dtype == dtype_v, "k and v of one shape and type")
     _chk(ffi.lib().pegainfer_kv8_append(ctypes.addressof(cache), k.data_ptr(), v.data_ptr(), k_apart, v_apart, *tables, n, _kv8_most(max_rows, n, entries), dtype,
-                                        _stream()), "kv8_append")
+                                        _raw_stream(device)), "kv8_append")
 
 
 def kv8_read(codes, scales, row0, starts, page_indptr, page_ids, n_rows, dtype=torch.bfloat16, max_rows=None, out=None):
@@ -1042,7 +1043,7 @@ def kv8_read(codes, scales, row0, starts, page_indptr, page_ids, n_rows, dtype=t
             _kv8_need(x.shape == (n_rows, kv, dim) and x.dtype is dtype and x.device == codes.device and x.is_contiguous() and x.data_ptr() % 16 == 0,
                       "out: two contiguous tensors [n_rows, kv_heads, dim] of dtype")
     _chk(ffi.lib().pegainfer_kv8_read(ctypes.addressof(cache), *tables, k.data_ptr(), v.data_ptr(), int(n_rows),
-                                      _kv8_most(max_rows, n_rows, entries), _KV8_DTYPES[dtype], _stream()), "kv8_read")
+                                      _kv8_most(max_rows, n_rows, entries), _KV8_DTYPES[dtype], _raw_stream(device)), "kv8_read")
     return k, v
 
 
@@ -1069,11 +1070,12 @@ def kv8_attention(q, codes, scales, row0, starts, page_indptr, page_ids, scale, 
         if mass is not None:
             d.mass, d.mass_page_stride = mass.data_ptr(), _kv8_mass(mass, codes, "mass")
         d.mass_out, d.mass_out_page_stride, d.mass_keep = mass_out.data_ptr(), _kv8_mass(mass_out, codes, "mass_out"), float(mass_keep)
-    n = ffi.lib().pegainfer_kv8_attention_workspace(ctypes.addressof(cache), T, max_rows, max_len, H, dtype, mass_out is not None)
-    if n > 0:
-        ws = torch.empty(n, dtype=torch.float32, device=q.device)
-        d.workspace = ws.data_ptr()
-    _chk(ffi.lib().pegainfer_kv8_attention(ctypes.addressof(cache), ctypes.addressof(d), _stream()), "kv8_attention")
+    if mass_out is not None or max_len > KV8_WHOLE:
+        n = ffi.lib().pegainfer_kv8_attention_workspace(ctypes.addressof(cache), T, max_rows, max_len, H, dtype, mass_out is not None)
+        if n > 0:
+            ws = torch.empty(n, dtype=torch.float32, device=q.device)
+            d.workspace = ws.data_ptr()
+    _chk(ffi.lib().pegainfer_kv8_attention(ctypes.addressof(cache), ctypes.addressof(d), _raw_stream(device)), "kv8_attention")
     return out
 
 
@@ -1088,5 +1090,5 @@ def kv8_evict(codes, scales, mass, lens, page_indptr, page_ids, dst_indptr, dst_
     kept = torch.empty((entries, kv, budget), dtype=torch.int32, device=codes.device)
     _chk(ffi.lib().pegainfer_kv8_evict(ctypes.addressof(cache), mass.data_ptr(), stride, *tables, dst_ids.numel(),
                                        int(budget), int(keep_first), int(keep_last), _kv8_most(max_len, page_ids.numel() * 32, entries), kept.data_ptr(),
-                                       _stream()), "kv8_evict")
+                                       _raw_stream(device)), "kv8_evict")
     return kept

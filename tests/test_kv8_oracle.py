@@ -83,3 +83,20 @@ def test_wrappers_refuse_what_is_not_on_the_device():
     for dt in (torch.uint8, torch.int8):
         with pytest.raises(ValueError, match="kv8"):
             B.kv8_append(torch.zeros(1, 2, 64), torch.zeros(1, 2, 64), torch.zeros(3, 2, 2, 1024, dtype=dt), torch.zeros(3, 2, 2), i, i[:1], i, i)
+
+
+def test_what_is_not_cut_needs_no_workspace(built_libs):
+    """the wrapper asks for the size of a workspace only beyond KV8_WHOLE tokens"""
+    L, ref = ffi.lib(), ctypes.addressof
+    text = open(ffi.INCLUDE + "/pegainfer_kernels_blocks.h").read()
+    assert "PEGAINFER_KV8_WHOLE = %d " % B.KV8_WHOLE in text
+    for kv, dim in [(1, 64), (8, 128), (2, 256)]:
+        for entries in (1, 3, 400):
+            c = _cache(kv_heads=kv, dim=dim, code_page_stride=2 * kv * 16 * dim, scale_page_stride=2 * kv, n_entries=entries, n_page_ids=5)
+            for rows in (1, 5, 40, 1000, 100000):
+                for dtype in (0, 1):
+                    assert L.pegainfer_kv8_attention_workspace(ref(c), rows, rows, B.KV8_WHOLE, 4 * kv, dtype, 0) == 0
+                    assert L.pegainfer_kv8_attention_workspace(ref(c), rows, rows, B.KV8_WHOLE, 4 * kv, dtype, 1) >= rows * 4 * kv
+    # a long cache is cut where that fills the chip: one entry's is, that of 400 entries of 2 heads is not
+    assert L.pegainfer_kv8_attention_workspace(ref(c), 1, 1, 10 ** 6, 2, 0, 0) == 0
+    assert L.pegainfer_kv8_attention_workspace(ref(_cache()), 1, 1, 10 ** 6, 2, 0, 0) > 0
