@@ -178,6 +178,43 @@ def test_a_row_that_is_not_a_number_spoils_itself_alone(rows):
     assert torch.equal(got[~spoiled], want[~spoiled]) and torch.isnan(got[0, 1]).all()
 
 
+# A key that comes late and takes nearly all of a row gives its values: its own weight may not be rounded, so that what is left is the output's rounding, 2^-8 of it,
+# the others' weights, 2^-8 each of their small share, and the fp32 terms: scores below 48 off by (dim + 4) 2^-24 each and sums over 1024 tokens.
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("rows", [1, 16, 96])
+def test_a_late_key_with_nearly_all_of_a_row(fmt, rows):
+    n, dim, heads = 1024, 64, 4
+    rng = np.random.RandomState(31)
+    k, v = torch.zeros(n, 1, dim), torch.from_numpy(rng.randn(n, 1, dim).astype(np.float32))
+    k[:, 0, 1] = -1.0                                                    # far below, but for one token in 32 of the first 256, at zero, ...
+    k[0:256:32, 0, 1] = 0.0
+    late = 600                                                           # ... and one above them, behind every wave's first tokens
+    k[late, 0, 0], k[late, 0, 1] = 1.0, 0.0
+    c = Cache([0], [n], 1, dim, fmt, seed=31)
+    d = c.device()
+    codes, scales = c.codes.copy(), c.scales.copy()
+    R.append(k.numpy(), v.numpy(), codes, scales, fmt, c.row0, c.starts, c.tables)
+    B.kv8_append(k.cuda(), v.cuda(), d.codes, d.scales, d.row0, d.starts, d.indptr, d.ids)
+    same(d, c, codes, scales)
+    kk, vv = (x[:, 0] for x in R.read(codes, scales, fmt, dim, c.row0, c.starts, c.tables))
+    q = torch.from_numpy(rng.randn(rows, heads, dim).astype(np.float32))
+    q[..., 0] = torch.linspace(3.6, 5.4, rows * heads).view(rows, heads)    # factors of e^3.6 to e^5.4: 36 to 222 times the others at zero
+    q[..., 1] = 40.0
+    q = q.bfloat16()
+    at = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")    # noqa: E731
+    got = B.kv8_attention(q.cuda(), d.codes, d.scales, at(0, rows), at(n - rows), d.indptr, d.ids, 1.0).double().cpu().numpy()
+    z = q.double().numpy() @ kk.T
+    for i in range(rows):
+        z[i, :, n - rows + i + 1:] = -np.inf
+    p = np.exp(z - z.max(-1, keepdims=True))
+    p /= p.sum(-1, keepdims=True)
+    want, most = p @ vv, p[..., late, None] * np.abs(vv[late])
+    small = 2 * (2 * (dim + 4) * 48 + n + 16) * 2.0 ** -24
+    bound = 2.0 ** -8 * np.abs(want) + (1 + 2.0 ** -8) * (2.0 ** -8 * (p @ np.abs(vv) - most) * 2 + small * (p @ np.abs(vv)))
+    off = np.abs(got - want)
+    assert (off <= bound).all(), ((off / bound).max(), np.argwhere(off > bound)[:5])
+
+
 @pytest.mark.parametrize("entries,kv,group", [(300, 1, 1), (3, 9, 1), (2, 1, 64), (1, 40, 2)])
 def test_attention_of_many_entries_and_heads(entries, kv, group):
     rng = np.random.RandomState(entries)
