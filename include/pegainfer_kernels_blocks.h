@@ -1082,7 +1082,7 @@ pegainfer_status_t pegainfer_scale_rows(const void* in, int64_t in_stride, void*
  * replays of a captured graph.  A slot without a page in [0, n_pages) is not there: never written, never seen, read as 0;
  * no entry has more slots than its part of page_ids.  Rows behind row0[n_entries]
  * are left alone.  max_rows: about the most rows of an entry, max_len: about the most slots; they shape the grid, results hold for any (0 rows: no call).
- * At most 65535 entries; storage types as elsewhere: 0 = bf16, 1 = fp32. */
+ * At most 65535 entries and 2^26 page ids; storage types as elsewhere: 0 = bf16, 1 = fp32. */
 enum { PEGAINFER_KV8_E4M3 = 0, PEGAINFER_KV8_INT8 = 1 };
 /* keys of as many tokens (max_len) are not cut: without weights the attention then needs no workspace */
 enum { PEGAINFER_KV8_WHOLE = 1024 };
@@ -1109,7 +1109,8 @@ pegainfer_status_t pegainfer_kv8_read(const pegainfer_kv8_cache* cache, const in
  * queries and weights enter as three bf16 parts, nothing is rounded.  Entries may share pages (a common prompt).  out is not q.
  * mass_out given: mass_out[page][kv head][16] (fp32, pages mass_out_page_stride values apart) = mass_keep * mass + the weight that the call's rows and the kv
  * head's query heads gave to the token, for every slot of an entry that has rows (mass_out may be mass; mass_keep 0: mass is not read and may be NULL).  Every
- * sum has one order: results do not change from run to run.  A page that two entries of such a call shared would be written by both: it is a page of one.
+ * sum has one order: results do not change from run to run.  Entries of such a call must not share a page (both would write its weights): those of a common prompt
+ * go in calls of their own, one after the other.
  * workspace: fp32 scratch on 16 bytes of pegainfer_kv8_attention_workspace(...) values, of this call alone until it is done (0: NULL). */
 typedef struct {
   const void* q;

@@ -73,7 +73,7 @@ __global__ __launch_bounds__(128) void kv8_append_kernel(Kv8 c, const T* k, cons
   const T* base = (side == 0 ? k : v) + head * D;
   const int64_t stride = side == 0 ? k_stride : v_stride;
   const int end = (int)start + rows.n;
-  for (int b = (int)start / kKv8Page + blockIdx.x; b * kKv8Page < end; b += gridDim.x) {
+  for (int b = (int)start / kKv8Page + blockIdx.x, past = (end + kKv8Page - 1) / kKv8Page; b < past; b += gridDim.x) {   // in blocks: slots pass 2^31 a grid behind the last
     const int page = c.page(e, b);
     if (page < 0) continue;
     const int low = b * kKv8Page, first = max((int)start - low, 0);   // tokens 0 .. first - 1 of the block were there before
@@ -125,7 +125,7 @@ __global__ __launch_bounds__(128) void kv8_read_kernel(Kv8 c, T* k, T* v, const 
   const int64_t stride = (int64_t)c.kv_heads * D;
   T* base = (side == 0 ? k : v) + head * D;
   const int end = (int)start + rows.n;
-  for (int b = (int)start / kKv8Page + blockIdx.x; b * kKv8Page < end; b += gridDim.x) {
+  for (int b = (int)start / kKv8Page + blockIdx.x, past = (end + kKv8Page - 1) / kKv8Page; b < past; b += gridDim.x) {   // in blocks: slots pass 2^31 a grid behind the last
     const int page = c.page(e, b), low = b * kKv8Page;
     const float scale = page < 0 ? 0.f : *c.scale(page, side, head);
     const uint8_t* blk = page < 0 ? nullptr : c.block(page, side, head, D);
@@ -336,7 +336,7 @@ __global__ __launch_bounds__(128) void kv8_move_kernel(Kv8 c, const int32_t* dst
   to.indptr = dst_indptr;
   to.ids = dst_ids;
   to.n_ids = n_dst_ids;
-  for (int b = blockIdx.x; b * kKv8Page < len; b += gridDim.x) {
+  for (int b = blockIdx.x; b < (len + kKv8Page - 1) / kKv8Page; b += gridDim.x) {
     const int dst = to.page(e, b);
     if (dst < 0) continue;
     // lane n of every sixteen: where token n comes from

@@ -10,9 +10,12 @@
 
 namespace pk {
 
+// of an entry at most 2^30 slots, so that slots and a grid's steps over them stay within 32 bits
+constexpr int kKv8MostIds = 1 << 26;
+
 inline bool kv8_ok(const pegainfer_kv8_cache* c) {
   return c && (c->format == kE4m3 || c->format == kInt8) && (c->dim == 64 || c->dim == 128 || c->dim == 256) && c->kv_heads >= 1 && c->kv_heads <= 65535 &&
-         c->n_entries >= 0 && c->n_entries <= 65535 && c->n_pages >= 1 && c->n_page_ids >= 0 &&
+         c->n_entries >= 0 && c->n_entries <= 65535 && c->n_pages >= 1 && c->n_page_ids >= 0 && c->n_page_ids <= kKv8MostIds &&
          (c->n_entries == 0 || (c->codes && c->scales && c->page_indptr && (c->page_ids || c->n_page_ids == 0) && host_aligned16(c->codes) &&
                                 c->code_page_stride % 16 == 0 && c->code_page_stride >= (int64_t)2 * c->kv_heads * kKv8Page * c->dim &&
                                 c->scale_page_stride >= (int64_t)2 * c->kv_heads));

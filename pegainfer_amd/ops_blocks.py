@@ -1012,7 +1012,7 @@ def _kv8_mass(mass, codes, what):
 
 def _kv8_most(given, total, entries):
     """a hint of the most of an entry: as given, or the average"""
-    return int(given) if given is not None else -(-total // max(entries, 1))
+    return min(int(given) if given is not None else -(-total // max(entries, 1)), 2 ** 31 - 1)
 
 
 def kv8_append(k, v, codes, scales, row0, starts, page_indptr, page_ids, max_rows=None):
@@ -1049,8 +1049,9 @@ def kv8_read(codes, scales, row0, starts, page_indptr, page_ids, n_rows, dtype=t
 
 def kv8_attention(q, codes, scales, row0, starts, page_indptr, page_ids, scale, max_rows=None, max_len=None, out=None, mass=None, mass_out=None, mass_keep=1.0):
     """-> out [rows, heads, dim]: causal attention of q's rows (their own tokens are in the cache already).  max_rows / max_len: about the most rows / tokens of an
-    entry (None: the average of the rows, twice that of the pages); they choose how the call is cut, results are right for any.  mass fp32 [pages, kv_heads, 16]: mass_out (None: mass itself) becomes mass_keep * mass + the weight that every token got;
-    mass_out alone with mass_keep 0: the weight of this call."""
+    entry (None: the average of the rows, twice that of the pages); they choose how the call is cut, results are right for any.  mass fp32 [pages, kv_heads, 16]:
+    mass_out (None: mass itself) becomes mass_keep * mass + the weight that every token got; mass_out alone with mass_keep 0: the weight of this call.  Entries may
+    share pages, but not where a call writes weights."""
     entries = row0.numel() - 1
     cache, kv, dim, device = _kv8_cache(codes, scales, page_indptr, page_ids, entries)
     row0_at, starts_at = _kv8_index(row0, entries + 1, device, "row0"), _kv8_index(starts, entries, device, "starts")

@@ -265,6 +265,24 @@ def test_lengths_and_starts_of_any_size_end():
         assert (kept[1] == -1).all() if lens[1] < 0 else kept[1, :, -3:].tolist() == [[13, 14, 15]] * 2
 
 
+def test_rows_in_and_out_at_the_last_slots_of_32_bits():
+    """starts that have no page, and a grid that reaches past 2^31 behind them: the walks end, nothing is written, what is read is 0"""
+    c = Cache([0, 0], [16, 7984], 1, 64, "int8", seed=34)
+    d = c.device()
+    rows = torch.randn(8000, 1, 64, device="cuda").bfloat16()
+    pool, scales = d.pool.clone(), d.scales.clone()
+    for start in (2 ** 31 - 1 - 32 - 7984, 2 ** 31 - 40000, 2 ** 30):
+        at = torch.tensor([start, start], dtype=torch.int32, device="cuda")
+        for most in (None, 1, 8000, 2 ** 40):
+            B.kv8_append(rows, rows, d.codes, d.scales, d.row0, at, d.indptr, d.ids, max_rows=most)
+            k, v = B.kv8_read(d.codes, d.scales, d.row0, at, d.indptr, d.ids, 8000, max_rows=most)
+            assert (k == 0).all() and (v == 0).all()
+    assert torch.equal(d.pool, pool) and torch.equal(d.scales.nan_to_num(7), scales.nan_to_num(7))
+    many = torch.empty(2 ** 26 + 1, dtype=torch.int32, device="cuda")
+    with pytest.raises(RuntimeError):
+        B.kv8_append(rows, rows, d.codes, d.scales, d.row0, d.starts, d.indptr, many)
+
+
 def test_tables_that_lead_nowhere():
     """pages out of range, tables that end early, rows out of range, entries that start nowhere: not there, and nothing else is touched"""
     c = Cache([20, 40, 5, 33, 70], [4, 1, 1, 2, 1], 2, 64, "int8", seed=8)
