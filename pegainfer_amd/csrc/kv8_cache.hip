@@ -187,7 +187,7 @@ __device__ __forceinline__ uint32_t order_of(float m) {
 // Which tokens stay: one workgroup an (entry, head).  Three histograms over 11, 11 and 10 bits of the weights' order give the lightest weight that stays among those
 // between the first and the last tokens; then every wave counts, and after a barrier writes, the slots that stay of a run of its own, in order: of equal weights the
 // lowest slots.  Bound by the latency of few workgroups, so the weights are fetched once, through their pages, and kept in shared memory where they fit
-// (36 864 tokens; beyond that every pass fetches them).  11 bits reach into the mantissa: weights share few exponents, and counts of one address are taken in turn.
+// (36 864 tokens; of those beyond, every pass fetches them, sixteen a thread on their way).  11 bits reach into the mantissa: weights share few exponents, and counts of one address are taken in turn.
 constexpr int kPickThreads = 1024, kPickWaves = kPickThreads / 64, kPickCached = 36864;
 __global__ __launch_bounds__(kPickThreads) void kv8_pick_kernel(Kv8 c, const float* mass, int64_t mass_stride, const int32_t* lens, int budget, int keep_first,
                                                                 int keep_last, int cached, int32_t* kept) {
@@ -203,43 +203,39 @@ __global__ __launch_bounds__(kPickThreads) void kv8_pick_kernel(Kv8 c, const flo
     for (int i = tid; i < budget; i += kPickThreads) out[i] = i < len ? i : -1;
     return;
   }
-  auto fetch = [&](int s) {
-    const int page = c.page(e, s / kKv8Page);
-    return page < 0 ? 0u : order_of(mass[page * mass_stride + head * kKv8Page + s % kKv8Page]);
+  // the weights of N slots, page ids and weights each in one go: what is not there is read from the table's and the cache's first place and left out
+  const int first = c.indptr[e], pages = c.indptr[e + 1] - first;
+  auto fetch = [&](auto slot, auto& w) {
+    constexpr int N = sizeof(w) / sizeof(w[0]);
+    int page[N];
+    float m[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int block = slot(i) / kKv8Page, at = first + block;
+      const bool there = block < pages && (unsigned)at < (unsigned)c.n_ids;
+      const int id = c.ids[there ? at : 0];
+      page[i] = there && (unsigned)id < (unsigned)c.n_pages ? id : -1;
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) m[i] = mass[max(page[i], 0) * mass_stride + head * kKv8Page + slot(i) % kKv8Page];
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[i] = page[i] < 0 ? 0u : order_of(m[i]);
   };
-  const bool held = len <= cached;
+  const int held = min(len, cached);       // slots whose weights are in shared memory; the others' are fetched again
   const int lo = keep_first, hi = len - keep_last, chosen = budget - keep_first - keep_last;
   for (int i = tid; i < 2048; i += kPickThreads) hist[i] = 0;
   __syncthreads();
-  if (held && c.n_ids > 0) {
-    // sixteen slots a thread at a time, page ids and weights each in one go: what is not there is read from the table's and the cache's first place and left out
-    const int first = c.indptr[e], pages = c.indptr[e + 1] - first;
-    constexpr int N = 16;
-    for (int s0 = tid; s0 < len; s0 += N * kPickThreads) {
-      int page[N];
-      float m[N];
+  constexpr int N = 16;                    // slots a thread at a time
+  for (int s0 = tid; s0 < len; s0 += N * kPickThreads) {
+    uint32_t w[N];
+    fetch([&](int i) { return s0 + i * kPickThreads; }, w);
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const int block = (s0 + i * kPickThreads) / kKv8Page, at = first + block;
-        const bool there = block < pages && (unsigned)at < (unsigned)c.n_ids;
-        const int id = c.ids[there ? at : 0];
-        page[i] = there && (unsigned)id < (unsigned)c.n_pages ? id : -1;
-      }
-#pragma unroll
-      for (int i = 0; i < N; ++i) m[i] = mass[max(page[i], 0) * mass_stride + head * kKv8Page + (s0 + i * kPickThreads) % kKv8Page];
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const int s = s0 + i * kPickThreads;
-        const uint32_t w = page[i] < 0 ? 0u : order_of(m[i]);
-        if (s < len) s_order[s] = w;
-        if (s >= lo && s < hi) atomicAdd(&hist[w >> 21], 1u);
-      }
+    for (int i = 0; i < N; ++i) {
+      const int s = s0 + i * kPickThreads;
+      if (s < held) s_order[s] = w[i];
+      if (s >= lo && s < hi) atomicAdd(&hist[w[i] >> 21], 1u);
     }
-  } else if (held) {
-    for (int s = tid; s < len; s += kPickThreads) s_order[s] = 0;
-    if (tid == 0 && hi > lo) hist[0] = hi - lo;
   }
-  auto weight = [&](int s) { return held ? s_order[s] : fetch(s); };
   uint32_t bits = 0;                       // of the lightest weight that stays: its upper bits so far
   int left = chosen;                       // tokens still to be found that have those
   if (chosen > 0) {
@@ -250,11 +246,18 @@ __global__ __launch_bounds__(kPickThreads) void kv8_pick_kernel(Kv8 c, const flo
         __syncthreads();
       }
       const uint32_t mask = done == 0 ? 0u : 0xFFFFFFFFu << (32 - done);
-      if (done > 0 || !held) {             // the first is counted as the weights arrive
+      auto count = [&](uint32_t w) {
+        if ((w & mask) == bits) atomicAdd(&hist[(w >> shift) & 2047 >> (11 - width)], 1u);
+      };
+      if (done > 0) {                      // the first is counted as the weights arrive
 #pragma unroll 4
-        for (int s = lo + tid; s < hi; s += kPickThreads) {
-          const uint32_t w = weight(s);
-          if ((w & mask) == bits) atomicAdd(&hist[(w >> shift) & 2047 >> (11 - width)], 1u);
+        for (int s = lo + tid; s < min(hi, held); s += kPickThreads) count(s_order[s]);
+        for (int s0 = max(lo, held) + tid; s0 < hi; s0 += N * kPickThreads) {
+          uint32_t w[N];
+          fetch([&](int i) { return s0 + i * kPickThreads; }, w);
+#pragma unroll
+          for (int i = 0; i < N; ++i)
+            if (s0 + i * kPickThreads < hi) count(w[i]);
         }
       }
       __syncthreads();
@@ -282,15 +285,9 @@ __global__ __launch_bounds__(kPickThreads) void kv8_pick_kernel(Kv8 c, const flo
   }
   __syncthreads();
   const int run = (len + kPickThreads - 1) / kPickThreads * 64, from = min(wave * run, len), to = min(from + run, len);
-  // four slots a lane at a time, so that their reads do not wait for one another
-  constexpr int U = 4;
-  auto look = [&](int s0, auto&& each) {
-    uint32_t w[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int s = min(s0 + u * 64 + lane, len - 1);
-      w[u] = held ? s_order[s] : chosen > 0 ? fetch(s) : 0u;
-    }
+  // several slots a lane at a time, so that their reads do not wait for one another: four of shared memory, sixteen through the pages
+  auto look = [&](int s0, const auto& w, auto&& each) {
+    constexpr int U = sizeof(w) / sizeof(w[0]);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int s = s0 + u * 64 + lane;
@@ -298,12 +295,27 @@ __global__ __launch_bounds__(kPickThreads) void kv8_pick_kernel(Kv8 c, const flo
       each(s, always || (between && w[u] > bits), between && w[u] == bits);
     }
   };
+  auto walk = [&](auto&& each) {
+    constexpr int U = 4;
+    int s0 = from;
+    for (; s0 < min(to, held); s0 += 64 * U) {
+      if (s0 + 64 * U > held && held < len) break;
+      uint32_t w[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) w[u] = s_order[min(s0 + u * 64 + lane, len - 1)];
+      look(s0, w, each);
+    }
+    for (; s0 < to; s0 += 64 * N) {
+      uint32_t w[N];
+      fetch([&](int u) { return s0 + u * 64 + lane; }, w);
+      look(s0, w, each);
+    }
+  };
   int sures = 0, ties = 0;
-  for (int s0 = from; s0 < to; s0 += 64 * U)
-    look(s0, [&](int, bool sure, bool tie) {
-      sures += __popcll(__builtin_amdgcn_ballot_w64(sure));
-      ties += __popcll(__builtin_amdgcn_ballot_w64(tie));
-    });
+  walk([&](int, bool sure, bool tie) {
+    sures += __popcll(__builtin_amdgcn_ballot_w64(sure));
+    ties += __popcll(__builtin_amdgcn_ballot_w64(tie));
+  });
   if (lane == 0) { s_sure[wave] = sures; s_ties[wave] = ties; }
   __syncthreads();
   int at = 0, tied = 0;                    // tokens that stay, and ties met, in the slots before
@@ -313,16 +325,15 @@ __global__ __launch_bounds__(kPickThreads) void kv8_pick_kernel(Kv8 c, const flo
   }
   at += min(tied, left);
   const uint64_t below = (1ull << lane) - 1;
-  for (int s0 = from; s0 < to; s0 += 64 * U)
-    look(s0, [&](int s, bool sure, bool tie) {
-      const uint64_t tie_mask = __builtin_amdgcn_ballot_w64(tie);
-      const bool stays = sure || (tie && tied + __popcll(tie_mask & below) < left);
-      const uint64_t mask = __builtin_amdgcn_ballot_w64(stays);
-      const int to_at = at + __popcll(mask & below);
-      if (stays && to_at < budget) out[to_at] = s;
-      at += __popcll(mask);
-      tied += __popcll(tie_mask);
-    });
+  walk([&](int s, bool sure, bool tie) {
+    const uint64_t tie_mask = __builtin_amdgcn_ballot_w64(tie);
+    const bool stays = sure || (tie && tied + __popcll(tie_mask & below) < left);
+    const uint64_t mask = __builtin_amdgcn_ballot_w64(stays);
+    const int to_at = at + __popcll(mask & below);
+    if (stays && to_at < budget) out[to_at] = s;
+    at += __popcll(mask);
+    tied += __popcll(tie_mask);
+  });
 }
 
 // The kept tokens into fresh pages: a wave a block's keys, another its values.  A block's exponent is the largest of its tokens', whose codes stay as they are.

@@ -372,6 +372,24 @@ def test_evict_of_many_tokens_and_of_shared_pages():
     run_evict(c, lens, 1029, 4, 100, dst_extra=1)
 
 
+@pytest.mark.parametrize("first,last", [(0, 0), (4, 100), (700, 329)])
+def test_evict_whatever_the_hint(first, last):
+    """the weights of the first max_len tokens are kept at hand, the others' looked up again: ends of that part inside and at the ends of every wave's run"""
+    lens = [2500, 1030, 40000]
+    c = Cache(lens, [0] * 3, 1, 64, "int8", seed=3, dirty=False)
+    d, got = c.device(), []
+    dst = torch.zeros(4, dtype=torch.int32, device="cuda")               # no pages to move to: the slots that stay are what is looked at
+    order = [c.mass[[c.ids[i] for i in range(c.indptr[e], c.indptr[e + 1])], 0].reshape(-1)[:n] for e, n in enumerate(lens)]
+    for most in (None, 0, 1, 63, 64, 256, 1000, 1024, 2047, 2304, 2499, 2500, 20000, 36865, 10 ** 6):
+        kept = B.kv8_evict(d.codes, d.scales, d.mass, d.lens, d.indptr, d.ids, dst, dst[:0], 1029, first, last, max_len=most)
+        got.append(kept.cpu().numpy()[:, 0])
+    for e, n in enumerate(lens):
+        between = np.argsort(-order[e][first:n - last], kind="stable")[:1029 - first - last] + first
+        want = np.sort(np.concatenate([np.arange(first), between, np.arange(n - last, n)]))
+        for g in got:
+            assert np.array_equal(g[e], want), (e, np.argwhere(g[e] != want)[:4])
+
+
 def test_evict_with_pages_that_are_not_there():
     lens = [100, 90]
     c = Cache(lens, [0] * 2, 2, 64, "e4m3", seed=2, pages=60, dirty=False)
