@@ -187,11 +187,11 @@ __device__ __forceinline__ uint32_t order_of(float m) {
 // Which tokens stay: one workgroup an (entry, head).  Three histograms over 11, 11 and 10 bits of the weights' order give the lightest weight that stays among those
 // between the first and the last tokens; then every wave counts, and after a barrier writes, the slots that stay of a run of its own, in order: of equal weights the
 // lowest slots.  Bound by the latency of few workgroups, so the weights are fetched once, through their pages, and kept in shared memory where they fit
-// (36 864 tokens; of those beyond, every pass fetches them, sixteen a thread on their way).  11 bits reach into the mantissa: weights share few exponents, and counts of one address are taken in turn.
+// (36 864 tokens; of those beyond, every pass fetches them again).  11 bits reach into the mantissa: weights share few exponents, and counts of one address are taken in turn.
 constexpr int kPickThreads = 1024, kPickWaves = kPickThreads / 64, kPickCached = 36864;
 __global__ __launch_bounds__(kPickThreads) void kv8_pick_kernel(Kv8 c, const float* mass, int64_t mass_stride, const int32_t* lens, int budget, int keep_first,
                                                                 int keep_last, int cached, int32_t* kept) {
-  extern __shared__ uint32_t s_order[];
+  extern __shared__ u32x4 s_order[];
   __shared__ uint32_t hist[2048];
   __shared__ int s_sure[kPickWaves], s_ties[kPickWaves], s_sum[kPickWaves];
   __shared__ uint32_t s_bits;
@@ -203,12 +203,13 @@ __global__ __launch_bounds__(kPickThreads) void kv8_pick_kernel(Kv8 c, const flo
     for (int i = tid; i < budget; i += kPickThreads) out[i] = i < len ? i : -1;
     return;
   }
-  // the weights of N slots, page ids and weights each in one go: what is not there is read from the table's and the cache's first place and left out
+  // the weights of N fours of slots (from multiples of 4: of one page), page ids and weights each in one go: what is not there is read from the table's and the
+  // cache's first place and left out
   const int first = c.indptr[e], pages = c.indptr[e + 1] - first;
-  auto fetch = [&](auto slot, auto& w) {
-    constexpr int N = sizeof(w) / sizeof(w[0]);
+  constexpr int N = 4;
+  auto fetch = [&](auto slot, u32x4 (&w)[N]) {
     int page[N];
-    float m[N];
+    f32x4 m[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int block = slot(i) / kKv8Page, at = first + block;
@@ -217,23 +218,27 @@ __global__ __launch_bounds__(kPickThreads) void kv8_pick_kernel(Kv8 c, const flo
       page[i] = there && (unsigned)id < (unsigned)c.n_pages ? id : -1;
     }
 #pragma unroll
-    for (int i = 0; i < N; ++i) m[i] = mass[max(page[i], 0) * mass_stride + head * kKv8Page + slot(i) % kKv8Page];
+    for (int i = 0; i < N; ++i) __builtin_memcpy(&m[i], mass + max(page[i], 0) * mass_stride + head * kKv8Page + slot(i) % kKv8Page, 16);   // on 4 bytes
 #pragma unroll
-    for (int i = 0; i < N; ++i) w[i] = page[i] < 0 ? 0u : order_of(m[i]);
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[i][j] = page[i] < 0 ? 0u : order_of(m[i][j]);
   };
-  const int held = min(len, cached);       // slots whose weights are in shared memory; the others' are fetched again
+  const int held = min(len, cached);       // slots whose weights are in shared memory (a multiple of 4, or all); the others' are fetched again
   const int lo = keep_first, hi = len - keep_last, chosen = budget - keep_first - keep_last;
   for (int i = tid; i < 2048; i += kPickThreads) hist[i] = 0;
   __syncthreads();
-  constexpr int N = 16;                    // slots a thread at a time
-  for (int s0 = tid; s0 < len; s0 += N * kPickThreads) {
-    uint32_t w[N];
-    fetch([&](int i) { return s0 + i * kPickThreads; }, w);
+  constexpr int kStep = 4 * kPickThreads;
+  for (int s0 = 4 * tid; s0 < len; s0 += N * kStep) {
+    u32x4 w[N];
+    fetch([&](int i) { return s0 + i * kStep; }, w);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int s = s0 + i * kPickThreads;
-      if (s < held) s_order[s] = w[i];
-      if (s >= lo && s < hi) atomicAdd(&hist[w[i] >> 21], 1u);
+      const int s = s0 + i * kStep;
+      if (s < held) s_order[s / 4] = w[i];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (s + j >= lo && s + j < hi) atomicAdd(&hist[w[i][j] >> 21], 1u);
     }
   }
   uint32_t bits = 0;                       // of the lightest weight that stays: its upper bits so far
@@ -246,18 +251,19 @@ __global__ __launch_bounds__(kPickThreads) void kv8_pick_kernel(Kv8 c, const flo
         __syncthreads();
       }
       const uint32_t mask = done == 0 ? 0u : 0xFFFFFFFFu << (32 - done);
-      auto count = [&](uint32_t w) {
-        if ((w & mask) == bits) atomicAdd(&hist[(w >> shift) & 2047 >> (11 - width)], 1u);
-      };
       if (done > 0) {                      // the first is counted as the weights arrive
-#pragma unroll 4
-        for (int s = lo + tid; s < min(hi, held); s += kPickThreads) count(s_order[s]);
-        for (int s0 = max(lo, held) + tid; s0 < hi; s0 += N * kPickThreads) {
-          uint32_t w[N];
-          fetch([&](int i) { return s0 + i * kPickThreads; }, w);
+        auto count = [&](int s, const u32x4& w) {
 #pragma unroll
-          for (int i = 0; i < N; ++i)
-            if (s0 + i * kPickThreads < hi) count(w[i]);
+          for (int j = 0; j < 4; ++j)
+            if (s + j >= lo && s + j < hi && (w[j] & mask) == bits) atomicAdd(&hist[(w[j] >> shift) & 2047 >> (11 - width)], 1u);
+        };
+#pragma unroll 2
+        for (int s = lo / 4 * 4 + 4 * tid; s < min(hi, held); s += kStep) count(s, s_order[s / 4]);
+        for (int s0 = max(lo / 4 * 4, held) + 4 * tid; held < len && s0 < hi; s0 += N * kStep) {
+          u32x4 w[N];
+          fetch([&](int i) { return s0 + i * kStep; }, w);
+#pragma unroll
+          for (int i = 0; i < N; ++i) count(s0 + i * kStep, w[i]);
         }
       }
       __syncthreads();
@@ -284,37 +290,42 @@ __global__ __launch_bounds__(kPickThreads) void kv8_pick_kernel(Kv8 c, const flo
     }
   }
   __syncthreads();
-  const int run = (len + kPickThreads - 1) / kPickThreads * 64, from = min(wave * run, len), to = min(from + run, len);
-  // several slots a lane at a time, so that their reads do not wait for one another: four of shared memory, sixteen through the pages
-  auto look = [&](int s0, const auto& w, auto&& each) {
-    constexpr int U = sizeof(w) / sizeof(w[0]);
+  const int run = (len + kStep - 1) / kStep * 256, from = min(wave * run, len), to = min(from + run, len);
+  // four slots a lane, so that a wave's lanes and their slots are in order; two of shared memory at a time, or N through the pages
+  auto look = [&](int s, const u32x4& w, auto&& each) {
+    bool sure[4], tie[4];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int s = s0 + u * 64 + lane;
-      const bool in = s < to, always = in && (s < lo || s >= hi), between = in && !always && chosen > 0;
-      each(s, always || (between && w[u] > bits), between && w[u] == bits);
+    for (int j = 0; j < 4; ++j) {
+      const bool in = s + j < to, always = in && (s + j < lo || s + j >= hi), between = in && !always && chosen > 0;
+      sure[j] = always || (between && w[j] > bits);
+      tie[j] = between && w[j] == bits;
     }
+    each(s, sure, tie);
   };
   auto walk = [&](auto&& each) {
-    constexpr int U = 4;
-    int s0 = from;
-    for (; s0 < min(to, held); s0 += 64 * U) {
-      if (s0 + 64 * U > held && held < len) break;
-      uint32_t w[U];
+    constexpr int U = 2;
+    int s0 = from + 4 * lane;
+    for (int at = from; at < min(to, held) && (held == len || at + 256 * U <= held); at += 256 * U, s0 += 256 * U) {
+      u32x4 w[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) w[u] = s_order[min(s0 + u * 64 + lane, len - 1)];
-      look(s0, w, each);
+      for (int u = 0; u < U; ++u) w[u] = s_order[min(s0 + u * 256, held - 1) / 4];
+#pragma unroll
+      for (int u = 0; u < U; ++u) look(s0 + u * 256, w[u], each);
     }
-    for (; s0 < to; s0 += 64 * N) {
-      uint32_t w[N];
-      fetch([&](int u) { return s0 + u * 64 + lane; }, w);
-      look(s0, w, each);
+    for (; s0 - 4 * lane < to; s0 += 256 * N) {
+      u32x4 w[N];
+      fetch([&](int i) { return s0 + i * 256; }, w);
+#pragma unroll
+      for (int i = 0; i < N; ++i) look(s0 + i * 256, w[i], each);
     }
   };
   int sures = 0, ties = 0;
-  walk([&](int, bool sure, bool tie) {
-    sures += __popcll(__builtin_amdgcn_ballot_w64(sure));
-    ties += __popcll(__builtin_amdgcn_ballot_w64(tie));
+  walk([&](int, const bool (&sure)[4], const bool (&tie)[4]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      sures += __popcll(__builtin_amdgcn_ballot_w64(sure[j]));
+      ties += __popcll(__builtin_amdgcn_ballot_w64(tie[j]));
+    }
   });
   if (lane == 0) { s_sure[wave] = sures; s_ties[wave] = ties; }
   __syncthreads();
@@ -325,14 +336,35 @@ __global__ __launch_bounds__(kPickThreads) void kv8_pick_kernel(Kv8 c, const flo
   }
   at += min(tied, left);
   const uint64_t below = (1ull << lane) - 1;
-  walk([&](int s, bool sure, bool tie) {
-    const uint64_t tie_mask = __builtin_amdgcn_ballot_w64(tie);
-    const bool stays = sure || (tie && tied + __popcll(tie_mask & below) < left);
-    const uint64_t mask = __builtin_amdgcn_ballot_w64(stays);
-    const int to_at = at + __popcll(mask & below);
-    if (stays && to_at < budget) out[to_at] = s;
-    at += __popcll(mask);
-    tied += __popcll(tie_mask);
+  // how many of a wave's flags are before this lane's first, and in all
+  auto rank = [&](const bool (&flag)[4], int& before, int& all) {
+    before = all = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint64_t mask = __builtin_amdgcn_ballot_w64(flag[j]);
+      before += __popcll(mask & below);
+      all += __popcll(mask);
+    }
+  };
+  walk([&](int s, const bool (&sure)[4], const bool (&tie)[4]) {
+    bool stays[4];
+    int before, all;
+    rank(tie, before, all);
+    before += tied;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      stays[j] = sure[j] || (tie[j] && before < left);
+      before += tie[j];
+    }
+    tied += all;
+    rank(stays, before, all);
+    before += at;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (stays[j] && before < budget) out[before] = s + j;
+      before += stays[j];
+    }
+    at += all;
   });
 }
 
@@ -462,7 +494,7 @@ pegainfer_status_t pegainfer_kv8_evict(const pegainfer_kv8_cache* cache, float* 
   if (cache->n_entries == 0) return 0;
   if (!mass || !lens || !dst_indptr || (!dst_ids && n_dst_ids > 0) || !kept || mass_page_stride < (int64_t)cache->kv_heads * kKv8Page) return PK_BAD;
   const Kv8 c = kv8_of(cache);
-  const int cached = std::min(max_len, kPickCached);
+  const int cached = (std::min(max_len, kPickCached) + 3) / 4 * 4;
   if (hipFuncSetAttribute(reinterpret_cast<const void*>(kv8_pick_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kPickCached * 4) != hipSuccess) return PK_BAD;
   kv8_pick_kernel<<<dim3(c.kv_heads, c.entries), kPickThreads, cached * 4, as_stream(stream)>>>(c, mass, mass_page_stride, lens, budget, keep_first, keep_last, cached, kept);
   const dim3 grid(std::max(1, ceil_div(std::min(budget, max_len), kKv8Page)), c.kv_heads, c.entries);
