@@ -184,16 +184,30 @@ __device__ __forceinline__ uint32_t order_of(float m) {
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
+// the sum of the lanes up to this one
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);      // from 1, 2, 4 and 8 lanes before, within sixteen
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);     // lane 15 to the second sixteen, 47 to the fourth
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);     // lane 31 to the upper half
+  return v;
+}
+// flags of the lanes before this one, on top of n
+__device__ __forceinline__ int lanes_before(uint64_t mask, int n) { return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, n)); }
+
 // Which tokens stay: one workgroup an (entry, head).  Three histograms over 11, 11 and 10 bits of the weights' order give the lightest weight that stays among those
 // between the first and the last tokens; then every wave counts, and after a barrier writes, the slots that stay of a run of its own, in order: of equal weights the
 // lowest slots.  Bound by the latency of few workgroups, so the weights are fetched once, through their pages, and kept in shared memory where they fit
 // (36 864 tokens; of those beyond, every pass fetches them again).  11 bits reach into the mantissa: weights share few exponents, and counts of one address are taken in turn.
 constexpr int kPickThreads = 1024, kPickWaves = kPickThreads / 64, kPickCached = 36864;
+constexpr uint32_t kAlways = 0xFFFFFFFFu;   // in the place of a weight's order, which never has it: the first and last tokens, and what lies behind the last
 __global__ __launch_bounds__(kPickThreads) void kv8_pick_kernel(Kv8 c, const float* mass, int64_t mass_stride, const int32_t* lens, int budget, int keep_first,
                                                                 int keep_last, int cached, int32_t* kept) {
   extern __shared__ u32x4 s_order[];
   __shared__ uint32_t hist[2048];
-  __shared__ int s_sure[kPickWaves], s_ties[kPickWaves], s_sum[kPickWaves];
+  __shared__ __attribute__((aligned(16))) int s_sure[kPickWaves], s_ties[kPickWaves], s_sum[kPickWaves];
   __shared__ uint32_t s_bits;
   __shared__ int s_left;
   const int e = blockIdx.y, head = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -206,6 +220,7 @@ __global__ __launch_bounds__(kPickThreads) void kv8_pick_kernel(Kv8 c, const flo
   // the weights of N fours of slots (from multiples of 4: of one page), page ids and weights each in one go: what is not there is read from the table's and the
   // cache's first place and left out
   const int first = c.indptr[e], pages = c.indptr[e + 1] - first;
+  const int lo = keep_first, hi = len - keep_last, chosen = budget - keep_first - keep_last;
   constexpr int N = 4;
   auto fetch = [&](auto slot, u32x4 (&w)[N]) {
     int page[N];
@@ -222,10 +237,18 @@ __global__ __launch_bounds__(kPickThreads) void kv8_pick_kernel(Kv8 c, const flo
 #pragma unroll
     for (int i = 0; i < N; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) w[i][j] = page[i] < 0 ? 0u : order_of(m[i][j]);
+      for (int j = 0; j < 4; ++j) {
+        const int s = slot(i) + j;
+        w[i][j] = s < lo || s >= hi ? kAlways : page[i] < 0 ? 0u : order_of(m[i][j]);
+      }
+  };
+  auto of_waves_before = [&](const int (&x)[kPickWaves]) {
+    int sum = 0;
+#pragma unroll
+    for (int i = 0; i < kPickWaves; ++i) sum += i < wave ? x[i] : 0;
+    return sum;
   };
   const int held = min(len, cached);       // slots whose weights are in shared memory (a multiple of 4, or all); the others' are fetched again
-  const int lo = keep_first, hi = len - keep_last, chosen = budget - keep_first - keep_last;
   for (int i = tid; i < 2048; i += kPickThreads) hist[i] = 0;
   __syncthreads();
   constexpr int kStep = 4 * kPickThreads;
@@ -238,10 +261,10 @@ __global__ __launch_bounds__(kPickThreads) void kv8_pick_kernel(Kv8 c, const flo
       if (s < held) s_order[s / 4] = w[i];
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (s + j >= lo && s + j < hi) atomicAdd(&hist[w[i][j] >> 21], 1u);
+        if (w[i][j] != kAlways) atomicAdd(&hist[w[i][j] >> 21], 1u);
     }
   }
-  uint32_t bits = 0;                       // of the lightest weight that stays: its upper bits so far
+  uint32_t bits = chosen > 0 ? 0u : kAlways - 1;   // of the lightest weight that stays: its upper bits so far
   int left = chosen;                       // tokens still to be found that have those
   if (chosen > 0) {
     for (int done = 0; done < 32; done += 11) {
@@ -252,32 +275,27 @@ __global__ __launch_bounds__(kPickThreads) void kv8_pick_kernel(Kv8 c, const flo
       }
       const uint32_t mask = done == 0 ? 0u : 0xFFFFFFFFu << (32 - done);
       if (done > 0) {                      // the first is counted as the weights arrive
-        auto count = [&](int s, const u32x4& w) {
+        auto count = [&](const u32x4& w) {
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            if (s + j >= lo && s + j < hi && (w[j] & mask) == bits) atomicAdd(&hist[(w[j] >> shift) & 2047 >> (11 - width)], 1u);
+            if ((w[j] & mask) == bits) atomicAdd(&hist[(w[j] >> shift) & 2047 >> (11 - width)], 1u);     // never one that always stays
         };
-#pragma unroll 2
-        for (int s = lo / 4 * 4 + 4 * tid; s < min(hi, held); s += kStep) count(s, s_order[s / 4]);
-        for (int s0 = max(lo / 4 * 4, held) + 4 * tid; held < len && s0 < hi; s0 += N * kStep) {
+#pragma unroll 4
+        for (int s = 4 * tid; s < held; s += kStep) count(s_order[s / 4]);
+        for (int s0 = held + 4 * tid; held < len && s0 < len; s0 += N * kStep) {
           u32x4 w[N];
           fetch([&](int i) { return s0 + i * kStep; }, w);
 #pragma unroll
-          for (int i = 0; i < N; ++i) count(s0 + i * kStep, w[i]);
+          for (int i = 0; i < N; ++i) count(w[i]);
         }
       }
       __syncthreads();
       // thread t: digits 2047 - 2 t and 2046 - 2 t; how many weights have a larger digit
       const int a = (int)hist[2047 - 2 * tid], b = (int)hist[2046 - 2 * tid];
-      int sum = a + b;
-#pragma unroll
-      for (int d = 1; d < 64; d <<= 1) {
-        const int o = __shfl_up(sum, d, 64);
-        if (lane >= d) sum += o;
-      }
+      int sum = wave_scan(a + b);
       if (lane == 63) s_sum[wave] = sum;
       __syncthreads();
-      for (int i = 0; i < wave; ++i) sum += s_sum[i];
+      sum += of_waves_before(s_sum);
       const int above = sum - a - b;
       if (above < left && left <= sum) {   // one thread: the counts reach `left` in its two digits
         const bool second = left > above + a;
@@ -293,12 +311,11 @@ __global__ __launch_bounds__(kPickThreads) void kv8_pick_kernel(Kv8 c, const flo
   const int run = (len + kStep - 1) / kStep * 256, from = min(wave * run, len), to = min(from + run, len);
   // four slots a lane, so that a wave's lanes and their slots are in order; two of shared memory at a time, or N through the pages
   auto look = [&](int s, const u32x4& w, auto&& each) {
-    bool sure[4], tie[4];
+    uint64_t sure[4], tie[4];              // of the wave's lanes, of each of their slots
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const bool in = s + j < to, always = in && (s + j < lo || s + j >= hi), between = in && !always && chosen > 0;
-      sure[j] = always || (between && w[j] > bits);
-      tie[j] = between && w[j] == bits;
+      sure[j] = __builtin_amdgcn_ballot_w64(s + j < to && w[j] > bits);
+      tie[j] = __builtin_amdgcn_ballot_w64(s + j < to && w[j] == bits);
     }
     each(s, sure, tie);
   };
@@ -320,51 +337,43 @@ __global__ __launch_bounds__(kPickThreads) void kv8_pick_kernel(Kv8 c, const flo
     }
   };
   int sures = 0, ties = 0;
-  walk([&](int, const bool (&sure)[4], const bool (&tie)[4]) {
+  walk([&](int, const uint64_t (&sure)[4], const uint64_t (&tie)[4]) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      sures += __popcll(__builtin_amdgcn_ballot_w64(sure[j]));
-      ties += __popcll(__builtin_amdgcn_ballot_w64(tie[j]));
+      sures += __popcll(sure[j]);
+      ties += __popcll(tie[j]);
     }
   });
   if (lane == 0) { s_sure[wave] = sures; s_ties[wave] = ties; }
   __syncthreads();
-  int at = 0, tied = 0;                    // tokens that stay, and ties met, in the slots before
-  for (int i = 0; i < wave; ++i) {
-    at += s_sure[i];
-    tied += s_ties[i];
-  }
-  at += min(tied, left);
-  const uint64_t below = (1ull << lane) - 1;
-  // how many of a wave's flags are before this lane's first, and in all
-  auto rank = [&](const bool (&flag)[4], int& before, int& all) {
-    before = all = 0;
+  int tied = of_waves_before(s_ties), at = of_waves_before(s_sure) + min(tied, left);      // ties met, and tokens that stay, in the slots before
+  walk([&](int s, const uint64_t (&sure)[4], const uint64_t (&tie)[4]) {
+    uint64_t stays[4];
+    int before = tied;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const uint64_t mask = __builtin_amdgcn_ballot_w64(flag[j]);
-      before += __popcll(mask & below);
-      all += __popcll(mask);
+      stays[j] = sure[j];
+      before = lanes_before(tie[j], before);
     }
-  };
-  walk([&](int s, const bool (&sure)[4], const bool (&tie)[4]) {
-    bool stays[4];
-    int before, all;
-    rank(tie, before, all);
-    before += tied;
+    if (tie[0] | tie[1] | tie[2] | tie[3]) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const bool here = tie[j] >> lane & 1;
+        stays[j] |= __builtin_amdgcn_ballot_w64(here && before < left);
+        before += here;
+        tied += __popcll(tie[j]);
+      }
+    }
+    int put = at;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) put = lanes_before(stays[j], put);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      stays[j] = sure[j] || (tie[j] && before < left);
-      before += tie[j];
+      const bool here = stays[j] >> lane & 1;
+      if (here && put < budget) out[put] = s + j;
+      put += here;
+      at += __popcll(stays[j]);
     }
-    tied += all;
-    rank(stays, before, all);
-    before += at;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (stays[j] && before < budget) out[before] = s + j;
-      before += stays[j];
-    }
-    at += all;
   });
 }
 
