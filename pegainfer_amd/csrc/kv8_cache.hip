@@ -276,9 +276,13 @@ __global__ __launch_bounds__(kPickThreads) void kv8_pick_kernel(Kv8 c, const flo
       const uint32_t mask = done == 0 ? 0u : 0xFFFFFFFFu << (32 - done);
       if (done > 0) {                      // the first is counted as the weights arrive
         auto count = [&](const u32x4& w) {
+          bool here[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if ((w[j] & mask) == bits) atomicAdd(&hist[(w[j] >> shift) & 2047 >> (11 - width)], 1u);     // never one that always stays
+          for (int j = 0; j < 4; ++j) here[j] = (w[j] & mask) == bits;     // never one that always stays
+          if (here[0] | here[1] | here[2] | here[3])
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (here[j]) atomicAdd(&hist[(w[j] >> shift) & 2047 >> (11 - width)], 1u);
         };
 #pragma unroll 4
         for (int s = 4 * tid; s < held; s += kStep) count(s_order[s / 4]);
@@ -308,32 +312,33 @@ __global__ __launch_bounds__(kPickThreads) void kv8_pick_kernel(Kv8 c, const flo
     }
   }
   __syncthreads();
-  const int run = (len + kStep - 1) / kStep * 256, from = min(wave * run, len), to = min(from + run, len);
-  // four slots a lane, so that a wave's lanes and their slots are in order; two of shared memory at a time, or N through the pages
+  // A wave's run is whole steps of its walk.  What the last one sees behind the last token always stays, or is the last token again: it comes when all places are taken.
+  constexpr int U = 2;                     // fours of slots a lane at a time: two of shared memory, or N through the pages
+  const int unit = 256 * (held < len ? N : U), run = (len + kPickWaves * unit - 1) / (kPickWaves * unit) * unit, from = min(wave * run, len), to = min(from + run, len);
+  const int near = held == len ? to : min(to, from + max(held - from, 0) / unit * unit);      // of the run, in shared memory
   auto look = [&](int s, const u32x4& w, auto&& each) {
     uint64_t sure[4], tie[4];              // of the wave's lanes, of each of their slots
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      sure[j] = __builtin_amdgcn_ballot_w64(s + j < to && w[j] > bits);
-      tie[j] = __builtin_amdgcn_ballot_w64(s + j < to && w[j] == bits);
+      sure[j] = __builtin_amdgcn_ballot_w64(w[j] > bits);
+      tie[j] = __builtin_amdgcn_ballot_w64(w[j] == bits);
     }
     each(s, sure, tie);
   };
   auto walk = [&](auto&& each) {
-    constexpr int U = 2;
-    int s0 = from + 4 * lane;
-    for (int at = from; at < min(to, held) && (held == len || at + 256 * U <= held); at += 256 * U, s0 += 256 * U) {
+    int at = from;
+    for (; at < near; at += 256 * U) {
       u32x4 w[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) w[u] = s_order[min(s0 + u * 256, held - 1) / 4];
+      for (int u = 0; u < U; ++u) w[u] = s_order[min(at + u * 256 + 4 * lane, held - 1) / 4];
 #pragma unroll
-      for (int u = 0; u < U; ++u) look(s0 + u * 256, w[u], each);
+      for (int u = 0; u < U; ++u) look(at + u * 256 + 4 * lane, w[u], each);
     }
-    for (; s0 - 4 * lane < to; s0 += 256 * N) {
+    for (; at < to; at += 256 * N) {
       u32x4 w[N];
-      fetch([&](int i) { return s0 + i * 256; }, w);
+      fetch([&](int i) { return at + i * 256 + 4 * lane; }, w);
 #pragma unroll
-      for (int i = 0; i < N; ++i) look(s0 + i * 256, w[i], each);
+      for (int i = 0; i < N; ++i) look(at + i * 256 + 4 * lane, w[i], each);
     }
   };
   int sures = 0, ties = 0;
