@@ -323,7 +323,8 @@ __global__ __launch_bounds__(256, (attn_waves<T, D, NT>())) void kv8_attn_kernel
 // Prompts: one workgroup, 128 query rows of a kv head.  Every step's blocks of keys and values (16 KB of codes, 32 KB as operands) are widened once, an equal share by
 // every wave, into one of two buffers of shared memory, while the other is read: a code is widened once for 128 rows and not for 32, and no states are joined at
 // the end.  Operands lie in shared memory as the lanes read them, 16 bytes a lane, without bank conflicts.  Four waves of 32 rows read least (D <= 128: 224 registers);
-// heads of 256 take eight waves of 16 rows, whose outputs and queries fit beside the rest.
+// heads of 256 take eight waves of 16 rows, whose outputs and queries fit beside the rest.  8000 rows of 32 / 8 heads of 128 over themselves: 500 us, 1.05 PFLOP/s; bound
+// by shared memory's reads (one for two products) and, for few tiles, by those that have a compute unit to themselves (1.5 us a step, two together 1.0 each).
 template <int D> constexpr int prompt_blocks() { return 512 / D; }   // of a step
 template <int D> constexpr int prompt_tiles() { return D == 256 ? 1 : 2; }   // of sixteen rows, a wave
 
@@ -526,7 +527,8 @@ __global__ __launch_bounds__(64 * 8 / prompt_tiles<D>(), 2) void kv8_prompt_kern
   }
 }
 
-// The splits' states of a (row, head) into its output: a workgroup takes 64 of its values, a wave every W-th split, sixteen of them on their way at a time.
+// The splits' states of a (row, head) into its output: a workgroup takes 64 of its values, a wave every W-th split, sixteen of them on their way at a time.  A launch
+// and two memory round trips: 128 splits of 16 rows of 256 values 5 us.
 template <typename T, int D>
 __global__ __launch_bounds__(512) void kv8_merge_kernel(AttnArgs a) {
   constexpr int C = D / 64;
@@ -640,7 +642,8 @@ __global__ __launch_bounds__(256) void kv8_merge_rows_kernel(AttnArgs a) {
 // The weights that a call gives to the cached tokens, from the sums that the attention left.  A wave holds four blocks of keys (two of 256 values) as operands while the workgroup walks
 // the rows that see them, MT tiles of sixteen a step, which its four waves (each with keys of its own) fetch together, two steps ahead, into shared memory: a
 // token's sum is one wave's, in the rows' order.  n_slice > 1, where that leaves too few workgroups: every slice of the rows leaves its sums in part,
-// kv8_mass_sum_kernel adds them in order.
+// kv8_mass_sum_kernel adds them in order.  Bound by shared memory's reads (one for four products, of 256 values for two) and the exponentials: 8000 rows of 32 / 8 heads of
+// 128 over themselves 382 us, 0.69 PFLOP/s; 3 prompts of up to 2000 of 16 / 4 x 256: 78.
 struct MassArgs {
   const float* mass;
   float *out, *part;     // part [n_slice][n_ids][kv_heads][16]
