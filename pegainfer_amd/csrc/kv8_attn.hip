@@ -910,7 +910,9 @@ inline AttnPlan attn_plan(const pegainfer_kv8_cache* cache, int n_rows, int max_
   p.snake = p.n_split == 1 && p.tiles > p.round && p.tiles <= 2 * p.round;
   p.score_rows = rows <= kStepRows ? (int)rows : 0;
   p.mass_groups = p.score_rows ? ceil_div(blocks, 256 / kKv8Page) : ceil_div(blocks, 4 * (cache->dim == 256 ? mass_blocks<256>() : mass_blocks<128>()));
-  p.n_slice = p.score_rows ? 1 : cut((p.mass_groups * pairs + 1) / 2, std::min<int64_t>((rows + 255) / 256, 16));   // the first keys' rows are twice the average's
+  // Weights: the first keys' rows are twice the average's.  Slices of 128 rows (four steps) at least: a step waits for its rows, 1 us, and the sum of the slices is a launch of 5
+  // (88 tokens of 8 heads a group: 39 us whole, 26 in slices of 256, 22 of 128, 20 of 64; 30 rows over 4 x 2000 tokens 35, 35, 35, 36.5).
+  p.n_slice = p.score_rows ? 1 : cut((p.mass_groups * pairs + 1) / 2, std::min<int64_t>((rows + 127) / 128, 16));
   return p;
 }
 // workgroups of `items` pieces of work cut `ways`, in whole pieces; kernels walk what a grid cannot hold
