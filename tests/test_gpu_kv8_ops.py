@@ -364,6 +364,33 @@ def test_evict_equal_and_odd_weights(fmt):
     run_evict(c, lens, 100, 0, 0)
 
 
+def test_weights_at_any_four_bytes():
+    """weights and scales whose pages lie an odd number of values apart, from an odd place: what aligned ones give, and nothing between them is touched"""
+    lens = [300, 41]
+    c = Cache([x - 1 for x in lens], [1, 1], 3, 64, "e4m3", seed=12, dirty=False, pages=60)
+    a, b = c.device(), c.device()
+    apart = 3 * 16 + 3
+    room = torch.full((c.pages * apart + 5,), 9.0, device="cuda")
+    b.mass = room[5:].as_strided((c.pages, 3, 16), (apart, 16, 1))
+    b.mass.copy_(a.mass)
+    scales = torch.zeros(c.pages * 7 + 1, device="cuda")[1:].as_strided((c.pages, 2, 3), (7, 3, 1))
+    scales.copy_(b.scales)
+    b.scales = scales
+    q = torch.randn(2, 6, 64, device="cuda").bfloat16()
+    free = torch.tensor([p for p in range(c.pages) if p not in c.ids], dtype=torch.int32, device="cuda")
+    dst = torch.tensor([0, 7, 10], dtype=torch.int32, device="cuda")
+    got = []
+    for d in (a, b):
+        out = B.kv8_attention(q, d.codes, d.scales, d.row0, d.starts, d.indptr, d.ids, 0.125, mass=d.mass, mass_keep=0.5)
+        kept = B.kv8_evict(d.codes, d.scales, d.mass, d.lens, d.indptr, d.ids, dst, free, 100, 5, 9)
+        got.append((out, kept, d.mass.contiguous(), d.scales.contiguous(), d.codes.contiguous().view(torch.uint8)))
+    for x, y in zip(*got):
+        assert torch.equal(x, y)
+    rest = torch.ones_like(room, dtype=torch.bool)
+    rest[5:].as_strided((c.pages, 3, 16), (apart, 16, 1)).fill_(False)
+    assert (room[rest] == 9).all()
+
+
 def test_evict_of_many_tokens_and_of_shared_pages():
     lens = [2500, 1030, 2500]
     c = Cache(lens, [0] * 3, 2, 64, "int8", seed=2, pages=700, dirty=False)
