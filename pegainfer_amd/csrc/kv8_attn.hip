@@ -99,6 +99,78 @@ __device__ __forceinline__ void put_row(const AttnArgs& a, const QueryRow& r, in
   }
 }
 
+struct MassArgs {
+  const float* mass;
+  float *out, *part;     // part [n_slice][n_ids][kv_heads][16]
+  int64_t mass_stride, out_stride;
+  float keep;
+  int n_slice;
+};
+__device__ __forceinline__ void put_mass(const MassArgs& w, int page, int at, float x) {
+  // 0 means without what was there, whatever that is
+  w.out[page * w.out_stride + at] = w.keep == 0.f ? x : fmaf(w.keep, w.mass[page * w.mass_stride + at], x);
+}
+
+// log2 of a row's sum of exp(scores) from its splits' states, a wave's lanes a split each
+__device__ __forceinline__ float lse_of_splits(const AttnArgs& a, int64_t rh, int lane) {
+  const f32x2* ml = reinterpret_cast<const f32x2*>(a.part_ml) + rh * a.n_split;
+  float m = -INFINITY, l = 0.f;
+  for (int i = lane; i < a.n_split; i += 64) m = fmaxf(m, ml[i].x);
+  m = wave_max(m);
+  const float base = m == -INFINITY ? 0.f : m;
+  for (int i = lane; i < a.n_split; i += 64) l += ml[i].y * exp2_of(ml[i].x - base);     // of a split without a key: 0 times exp2(-infinity)
+  l = wave_sum(l);
+  return l > 0.f || l != l ? m + __log2f(l) : INFINITY;
+}
+
+// What an entry's tokens weigh in a step, a thread a token, by workgroup z of `ways`, from the scores that the attention left (4 bytes a row beside D of the keys) and the
+// rows' log-sums; an entry with more rows than the call said has no scores, and its threads take the products themselves.
+constexpr int kStepRows = 16;
+template <typename T, int FMT, int D>
+__device__ __forceinline__ void step_mass(const AttnArgs& a, const MassArgs& w, int e, int head, const RowSpan& rows, int start, int z, int ways, float (&s_lse)[kStepRows]) {
+  const int len = a.c.tokens(e, start + rows.n), first_block = a.c.indptr[e], total = rows.n * a.group, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  if (z * 256 >= len) return;
+  const bool scored = total <= a.score_rows;
+  auto row_head = [&](int rr) { const QueryRow r = query_row(rr, total, a.group, rows, start, head); return (int64_t)r.row * a.heads + r.head; };
+  if (scored) {
+    for (int rr = wave; rr < total; rr += 4) {
+      const float x = a.n_split > 1 ? lse_of_splits(a, row_head(rr), lane) : a.lse[row_head(rr)];
+      if (lane == 0) s_lse[rr] = x;
+    }
+    __syncthreads();
+  }
+  for (int slot0 = z * 256; slot0 < len; slot0 += ways * 256) {
+    const int slot = slot0 + threadIdx.x, block = slot / kKv8Page, t = slot % kKv8Page, page = slot < len ? a.c.page(e, block) : -1;
+    float x = 0.f;
+    if (scored) {
+      if (page < 0) continue;
+      const float* s = a.scores + (((int64_t)first_block + block) * a.c.kv_heads + head) * a.score_rows * kKv8Page + t;
+#pragma unroll 4
+      for (int rr = 0; rr < total; ++rr) x += exp2_of(s[rr * kKv8Page] - s_lse[rr]);
+    } else {
+      const uint8_t* kb = a.c.block(max(page, 0), 0, head, D) + t * 64;
+      const float ks = *a.c.scale(max(page, 0), 0, head) * a.scale_log2;
+      for (int rr = 0; rr < total; ++rr) {             // all lanes walk all rows: a row's log-sum is a wave's work
+        const QueryRow r = query_row(rr, total, a.group, rows, start, head);
+        const int64_t rh = (int64_t)r.row * a.heads + r.head;
+        const float lse = a.n_split > 1 ? lse_of_splits(a, rh, lane) : a.lse[rh];
+        const T* q = static_cast<const T*>(a.q) + r.row * a.q_stride + (int64_t)r.head * D;
+        float dot = 0.f;
+#pragma unroll 1
+        for (int d = 0; d < D; d += 4) {
+          float k[4], y[4];
+          kv8_numbers<FMT>(*reinterpret_cast<const uint32_t*>(kb + d / 64 * 1024 + d % 64), k);
+          ld4(q + d, y);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) dot = fmaf(k[i], y[i], dot);
+        }
+        if (slot <= r.far) x += exp2_of(fmaf(dot, ks, -lse));
+      }
+    }
+    if (page >= 0) put_mass(w, page, head * kKv8Page + t, x);
+  }
+}
+
 // Blocks a wave takes at a time, and waves of a SIMD: what the registers hold without spilling.  Four blocks of 128 values and two row tiles spill, and are slower by
 // a tenth than two blocks (8 entries of 16 rows over 4000 tokens: 28.2 and 26.4 us); with one tile four are faster over short contexts (1024 tokens: 9.8 and 10.3 us)
 // and two over longer ones of few entries (8 x 4096: 16.2 and 15.2).
@@ -112,12 +184,14 @@ template <typename T, int D, int NT> constexpr int attn_waves() {
 // keys' scores of one row, exactly what the second product wants from it.  The next keys are on their way while the weights are made, the next values while
 // the next scores are.
 // ONCE: the rows are one tile, so nobody reads the keys again and they pass the caches by (32 x 8192 tokens int8: 78 -> 70 us, 4.8 TB/s).
-template <typename T, int FMT, int D, int NT, bool ONCE>
-__global__ __launch_bounds__(256, (attn_waves<T, D, NT>())) void kv8_attn_kernel(AttnArgs a) {
+// FEW: a step over so few tokens that the workgroup, which has seen them all, gives them their weights as well, without a second launch (100 tokens: 9.5 -> 8.2 us, of the
+// host 15.2 -> 12.4; over 1000 tokens the four walks through the scores take 1 us more than the launch).  An instance of its own: at its end the others lose 0.6 us.
+template <typename T, int FMT, int D, int NT, bool ONCE, bool FEW>
+__global__ __launch_bounds__(256, (attn_waves<T, D, NT>())) void kv8_attn_kernel(AttnArgs a, MassArgs w) {
   constexpr int NP = kv8_parts<T>(), C = D / 64, KB = attn_kb<T, D, NT>(), W = 4;
   constexpr bool kScaled = FMT == kE4m3;   // the conversion takes the block's scale along; int8 scales scores and weights instead
   __shared__ f32x4 s_o[W / 2][D / 16][64];
-  __shared__ float s_m[W / 2][16], s_l[W / 2][16];
+  __shared__ float s_m[W / 2][16], s_l[W / 2][16], s_lse[FEW ? kStepRows : 1];
   const int e = (blockIdx.y + blockIdx.z / a.n_split / a.round) % gridDim.y, head = blockIdx.x, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   const RowSpan rows = row_span(a.row0, e, a.n_rows);
   const int start = a.starts[e], total = rows.n * a.group;
@@ -318,6 +392,7 @@ __global__ __launch_bounds__(256, (attn_waves<T, D, NT>())) void kv8_attn_kernel
     }
     __syncthreads();
   }
+  if constexpr (FEW) step_mass<T, FMT, D>(a, w, e, head, rows, start, 0, 1, s_lse);      // what the workgroup left in memory is there since the barrier
 }
 
 // Prompts: one workgroup, 128 query rows of a kv head.  Every step's blocks of keys and values (16 KB of codes, 32 KB as operands) are widened once, an equal share by
@@ -644,18 +719,6 @@ __global__ __launch_bounds__(256) void kv8_merge_rows_kernel(AttnArgs a) {
 // token's sum is one wave's, in the rows' order.  n_slice > 1, where that leaves too few workgroups: every slice of the rows leaves its sums in part,
 // kv8_mass_sum_kernel adds them in order.  Bound by shared memory's reads (one for four products, of 256 values for two) and the exponentials: 8000 rows of 32 / 8 heads of
 // 128 over themselves 382 us, 0.69 PFLOP/s; 3 prompts of up to 2000 of 16 / 4 x 256: 78.
-struct MassArgs {
-  const float* mass;
-  float *out, *part;     // part [n_slice][n_ids][kv_heads][16]
-  int64_t mass_stride, out_stride;
-  float keep;
-  int n_slice;
-};
-__device__ __forceinline__ void put_mass(const MassArgs& w, int page, int at, float x) {
-  // 0 means without what was there, whatever that is
-  w.out[page * w.out_stride + at] = w.keep == 0.f ? x : fmaf(w.keep, w.mass[page * w.mass_stride + at], x);
-}
-
 template <int D> constexpr int mass_blocks() { return D == 256 ? 2 : 4; }   // of keys, a wave
 template <typename T, int D> constexpr int mass_tiles() { return sizeof(T) == 2 ? 2 : 1; }   // fp32: three parts of every query
 
@@ -798,22 +861,8 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? 2 : 1)) void kv8_mass_kernel
   }
 }
 
-// log2 of a row's sum of exp(scores) from its splits' states, a wave's lanes a split each
-__device__ __forceinline__ float lse_of_splits(const AttnArgs& a, int64_t rh, int lane) {
-  const f32x2* ml = reinterpret_cast<const f32x2*>(a.part_ml) + rh * a.n_split;
-  float m = -INFINITY, l = 0.f;
-  for (int i = lane; i < a.n_split; i += 64) m = fmaxf(m, ml[i].x);
-  m = wave_max(m);
-  const float base = m == -INFINITY ? 0.f : m;
-  for (int i = lane; i < a.n_split; i += 64) l += ml[i].y * exp2_of(ml[i].x - base);     // of a split without a key: 0 times exp2(-infinity)
-  l = wave_sum(l);
-  return l > 0.f || l != l ? m + __log2f(l) : INFINITY;
-}
-
-// The same for steps: a thread a token, whose rows' scores the attention left (4 bytes a row beside D of the keys); an entry with more rows than the call said has
-// none, and its threads take the products themselves.  Where the keys were split, the first `merges` workgroups of an entry and head join its outputs and the
-// others take the rows' log-sums from the splits' states: one launch for both (16 x 4096 tokens: 29.7 -> 27.5 us).
-constexpr int kStepRows = 16;
+// The weights of steps over many tokens.  Where the keys were split, the first `merges` workgroups of an entry and head join its outputs and the others take the rows'
+// log-sums from the splits' states: one launch for both (16 x 4096 tokens: 29.7 -> 27.5 us).
 template <typename T, int FMT, int D>
 __global__ __launch_bounds__(256) void kv8_step_finish_kernel(AttnArgs a, MassArgs w, int merges) {
   __shared__ float s_lse[kStepRows];
@@ -825,47 +874,7 @@ __global__ __launch_bounds__(256) void kv8_step_finish_kernel(AttnArgs a, MassAr
     for (int rr = blockIdx.z * 4 + wave; rr < total; rr += merges * 4) merge_row<T, D>(a, query_row(rr, total, a.group, rows, start, head), lane);
     return;
   }
-  const int len = a.c.tokens(e, start + rows.n), first_block = a.c.indptr[e], z = blockIdx.z - merges;
-  if (z * 256 >= len) return;
-  const bool scored = total <= a.score_rows;
-  auto row_head = [&](int rr) { const QueryRow r = query_row(rr, total, a.group, rows, start, head); return (int64_t)r.row * a.heads + r.head; };
-  if (scored) {
-    for (int rr = wave; rr < total; rr += 4) {
-      const float x = a.n_split > 1 ? lse_of_splits(a, row_head(rr), lane) : a.lse[row_head(rr)];
-      if (lane == 0) s_lse[rr] = x;
-    }
-    __syncthreads();
-  }
-  for (int slot0 = z * 256; slot0 < len; slot0 += (gridDim.z - merges) * 256) {
-    const int slot = slot0 + threadIdx.x, block = slot / kKv8Page, t = slot % kKv8Page, page = slot < len ? a.c.page(e, block) : -1;
-    float x = 0.f;
-    if (scored) {
-      if (page < 0) continue;
-      const float* s = a.scores + (((int64_t)first_block + block) * a.c.kv_heads + head) * a.score_rows * kKv8Page + t;
-#pragma unroll 4
-      for (int rr = 0; rr < total; ++rr) x += exp2_of(s[rr * kKv8Page] - s_lse[rr]);
-    } else {
-      const uint8_t* kb = a.c.block(max(page, 0), 0, head, D) + t * 64;
-      const float ks = *a.c.scale(max(page, 0), 0, head) * a.scale_log2;
-      for (int rr = 0; rr < total; ++rr) {             // all lanes walk all rows: a row's log-sum is a wave's work
-        const QueryRow r = query_row(rr, total, a.group, rows, start, head);
-        const int64_t rh = (int64_t)r.row * a.heads + r.head;
-        const float lse = a.n_split > 1 ? lse_of_splits(a, rh, lane) : a.lse[rh];
-        const T* q = static_cast<const T*>(a.q) + r.row * a.q_stride + (int64_t)r.head * D;
-        float dot = 0.f;
-#pragma unroll 1
-        for (int d = 0; d < D; d += 4) {
-          float k[4], y[4];
-          kv8_numbers<FMT>(*reinterpret_cast<const uint32_t*>(kb + d / 64 * 1024 + d % 64), k);
-          ld4(q + d, y);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) dot = fmaf(k[i], y[i], dot);
-        }
-        if (slot <= r.far) x += exp2_of(fmaf(dot, ks, -lse));
-      }
-    }
-    if (page >= 0) put_mass(w, page, head * kKv8Page + t, x);
-  }
+  step_mass<T, FMT, D>(a, w, e, head, rows, start, blockIdx.z - merges, gridDim.z - merges, s_lse);
 }
 
 // the slices' sums of a block's tokens, in order: a wave four blocks of a head
@@ -887,7 +896,7 @@ __global__ __launch_bounds__(256) void kv8_mass_sum_kernel(AttnArgs a, MassArgs 
 constexpr int kWholeBlocks = PEGAINFER_KV8_WHOLE / kKv8Page;
 
 // How a call is cut: rows of a workgroup, splits of the keys and slices of the weights' rows where those leave too few workgroups.
-struct AttnPlan { bool prompt; int tiles, row_tiles, n_split, split_blocks, mass_groups, n_slice, score_rows, round, snake; };
+struct AttnPlan { bool prompt, few; int tiles, row_tiles, n_split, split_blocks, mass_groups, n_slice, score_rows, round, snake; };
 inline AttnPlan attn_plan(const pegainfer_kv8_cache* cache, int n_rows, int max_rows, int max_len, int heads, int dtype) {
   AttnPlan p;
   const int64_t rows = (int64_t)std::min(max_rows, n_rows) * (heads / cache->kv_heads), pairs = (int64_t)cache->kv_heads * cache->n_entries;
@@ -906,6 +915,7 @@ inline AttnPlan attn_plan(const pegainfer_kv8_cache* cache, int n_rows, int max_
               : groups >= device_cus() ? 1
                                        : (int)std::max<int64_t>(1, std::min<int64_t>({want / groups, blocks / 32, 256}));
   p.split_blocks = ceil_div(blocks, p.n_split);
+  p.few = blocks <= 32;                    // a step's weights by the attention's workgroups: two tokens a thread
   p.round = (int)std::max<int64_t>(1, device_cus() / pairs);
   p.snake = p.n_split == 1 && p.tiles > p.round && p.tiles <= 2 * p.round;
   p.score_rows = rows <= kStepRows ? (int)rows : 0;
@@ -976,18 +986,19 @@ pegainfer_status_t pegainfer_kv8_attention(const pegainfer_kv8_cache* cache, con
       if (p.prompt) kv8_prompt_kernel<fmt(), D><<<grid, 64 * 8 / prompt_tiles<D>(), 0, as_stream(stream)>>>(a);
     }
     if constexpr (sizeof(T) == 2 || D < 256) {
-      if (!p.prompt && p.row_tiles == 2) kv8_attn_kernel<T, fmt(), D, 2, false><<<grid, 256, 0, as_stream(stream)>>>(a);
+      if (!p.prompt && p.row_tiles == 2) kv8_attn_kernel<T, fmt(), D, 2, false, false><<<grid, 256, 0, as_stream(stream)>>>(a, w);
     }
     if (!p.prompt && p.row_tiles == 1) {
-      if (p.score_rows) kv8_attn_kernel<T, fmt(), D, 1, true><<<grid, 256, 0, as_stream(stream)>>>(a);
-      else if constexpr (sizeof(T) == 4 && D == 256) kv8_attn_kernel<T, fmt(), D, 1, false><<<grid, 256, 0, as_stream(stream)>>>(a);
+      if (p.score_rows && weigh && p.few) kv8_attn_kernel<T, fmt(), D, 1, true, true><<<grid, 256, 0, as_stream(stream)>>>(a, w);
+      else if (p.score_rows) kv8_attn_kernel<T, fmt(), D, 1, true, false><<<grid, 256, 0, as_stream(stream)>>>(a, w);
+      else if constexpr (sizeof(T) == 4 && D == 256) kv8_attn_kernel<T, fmt(), D, 1, false, false><<<grid, 256, 0, as_stream(stream)>>>(a, w);
     }
     const bool step = weigh && p.score_rows, merge = p.n_split > 1 && !step;
     if (merge && many) kv8_merge_rows_kernel<T, D><<<rows_grid, 256, 0, as_stream(stream)>>>(a);
     if (merge && !many) kv8_merge_kernel<T, D><<<merge_grid, 64 * std::min(8, p.n_split), 0, as_stream(stream)>>>(a);
     const int merges = p.n_split > 1 ? ceil_div(p.score_rows, 4) : 0;
-    if (step) kv8_step_finish_kernel<T, fmt(), D><<<dim3(mass_grid.x, mass_grid.y, mass_grid.z + merges), 256, 0, as_stream(stream)>>>(a, w, merges);
-    else if (weigh) kv8_mass_kernel<T, fmt(), D><<<mass_grid, 256, 0, as_stream(stream)>>>(a, w);
+    if (step && !p.few) kv8_step_finish_kernel<T, fmt(), D><<<dim3(mass_grid.x, mass_grid.y, mass_grid.z + merges), 256, 0, as_stream(stream)>>>(a, w, merges);
+    if (weigh && !step) kv8_mass_kernel<T, fmt(), D><<<mass_grid, 256, 0, as_stream(stream)>>>(a, w);
   });
   if (weigh && p.n_slice > 1) kv8_mass_sum_kernel<<<sum_grid, 256, 0, as_stream(stream)>>>(a, w);
   return (pegainfer_status_t)hipGetLastError();

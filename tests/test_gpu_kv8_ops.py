@@ -152,6 +152,16 @@ def test_weights_of_cached_tokens(fmt, dtype, kv, group, dim):
     attend(c, kv * group, TYPES[dtype], weigh=True, keep=0.0)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("most", [1, 512, 513, 1024, 1025, 5000])
+def test_weights_whatever_the_hints(dtype, most):
+    """a step's weights by the attention itself, by a launch of its own, and beside the join of split keys; entries of more rows and tokens than was said"""
+    steps = Cache([511, 512, 20, 1300, 0], [1, 1, 1, 1, 1], 2, 64, "e4m3", seed=most)
+    mixed = Cache([600, 3, 0, 40], [1, 20, 0, 2], 1, 128, "int8", seed=most)
+    for c, group in ((steps, 4), (mixed, 3)):
+        attend(c, c.kv * group, TYPES[dtype], weigh=True, keep=0.5, hints=(1, most))
+
+
 def test_weights_of_many_rows():
     attend(Cache([0, 300], [200, 90], 1, 64, "e4m3", seed=9), 4, torch.bfloat16, weigh=True)
 
