@@ -1096,7 +1096,8 @@ typedef struct {
 } pegainfer_kv8_cache;
 /* Rows of k, v [n_rows][kv_heads][dim] (rows of dtype at strides of 16 bytes) into the slots starts[e] ...  A block's scale is the least 2^e (e >= -100) whose
  * top reaches its largest finite value, and not below that of the tokens that were in the block before starts[e], which are rescaled where it grew; codes are
- * rounded to nearest, ties to even; infinities become the top, a NaN becomes 0.  Slots of a written block behind the entry's last row become 0.  Two entries
+ * rounded to nearest, ties to even, but never to 2^128: what lies beyond the largest code * 2^e within fp32 (240 * 2^120, int8 127 * 2^121) becomes it; infinities
+ * become the top, a NaN becomes 0.  Slots of a written block behind the entry's last row become 0.  Two entries
  * of a call must not write the same page. */
 pegainfer_status_t pegainfer_kv8_append(const pegainfer_kv8_cache* cache, const void* k, const void* v, int64_t k_row_stride, int64_t v_row_stride,
                                         const int32_t* row0, const int32_t* starts, int32_t n_rows, int32_t max_rows, int32_t dtype, pegainfer_stream_t stream);
@@ -1106,7 +1107,8 @@ pegainfer_status_t pegainfer_kv8_read(const pegainfer_kv8_cache* cache, const in
 /* Causal softmax attention: row i of entry e sees the slots up to starts[e] + i (its own token is in the cache already), query head h reads kv head
  * h / (heads / kv_heads);  scale >= 0;  out[row, h] = sum_j softmax_j(scale q . k_j) v_j, zeros where a row sees nothing.  q, out: rows [heads][dim] of dtype at strides of
  * 16 bytes.  Scores, softmax state and sums are fp32; bf16: the softmax weights are rounded to bf16 where they enter the matrix cores (their sum is not); fp32:
- * queries and weights enter as three bf16 parts, nothing is rounded.  Entries may share pages (a common prompt).  out is not q.
+ * queries and weights enter as three bf16 parts, nothing is rounded.  Sums are divided at the end: values near fp32's largest must add up below it, each by its
+ * weight beside about the row's largest.  Entries may share pages (a common prompt).  out is not q.
  * mass_out given: mass_out[page][kv head][16] (fp32, pages mass_out_page_stride values apart) = mass_keep * mass + the weight that the call's rows and the kv
  * head's query heads gave to the token, for every slot of an entry that has rows (mass_out may be mass; mass_keep 0: mass is not read and may be NULL).  Every
  * sum has one order: results do not change from run to run.  Entries of such a call must not share a page (both would write its weights): those of a common prompt

@@ -4,6 +4,7 @@
 import numpy as np
 
 PAGE, TOP, LEAST = 16, {"e4m3": 448.0, "int8": 127.0}, -100
+LARGEST = {"e4m3": 240.0 * 2.0 ** 120, "int8": 127.0 * 2.0 ** 121}      # code * 2^e within fp32: the next one up is 2^128
 
 
 def _e4m3_numbers():
@@ -78,13 +79,13 @@ def append(k, v, codes, scales, fmt, row0, starts, tables):
                     old = max(start - low, 0)
                     rows = {t: x[row0[e] + low + t - start, h].astype(np.float64) for t in range(old, PAGE) if start <= low + t < start + n}
                     vals = np.abs(np.concatenate(list(rows.values())))
-                    ex = exponent(np.max(vals, where=np.isfinite(vals), initial=0.0), fmt)
+                    ex = exponent(min(np.max(vals, where=np.isfinite(vals), initial=0.0), LARGEST[fmt]), fmt)
                     was = scales[p, side, h]
                     if old:
                         ex = max(ex, int(np.log2(was)))
                     for t in range(PAGE):
                         at = offsets(dim, side, t)
-                        y = number(codes[p, side, h, at], fmt) * (float(was) * 2.0 ** -ex) if t < old else rows[t] * 2.0 ** -ex if t in rows else np.zeros(dim)
+                        y = number(codes[p, side, h, at], fmt) * (float(was) * 2.0 ** -ex) if t < old else np.clip(rows[t], -LARGEST[fmt], LARGEST[fmt]) * 2.0 ** -ex if t in rows else np.zeros(dim)
                         codes[p, side, h, at] = code(y, fmt)
                     scales[p, side, h] = 2.0 ** ex
 

@@ -90,12 +90,12 @@ __global__ __launch_bounds__(128) void kv8_append_kernel(Kv8 c, const T* k, cons
         amax = a <= 3.4028234e38f ? fmaxf(amax, a) : amax;            // finite values alone say how large the block is
       }
     }
-    int ex = kv8_exp<FMT>(wave_max(amax));
+    int ex = kv8_exp<FMT>(fminf(wave_max(amax), kv8_largest<FMT>()));
     uint8_t* blk = c.block(page, side, head, D);
     float* scale = c.scale(page, side, head);
     const int was = first > 0 ? exp_of(*scale) : ex;
     ex = max(ex, was);
-    const float to = pow2f(-ex), again = pow2f(was - ex);
+    const float to = pow2f(-ex), again = pow2f(was - ex), top = fminf(kv8_top<FMT>(), kv8_largest<FMT>() * to);
 #pragma unroll
     for (int ch = 0; ch < D / 64; ++ch) {
       uint8_t* at = blk + unit_at(side, ch, n, q);
@@ -108,7 +108,7 @@ __global__ __launch_bounds__(128) void kv8_append_kernel(Kv8 c, const T* k, cons
         if (first > 0) kv8_numbers<FMT>(old[w], y);
 #pragma unroll
         for (int i = 0; i < 4; ++i) y[i] = first > 0 && unit_token(side, n, q, 4 * w + i) < first ? y[i] * again : x[ch][4 * w + i] * to;
-        out[w] = kv8_codes<FMT>(y);
+        out[w] = kv8_codes<FMT>(y, top);
       }
       *reinterpret_cast<u32x4*>(at) = out;
     }

@@ -52,6 +52,8 @@ __device__ __forceinline__ RowSpan row_span(const int32_t* row0, int e, int n_ro
 }
 
 template <int FMT> constexpr float kv8_top() { return FMT == kE4m3 ? 448.f : 127.f; }
+// the largest code * 2^e within fp32, 240 * 2^120 or 127 * 2^121: a value that would be rounded past it, to 2^128, is taken for it
+template <int FMT> constexpr float kv8_largest() { return FMT == kE4m3 ? 0x1.ep127f : 0x1.fcp127f; }
 
 // least e with amax <= top 2^e: 448 = 1.75 * 2^8, 127 = 1.984375 * 2^6
 template <int FMT>
@@ -81,10 +83,10 @@ __device__ __forceinline__ void kv8_numbers(uint32_t w, float* o) {
 }
 // four numbers, already divided by the scale, to the nearest codes (ties to even; beyond the top: the top; NaN: 0)
 template <int FMT>
-__device__ __forceinline__ uint32_t kv8_codes(const float* x) {
+__device__ __forceinline__ uint32_t kv8_codes(const float* x, float top = kv8_top<FMT>()) {
   float y[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) y[i] = x[i] == x[i] ? fminf(fmaxf(x[i], -kv8_top<FMT>()), kv8_top<FMT>()) : 0.f;
+  for (int i = 0; i < 4; ++i) y[i] = x[i] == x[i] ? fminf(fmaxf(x[i], -top), top) : 0.f;
   if constexpr (FMT == kE4m3) {
     int w = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
     return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], w, true);
