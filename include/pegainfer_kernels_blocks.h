@@ -1101,6 +1101,12 @@ typedef struct {
  * of a call must not write the same page. */
 pegainfer_status_t pegainfer_kv8_append(const pegainfer_kv8_cache* cache, const void* k, const void* v, int64_t k_row_stride, int64_t v_row_stride,
                                         const int32_t* row0, const int32_t* starts, int32_t n_rows, int32_t max_rows, int32_t dtype, pegainfer_stream_t stream);
+/* The same into a cache whose tokens are weighed: mass [page][kv_heads][16] (fp32, pages mass_page_stride values apart) becomes 0 for the tokens that the rows bring and
+ * for the slots behind them in their last block.  Without it a page that another entry gave back still holds that entry's weights, and an attention that keeps the weights
+ * there were (mass_keep other than 0) adds to them. */
+pegainfer_status_t pegainfer_kv8_append_weighed(const pegainfer_kv8_cache* cache, float* mass, int64_t mass_page_stride, const void* k, const void* v, int64_t k_row_stride,
+                                                int64_t v_row_stride, const int32_t* row0, const int32_t* starts, int32_t n_rows, int32_t max_rows, int32_t dtype,
+                                                pegainfer_stream_t stream);
 /* The slots starts[e] ... as values, into k, v [n_rows][kv_heads][dim]; exact in both types */
 pegainfer_status_t pegainfer_kv8_read(const pegainfer_kv8_cache* cache, const int32_t* row0, const int32_t* starts, void* k, void* v, int32_t n_rows, int32_t max_rows,
                                       int32_t dtype, pegainfer_stream_t stream);
@@ -1110,7 +1116,8 @@ pegainfer_status_t pegainfer_kv8_read(const pegainfer_kv8_cache* cache, const in
  * queries and weights enter as three bf16 parts, nothing is rounded.  Sums are divided at the end: values near fp32's largest must add up below it, each by its
  * weight beside about the row's largest.  Entries may share pages (a common prompt).  out is not q.
  * mass_out given: mass_out[page][kv head][16] (fp32, pages mass_out_page_stride values apart) = mass_keep * mass + the weight that the call's rows and the kv
- * head's query heads gave to the token, for every slot of an entry that has rows (mass_out may be mass; mass_keep 0: mass is not read and may be NULL).  Every
+ * head's query heads gave to the token, for every slot of an entry that has rows, its new tokens among them (pegainfer_kv8_append_weighed sets theirs to 0; mass_out may
+ * be mass; mass_keep 0: mass is not read and may be NULL).  Every
  * sum has one order: results do not change from run to run.  Entries of such a call must not share a page (both would write its weights): those of a common prompt
  * go in calls of their own, one after the other.
  * workspace: fp32 scratch on 16 bytes of pegainfer_kv8_attention_workspace(...) values, of this call alone until it is done (0: NULL). */

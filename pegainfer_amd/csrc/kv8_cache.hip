@@ -63,10 +63,12 @@ __device__ __forceinline__ int unit_token(int side, int n, int q, int i) { retur
 
 // Rows into the cache.  One workgroup of two waves a (block, head): the rows' largest value, the exponent it wants (not below that of the tokens in front of
 // them in the block), their codes, and the older tokens' codes again where the exponent grew.  Bound by bytes: the rows are read once
-// (20 000 tokens of 8 x 128 from bf16: 34 us, 3.6 TB/s; 16 single tokens 5 us, a launch).
+// (20 000 tokens of 8 x 128 from bf16: 34 us, 3.6 TB/s; 16 single tokens 5 us, a launch).  mass: given, the tokens that the rows bring weigh nothing yet, and the
+// slots behind them neither, whatever a page's last owner left there.
+template <int D> constexpr int append_waves() { return D == 64 ? 8 : D == 128 ? 6 : 4; }   // of a SIMD, that the registers hold (8 x 128, prompts of up to 8000 rows in int8, with what is read back: 53 us with six or seven, 57 with five)
 template <typename T, int FMT, int D>
-__global__ __launch_bounds__(128) void kv8_append_kernel(Kv8 c, const T* k, const T* v, int64_t k_stride, int64_t v_stride, const int32_t* row0,
-                                                         const int32_t* starts, int n_rows) {
+__global__ __launch_bounds__(128, append_waves<D>()) void kv8_append_kernel(Kv8 c, float* mass, int64_t mass_stride, const T* k, const T* v, int64_t k_stride, int64_t v_stride,
+                                                         const int32_t* row0, const int32_t* starts, int n_rows) {
   const int e = blockIdx.z, head = blockIdx.y, side = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 15, q = lane >> 4;
   const RowSpan rows = row_span(row0, e, n_rows);
   const int64_t start = starts[e];
@@ -78,6 +80,7 @@ __global__ __launch_bounds__(128) void kv8_append_kernel(Kv8 c, const T* k, cons
     const int page = c.page(e, b);
     if (page < 0) continue;
     const int low = b * kKv8Page, first = max((int)start - low, 0);   // tokens 0 .. first - 1 of the block were there before
+    if (mass && side == 0 && q == 0 && n >= first) mass[page * mass_stride + head * kKv8Page + n] = 0.f;
     auto row = [&](int t) { const int s = low + t; return s >= start && s < end ? rows.first + (s - (int)start) : -1; };
     float x[D / 64][16], amax = 0.f;
 #pragma unroll
@@ -95,7 +98,7 @@ __global__ __launch_bounds__(128) void kv8_append_kernel(Kv8 c, const T* k, cons
     float* scale = c.scale(page, side, head);
     const int was = first > 0 ? exp_of(*scale) : ex;
     ex = max(ex, was);
-    const float to = pow2f(-ex), again = pow2f(was - ex), top = fminf(kv8_top<FMT>(), kv8_largest<FMT>() * to);
+    const float to = pow2f(-ex), again = pow2f(was - ex), top = FMT == kE4m3 && ex == 120 ? 240.f : kv8_top<FMT>();      // int8's exponent does not reach 122
 #pragma unroll
     for (int ch = 0; ch < D / 64; ++ch) {
       uint8_t* at = blk + unit_at(side, ch, n, q);
@@ -469,14 +472,9 @@ __global__ __launch_bounds__(128) void kv8_move_kernel(Kv8 c, const int32_t* dst
   }
 }
 
-}  // namespace pk
-
-using namespace pk;
-
-extern "C" {
-
-pegainfer_status_t pegainfer_kv8_append(const pegainfer_kv8_cache* cache, const void* k, const void* v, int64_t k_row_stride, int64_t v_row_stride,
-                                        const int32_t* row0, const int32_t* starts, int32_t n_rows, int32_t max_rows, int32_t dtype, pegainfer_stream_t stream) {
+static pegainfer_status_t append_rows(const pegainfer_kv8_cache* cache, float* mass, int64_t mass_page_stride, const void* k, const void* v, int64_t k_row_stride,
+                                      int64_t v_row_stride, const int32_t* row0, const int32_t* starts, int32_t n_rows, int32_t max_rows, int32_t dtype,
+                                      pegainfer_stream_t stream) {
   if (!kv8_ok(cache) || n_rows < 0 || max_rows < 0 || (dtype != kDtBf16 && dtype != kDtF32)) return PK_BAD;
   if (n_rows == 0 || max_rows == 0 || cache->n_entries == 0) return 0;
   const int64_t width = (int64_t)cache->kv_heads * cache->dim, unit = dtype == kDtBf16 ? 8 : 4;
@@ -486,10 +484,28 @@ pegainfer_status_t pegainfer_kv8_append(const pegainfer_kv8_cache* cache, const 
   const dim3 grid(std::min(max_rows, n_rows) / kKv8Page + 2, c.kv_heads, c.entries);
   kv8_by(dtype, cache->format, cache->dim, [&](auto* t, auto fmt, auto dim) {
     using T = std::remove_pointer_t<decltype(t)>;
-    kv8_append_kernel<T, fmt(), dim()><<<grid, 128, 0, as_stream(stream)>>>(c, static_cast<const T*>(k), static_cast<const T*>(v), k_row_stride, v_row_stride, row0,
-                                                                            starts, n_rows);
+    kv8_append_kernel<T, fmt(), dim()><<<grid, 128, 0, as_stream(stream)>>>(c, mass, mass_page_stride, static_cast<const T*>(k), static_cast<const T*>(v), k_row_stride,
+                                                                            v_row_stride, row0, starts, n_rows);
   });
   return (pegainfer_status_t)hipGetLastError();
+}
+
+}  // namespace pk
+
+using namespace pk;
+
+extern "C" {
+
+pegainfer_status_t pegainfer_kv8_append(const pegainfer_kv8_cache* cache, const void* k, const void* v, int64_t k_row_stride, int64_t v_row_stride,
+                                        const int32_t* row0, const int32_t* starts, int32_t n_rows, int32_t max_rows, int32_t dtype, pegainfer_stream_t stream) {
+  return append_rows(cache, nullptr, 0, k, v, k_row_stride, v_row_stride, row0, starts, n_rows, max_rows, dtype, stream);
+}
+
+pegainfer_status_t pegainfer_kv8_append_weighed(const pegainfer_kv8_cache* cache, float* mass, int64_t mass_page_stride, const void* k, const void* v, int64_t k_row_stride,
+                                                int64_t v_row_stride, const int32_t* row0, const int32_t* starts, int32_t n_rows, int32_t max_rows, int32_t dtype,
+                                                pegainfer_stream_t stream) {
+  if (!kv8_ok(cache) || !mass || mass_page_stride < (int64_t)cache->kv_heads * kKv8Page) return PK_BAD;
+  return append_rows(cache, mass, mass_page_stride, k, v, k_row_stride, v_row_stride, row0, starts, n_rows, max_rows, dtype, stream);
 }
 
 pegainfer_status_t pegainfer_kv8_read(const pegainfer_kv8_cache* cache, const int32_t* row0, const int32_t* starts, void* k, void* v, int32_t n_rows, int32_t max_rows,

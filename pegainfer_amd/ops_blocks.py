@@ -1015,16 +1015,21 @@ def _kv8_most(given, total, entries):
     return min(int(given) if given is not None else -(-total // max(entries, 1)), 2 ** 31 - 1)
 
 
-def kv8_append(k, v, codes, scales, row0, starts, page_indptr, page_ids, max_rows=None):
+def kv8_append(k, v, codes, scales, row0, starts, page_indptr, page_ids, max_rows=None, mass=None):
     """rows k, v [rows, kv_heads, dim] (bf16 or fp32 views, row stride free) into the cache behind the starts[e] tokens of their entry.  max_rows: about the most
-    rows of an entry (None: the average); it shapes the grid, the results are those of any"""
+    rows of an entry (None: the average); it shapes the grid, the results are those of any.  mass fp32 [pages, kv_heads, 16], of a cache whose tokens are weighed: 0 for
+    the tokens that the rows bring and the slots behind them in their block; without it what a page's last owner left there stays, and kv8_attention adds to it"""
     entries = row0.numel() - 1
     cache, kv, dim, device = _kv8_cache(codes, scales, page_indptr, page_ids, entries)
     tables = _kv8_index(row0, entries + 1, device, "row0"), _kv8_index(starts, entries, device, "starts")
     (n, _, k_apart, dtype), (n_v, _, v_apart, dtype_v) = _kv8_rows(k, kv, dim, device, "k"), _kv8_rows(v, kv, dim, device, "v")
     _kv8_need(n == n_v and dtype == dtype_v, "k and v of one shape and type")
-    _chk(ffi.lib().pegainfer_kv8_append(ctypes.addressof(cache), k.data_ptr(), v.data_ptr(), k_apart, v_apart, *tables, n, _kv8_most(max_rows, n, entries), dtype,
-                                        _raw_stream(device)), "kv8_append")
+    rows = k.data_ptr(), v.data_ptr(), k_apart, v_apart, *tables, n, _kv8_most(max_rows, n, entries), dtype, _raw_stream(device)
+    if mass is None:
+        _chk(ffi.lib().pegainfer_kv8_append(ctypes.addressof(cache), *rows), "kv8_append")
+    else:
+        apart = _kv8_mass(mass, codes, "mass")
+        _chk(ffi.lib().pegainfer_kv8_append_weighed(ctypes.addressof(cache), mass.data_ptr(), apart, *rows), "kv8_append")
 
 
 def kv8_read(codes, scales, row0, starts, page_indptr, page_ids, n_rows, dtype=torch.bfloat16, max_rows=None, out=None):
@@ -1050,8 +1055,8 @@ def kv8_read(codes, scales, row0, starts, page_indptr, page_ids, n_rows, dtype=t
 def kv8_attention(q, codes, scales, row0, starts, page_indptr, page_ids, scale, max_rows=None, max_len=None, out=None, mass=None, mass_out=None, mass_keep=1.0):
     """-> out [rows, heads, dim]: causal attention of q's rows (their own tokens are in the cache already).  max_rows / max_len: about the most rows / tokens of an
     entry (None: the average of the rows, twice that of the pages); they choose how the call is cut, results are right for any.  mass fp32 [pages, kv_heads, 16]:
-    mass_out (None: mass itself) becomes mass_keep * mass + the weight that every token got; mass_out alone with mass_keep 0: the weight of this call.  Entries may
-    share pages, but not where a call writes weights."""
+    mass_out (None: mass itself) becomes mass_keep * mass + the weight that every token got, the call's own among them (kv8_append(mass=) sets theirs to 0);
+    mass_out alone with mass_keep 0: the weight of this call.  Entries may share pages, but not where a call writes weights."""
     entries = row0.numel() - 1
     cache, kv, dim, device = _kv8_cache(codes, scales, page_indptr, page_ids, entries)
     row0_at, starts_at = _kv8_index(row0, entries + 1, device, "row0"), _kv8_index(starts, entries, device, "starts")

@@ -44,3 +44,56 @@ def test_values_next_to_the_largest_stay_finite(fmt, dtype):
         out = B.kv8_attention(torch.zeros(1, 2, 64, dtype=t, device="cuda"), d.codes, d.scales, i32(0, 1, 1), d.starts * 0, d.indptr, d.ids, 1.0)
         want = B.kv8_read(d.codes, d.scales, i32(0, 1, 1), d.starts * 0, d.indptr, d.ids, 1, dtype=t)[1]
         assert torch.equal(out, want.expand(1, 2, 64))
+
+
+# ---- weights of pages that another entry gave back ----
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("kv,dim", [(1, 64), (3, 128), (2, 256)])
+def test_appended_tokens_weigh_nothing(fmt, dtype, kv, dim):
+    c = Cache([0, 5, 16, 31, 40, 7, 0], [1, 1, 33, 1, 0, 9, 17], kv, dim, fmt, seed=kv, layers=2)
+    c.ids[c.indptr[2]], c.ids[c.indptr[6]] = -1, c.pages                 # pages that are not there
+    k = torch.randn(c.row0[-1], kv, dim, device="cuda").to(TYPES[dtype])
+    want = c.mass.copy()
+    for e in range(c.B):
+        for s in range(c.starts[e], (c.starts[e] + c.rows[e] + 15) // 16 * 16 if c.rows[e] else 0):
+            p = R.page_of(c.tables, e, s // 16, c.pages)
+            if p >= 0:
+                want[p, :, s % 16] = 0
+    for most in (None, 1, 33):
+        a, b = c.device(), c.device()
+        for d, kw in ((a, {}), (b, dict(mass=b.mass))):
+            B.kv8_append(k, k, d.codes, d.scales, d.row0, d.starts, d.indptr, d.ids, max_rows=most, **kw)
+        assert np.array_equal(b.mass.cpu().numpy(), want) and np.array_equal(a.mass.cpu().numpy(), c.mass)
+        assert torch.equal(a.pool, b.pool) and torch.equal(a.scales, b.scales)
+    with pytest.raises(ValueError):
+        B.kv8_append(k, k, b.codes, b.scales, b.row0, b.starts, b.indptr, b.ids, mass=b.mass[..., :8])
+
+
+def test_a_pool_that_pages_come_back_to():
+    """a session over pages that another one left: its weights, what it evicts and what it answers are those over a fresh pool"""
+    kv, H, dim, pages, budget = 2, 4, 64, 12, 40
+    order = i32(*range(1, pages))
+    rows = torch.randn(70, kv, dim, device="cuda").bfloat16()
+    q = torch.randn(70, H, dim, device="cuda").bfloat16()
+
+    def session(codes, scales, mass, n):
+        """a prompt, steps, a cut, a step behind it"""
+        got = []
+        for start, m in [(0, n)] + [(n + i, 1) for i in range(5)]:
+            t = i32(0, m), i32(start), i32(0, 7), order
+            B.kv8_append(rows[start:start + m], rows[start:start + m], codes, scales, *t, mass=mass)
+            got.append(B.kv8_attention(q[:m], codes, scales, *t, 0.125, mass=mass))
+        got.append(B.kv8_evict(codes, scales, mass, i32(n + 5), i32(0, 7), order, i32(0, 4), order[7:], budget, 2, 8))
+        t = i32(0, 1), i32(min(budget, n + 5)), i32(0, 4), order[7:]
+        B.kv8_append(rows[:1], rows[:1], codes, scales, *t, mass=mass)
+        return got + [B.kv8_attention(q[:1], codes, scales, *t, 0.125, mass=mass)]
+
+    def pool():
+        return torch.zeros(pages, 2, kv, 16 * dim, dtype=torch.int8, device="cuda"), torch.ones(pages, 2, kv, device="cuda"), torch.zeros(pages, kv, 16, device="cuda")
+
+    used, fresh = pool(), pool()
+    session(*used, 61)
+    for a, b in zip(session(*used, 50), session(*fresh, 50)):
+        assert torch.equal(a, b)
+    assert torch.equal(used[2][order[7:10].long()], fresh[2][order[7:10].long()])

@@ -1,8 +1,11 @@
-"""CPU: the ends of the 8-bit cache's ranges in the float64 restatement."""
+"""CPU: the ends of the 8-bit cache's ranges in the float64 restatement, and the refusals at them."""
+import ctypes
+
 import numpy as np
 import pytest
 
 from oracle import kv8_ref as R
+from pegainfer_amd import ffi, ops_blocks as B
 
 LARGEST = {"e4m3": 240 * 2.0 ** 120, "int8": 127 * 2.0 ** 121}      # code * 2^e: the next one up is 2^128
 
@@ -19,3 +22,13 @@ def test_what_is_kept_of_a_finite_value_is_finite(fmt, x):
         assert np.isfinite(got.astype(np.float32)).all() and np.abs(got).max() <= LARGEST[fmt]
         if np.isfinite(x):
             assert (np.abs(got - k) <= (2.0 ** -4 * np.abs(k) if fmt == "e4m3" else np.abs(k).max() / 127)).all()
+
+
+def test_rows_into_a_weighed_cache_need_its_weights(built_libs):
+    L, at = ffi.lib(), 1 << 20      # never followed: every call is refused before a launch
+    c = B.Kv8Cache(codes=at, scales=at, code_page_stride=2 * 2 * 16 * 64, scale_page_stride=4, format=0, n_pages=3, kv_heads=2, dim=64, page_indptr=at, page_ids=at,
+                   n_page_ids=3, n_entries=1)
+    for mass, apart, k in [(None, 32, at), (at, 31, at), (at, 32, None), (at, 32, at + 8)]:
+        assert L.pegainfer_kv8_append_weighed(ctypes.addressof(c), mass, apart, k, at, 128, 128, at, at, 4, 4, 0, None) == 1
+    assert L.pegainfer_kv8_append_weighed(None, at, 32, at, at, 128, 128, at, at, 4, 4, 0, None) == 1
+    assert L.pegainfer_kv8_append_weighed(ctypes.addressof(c), at, 32, None, None, 0, 0, None, None, 0, 4, 0, None) == 0
