@@ -1081,7 +1081,7 @@ pegainfer_status_t pegainfer_scale_rows(const void* in, int64_t in_stride, void*
  * page_ids[page_indptr[e]] ..; starts[e] = the tokens it holds in front of the call's rows.  All tables are int32 on the device and may change between the
  * replays of a captured graph.  A slot without a page in [0, n_pages) is not there: never written, never seen, read as 0;
  * no entry has more slots than its part of page_ids.  Rows behind row0[n_entries]
- * are left alone.  max_rows: about the most rows of an entry, max_len: about the most slots; they shape the grid, results hold for any (0 rows: no call).
+ * are left alone.  max_rows: about the most rows of an entry, max_len: about the most slots; they shape the grid, results hold for any (max_rows 0 counts as 1).
  * At most 65535 entries and 2^26 page ids; storage types as elsewhere: 0 = bf16, 1 = fp32. */
 enum { PEGAINFER_KV8_E4M3 = 0, PEGAINFER_KV8_INT8 = 1 };
 /* keys of as many tokens (max_len) are not cut: without weights the attention then needs no workspace */

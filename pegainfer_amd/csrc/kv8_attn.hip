@@ -897,9 +897,10 @@ constexpr int kWholeBlocks = PEGAINFER_KV8_WHOLE / kKv8Page;
 
 // How a call is cut: rows of a workgroup, splits of the keys and slices of the weights' rows where those leave too few workgroups.
 struct AttnPlan { bool prompt, few; int tiles, row_tiles, n_split, split_blocks, mass_groups, n_slice, score_rows, round, snake; };
+inline int rows_hint(int max_rows, int n_rows) { return std::min(std::max(max_rows, 1), n_rows); }
 inline AttnPlan attn_plan(const pegainfer_kv8_cache* cache, int n_rows, int max_rows, int max_len, int heads, int dtype) {
   AttnPlan p;
-  const int64_t rows = (int64_t)std::min(max_rows, n_rows) * (heads / cache->kv_heads), pairs = (int64_t)cache->kv_heads * cache->n_entries;
+  const int64_t rows = (int64_t)rows_hint(max_rows, n_rows) * (heads / cache->kv_heads), pairs = (int64_t)cache->kv_heads * cache->n_entries;
   p.row_tiles = rows > 16 && !(dtype == kDtF32 && cache->dim == 256) ? 2 : 1;
   p.prompt = dtype == kDtBf16 && rows >= kPromptRows;
   p.tiles = ceil_div(rows, p.prompt ? kPromptRows : 16 * p.row_tiles);
@@ -938,7 +939,7 @@ extern "C" {
 
 int64_t pegainfer_kv8_attention_workspace(const pegainfer_kv8_cache* cache, int32_t n_rows, int32_t max_rows, int32_t max_len, int32_t heads, int32_t dtype,
                                           int32_t with_mass) {
-  if (!kv8_ok(cache) || n_rows <= 0 || max_rows <= 0 || max_len < 0 || heads < cache->kv_heads || cache->n_entries == 0) return 0;
+  if (!kv8_ok(cache) || n_rows <= 0 || max_rows < 0 || max_len < 0 || heads < cache->kv_heads || cache->n_entries == 0) return 0;
   const AttnPlan p = attn_plan(cache, n_rows, max_rows, max_len, heads, dtype);
   const int64_t rh = (int64_t)n_rows * heads;
   const int64_t slots = (int64_t)cache->n_page_ids * cache->kv_heads * kKv8Page;
@@ -950,7 +951,7 @@ pegainfer_status_t pegainfer_kv8_attention(const pegainfer_kv8_cache* cache, con
   if (!kv8_ok(cache) || !d || (d->dtype != kDtBf16 && d->dtype != kDtF32) || d->heads < 1 || d->heads % cache->kv_heads || d->n_rows < 0 || d->max_rows < 0 || d->max_len < 0 ||
       !(d->scale >= 0.f))
     return PK_BAD;
-  if (d->n_rows == 0 || d->max_rows == 0 || cache->n_entries == 0) return 0;
+  if (d->n_rows == 0 || cache->n_entries == 0) return 0;
   const int64_t width = (int64_t)d->heads * cache->dim, unit = d->dtype == kDtBf16 ? 8 : 4;
   if (!d->q || !d->out || !d->row0 || !d->starts || !host_aligned16(d->q) || !host_aligned16(d->out) || d->q_row_stride < width || d->out_row_stride < width ||
       d->q_row_stride % unit || d->out_row_stride % unit || (int64_t)d->n_rows * (d->heads / cache->kv_heads) > INT32_MAX - 1024)
@@ -975,8 +976,9 @@ pegainfer_status_t pegainfer_kv8_attention(const pegainfer_kv8_cache* cache, con
   const dim3 grid(cache->kv_heads, cache->n_entries, deal(p.tiles, p.n_split)), mass_grid(cache->kv_heads, cache->n_entries, deal(p.mass_groups, p.n_slice));
   // splits of 2048 rows and heads fill the chip with a wave each; of fewer, a workgroup each shortens the walk over many splits
   const bool many = p.n_split <= 8 || rh >= 2048;
-  const dim3 merge_grid(std::min(d->max_rows, d->n_rows) * group * (cache->dim / 64), cache->kv_heads, cache->n_entries);
-  const dim3 rows_grid(ceil_div((int64_t)std::min(d->max_rows, d->n_rows) * group, 4), cache->kv_heads, cache->n_entries);
+  const int64_t rows = (int64_t)rows_hint(d->max_rows, d->n_rows) * group;
+  const dim3 merge_grid((uint32_t)(rows * (cache->dim / 64)), cache->kv_heads, cache->n_entries);
+  const dim3 rows_grid(ceil_div(rows, 4), cache->kv_heads, cache->n_entries);
   const dim3 sum_grid(std::max(1, ceil_div(d->max_len, 256)), cache->kv_heads, cache->n_entries);
   const MassArgs w{d->mass, d->mass_out, rest, d->mass_page_stride, d->mass_out_page_stride, d->mass_keep, p.n_slice};
   kv8_by(d->dtype, cache->format, cache->dim, [&](auto* t, auto fmt, auto dim) {

@@ -476,7 +476,7 @@ static pegainfer_status_t append_rows(const pegainfer_kv8_cache* cache, float* m
                                       int64_t v_row_stride, const int32_t* row0, const int32_t* starts, int32_t n_rows, int32_t max_rows, int32_t dtype,
                                       pegainfer_stream_t stream) {
   if (!kv8_ok(cache) || n_rows < 0 || max_rows < 0 || (dtype != kDtBf16 && dtype != kDtF32)) return PK_BAD;
-  if (n_rows == 0 || max_rows == 0 || cache->n_entries == 0) return 0;
+  if (n_rows == 0 || cache->n_entries == 0) return 0;
   const int64_t width = (int64_t)cache->kv_heads * cache->dim, unit = dtype == kDtBf16 ? 8 : 4;
   if (!k || !v || !row0 || !starts || !host_aligned16(k) || !host_aligned16(v) || k_row_stride < width || v_row_stride < width || k_row_stride % unit || v_row_stride % unit)
     return PK_BAD;
@@ -511,7 +511,7 @@ pegainfer_status_t pegainfer_kv8_append_weighed(const pegainfer_kv8_cache* cache
 pegainfer_status_t pegainfer_kv8_read(const pegainfer_kv8_cache* cache, const int32_t* row0, const int32_t* starts, void* k, void* v, int32_t n_rows, int32_t max_rows,
                                       int32_t dtype, pegainfer_stream_t stream) {
   if (!kv8_ok(cache) || n_rows < 0 || max_rows < 0 || (dtype != kDtBf16 && dtype != kDtF32)) return PK_BAD;
-  if (n_rows == 0 || max_rows == 0 || cache->n_entries == 0) return 0;
+  if (n_rows == 0 || cache->n_entries == 0) return 0;
   if (!row0 || !starts || !k || !v || !host_aligned16(k) || !host_aligned16(v)) return PK_BAD;
   const Kv8 c = kv8_of(cache);
   const dim3 grid(std::min(max_rows, n_rows) / kKv8Page + 2, c.kv_heads, c.entries);

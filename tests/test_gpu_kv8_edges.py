@@ -97,3 +97,19 @@ def test_a_pool_that_pages_come_back_to():
     for a, b in zip(session(*used, 50), session(*fresh, 50)):
         assert torch.equal(a, b)
     assert torch.equal(used[2][order[7:10].long()], fresh[2][order[7:10].long()])
+
+
+def test_a_hint_of_no_rows_gives_what_any_gives():
+    c = Cache([20, 0, 600], [4, 20, 1], 2, 64, "e4m3", seed=41, dirty=False)
+    a, b = c.device(), c.device()
+    k, q = torch.randn(25, 2, 64, device="cuda").bfloat16(), torch.randn(25, 4, 64, device="cuda").bfloat16()
+    got = []
+    for d, most in ((a, 0), (b, 1)):
+        t = d.row0, d.starts, d.indptr, d.ids
+        B.kv8_append(k, k, d.codes, d.scales, *t, max_rows=most)
+        for length in (700, 3000):
+            got.append((B.kv8_attention(q, d.codes, d.scales, *t, 0.1, max_rows=most, max_len=length, mass=d.mass, out=torch.full_like(q, 7.0)),
+                        *B.kv8_read(d.codes, d.scales, *t, 25, max_rows=most, out=(torch.full_like(k, 7.0), torch.full_like(k, 7.0)))))
+    for x, y in zip(got[:2], got[2:]):
+        assert all(torch.equal(i, j) for i, j in zip(x, y))
+    assert torch.equal(a.pool, b.pool) and torch.equal(a.scales, b.scales) and torch.equal(a.mass, b.mass)

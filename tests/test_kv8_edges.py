@@ -32,3 +32,17 @@ def test_rows_into_a_weighed_cache_need_its_weights(built_libs):
         assert L.pegainfer_kv8_append_weighed(ctypes.addressof(c), mass, apart, k, at, 128, 128, at, at, 4, 4, 0, None) == 1
     assert L.pegainfer_kv8_append_weighed(None, at, 32, at, at, 128, 128, at, at, 4, 4, 0, None) == 1
     assert L.pegainfer_kv8_append_weighed(ctypes.addressof(c), at, 32, None, None, 0, 0, None, None, 0, 4, 0, None) == 0
+
+
+def test_a_hint_of_no_rows_is_no_call_without_rows(built_libs):
+    """max_rows is about the most rows of an entry: whatever it says, the call's rows are looked at, and refused where they are wrong"""
+    L, at, ref = ffi.lib(), 1 << 20, ctypes.addressof
+    c = B.Kv8Cache(codes=at, scales=at, code_page_stride=2 * 2 * 16 * 64, scale_page_stride=4, format=0, n_pages=3, kv_heads=2, dim=64, page_indptr=at, page_ids=at,
+                   n_page_ids=3, n_entries=1)
+    assert L.pegainfer_kv8_append(ref(c), None, at, 128, 128, at, at, 4, 0, 0, None) == 1
+    assert L.pegainfer_kv8_read(ref(c), at, at, None, at, 4, 0, 0, None) == 1
+    d = B.Kv8AttnDesc(q=None, q_row_stride=256, out=at, out_row_stride=256, row0=at, starts=at, n_rows=4, max_rows=0, max_len=9, heads=4, scale=1.0, dtype=0)
+    assert L.pegainfer_kv8_attention(ref(c), ref(d), None) == 1
+    for max_len in (9, 5000):
+        for mass in (0, 1):
+            assert L.pegainfer_kv8_attention_workspace(ref(c), 4, 0, max_len, 4, 0, mass) == L.pegainfer_kv8_attention_workspace(ref(c), 4, 1, max_len, 4, 0, mass)
