@@ -955,7 +955,8 @@ def _kv8_need(ok, what):
         raise ValueError("kv8: " + what)
 
 
-_I32, _F32, _current_device, _raw_stream = torch.int32, torch.float32, torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+_I32, _F32 = torch.int32, torch.float32
+_current_device, _raw_stream = (getattr(torch._C, name, None) for name in ("_cuda_getDevice", "_cuda_getCurrentRawStream"))     # None: a torch without a GPU build, whose tensors are refused first
 _KV8_DTYPES, _KV8_BLOCKS = {torch.bfloat16: 0, torch.float32: 1}, (1024, 2048, 4096)
 
 

@@ -1,5 +1,8 @@
 """CPU: the ends of the 8-bit cache's ranges in the float64 restatement, and the refusals at them."""
 import ctypes
+import os
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -46,3 +49,16 @@ def test_a_hint_of_no_rows_is_no_call_without_rows(built_libs):
     for max_len in (9, 5000):
         for mass in (0, 1):
             assert L.pegainfer_kv8_attention_workspace(ref(c), 4, 0, max_len, 4, 0, mass) == L.pegainfer_kv8_attention_workspace(ref(c), 4, 1, max_len, 4, 0, mass)
+
+
+def test_the_wrappers_import_beside_a_torch_without_a_gpu_build():
+    """what such a torch lacks is looked up by the calls alone, which refuse first"""
+    code = ("import torch\n"
+            "for name in ('_cuda_getDevice', '_cuda_getCurrentRawStream'):\n"
+            "    if hasattr(torch._C, name): delattr(torch._C, name)\n"
+            "from pegainfer_amd import ops, ops_blocks as B\n"
+            "i = torch.zeros(2, dtype=torch.int32)\n"
+            "try: B.kv8_read(torch.zeros(3, 2, 2, 1024, dtype=torch.int8), torch.zeros(3, 2, 2), i, i[:1], i, i, 1)\n"
+            "except ValueError as e: print('refused', e)\n")
+    p = subprocess.run([sys.executable, "-c", code], cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))), capture_output=True, text=True, timeout=120)
+    assert p.returncode == 0 and "refused kv8" in p.stdout, p.stderr
