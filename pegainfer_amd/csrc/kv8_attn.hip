@@ -123,51 +123,98 @@ __device__ __forceinline__ float lse_of_splits(const AttnArgs& a, int64_t rh, in
   return l > 0.f || l != l ? m + __log2f(l) : INFINITY;
 }
 
+// The same of lane (n, g)'s row n, by the four lanes that have it
+__device__ __forceinline__ float lse_of_row(const AttnArgs& a, int64_t rh, int g) {
+  if (a.n_split == 1) return a.lse[rh];
+  const f32x2* ml = reinterpret_cast<const f32x2*>(a.part_ml) + rh * a.n_split;
+  float m = -INFINITY, l = 0.f;
+  for (int i = g; i < a.n_split; i += 4) m = fmaxf(m, ml[i].x);
+  m = quad_max(m);
+  const float base = m == -INFINITY ? 0.f : m;
+  for (int i = g; i < a.n_split; i += 4) l += ml[i].y * exp2_of(ml[i].x - base);
+  l = quad_sum(l);
+  return l > 0.f || l != l ? m + __log2f(l) : INFINITY;
+}
+
+// What the tokens of an entry weigh that has more rows than the call said, and so no scores, by workgroup z of `ways`: every wave two blocks (fp32: one; more
+// take registers that a step's waves want), sixteen rows at a time, their products taken again.  A portion of 256
+// rows of 128 values among 31 single ones that the hint is made for, 8 heads: 184 us over 300 tokens, 105 of them the attention, and 656, 521 of them, over 4000
+// (a thread a token took 3447 and 5169; with the portion's rows as the hint 52 and 257).
+template <typename T, int FMT, int D>
+__device__ __forceinline__ void rows_mass(const AttnArgs& a, const MassArgs& w, int e, int head, const RowSpan& rows, int start, int z, int ways) {
+  constexpr int NP = kv8_parts<T>(), C = D / 64, B = sizeof(T) == 2 ? 2 : 1;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+  const int len = a.c.tokens(e, start + rows.n), total = rows.n * a.group;
+  for (int b0 = (z * 4 + wave) * B; b0 * kKv8Page < len; b0 += ways * 4 * B) {
+    f32x4 sum[B];
+#pragma unroll
+    for (int h = 0; h < B; ++h) sum[h] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int first = (int)((int64_t)max(b0 * kKv8Page - start, 0) * a.group / 16);       // the first sixteen with a row that sees one of the blocks
+    for (int tile = first; tile * 16 < total; ++tile) {
+      const QueryRow r = query_row(tile * 16 + n, total, a.group, rows, start, head);
+      const float lse = lse_of_row(a, (int64_t)r.row * a.heads + r.head, g), off = r.real ? lse : INFINITY;     // a row behind the last weighs nothing
+      const T* qp = static_cast<const T*>(a.q) + r.row * a.q_stride + (int64_t)r.head * D + g * 16;
+      f32x4 s[B];
+#pragma unroll
+      for (int h = 0; h < B; ++h) s[h] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+      for (int c = 0; c < C; ++c) {
+        bf16x8_t q[2][NP];
+        kv8_query(qp + c * 64, q[0]);
+        kv8_query(qp + c * 64 + 8, q[1]);
+#pragma unroll
+        for (int h = 0; h < B; ++h) {
+          const u32x4 k = *reinterpret_cast<const u32x4*>(a.c.block(max(a.c.page(e, b0 + h), 0), 0, head, D) + c * 1024 + n * 64 + g * 16);
+          const bf16x8_t k0 = kv8_operand<FMT>(k.x, k.y), k1 = kv8_operand<FMT>(k.z, k.w);
+#pragma unroll
+          for (int p = NP - 1; p >= 0; --p) {
+            s[h] = mfma16(k0, q[0][p], s[h]);
+            s[h] = mfma16(k1, q[1][p], s[h]);
+          }
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < B; ++h) {
+        const float ks = *a.c.scale(max(a.c.page(e, b0 + h), 0), 0, head) * a.scale_log2;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[h][i] += (b0 + h) * kKv8Page + 4 * g + i <= r.far ? exp2_of(fmaf(s[h][i], ks, -off)) : 0.f;
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < B; ++h) {
+      const int page = a.c.page(e, b0 + h);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float x = row16_sum(sum[h][i]);
+        const int t = 4 * g + i;
+        if (n == i && page >= 0 && (b0 + h) * kKv8Page + t < len) put_mass(w, page, head * kKv8Page + t, x);
+      }
+    }
+  }
+}
+
 // What an entry's tokens weigh in a step, a thread a token, by workgroup z of `ways`, from the scores that the attention left (4 bytes a row beside D of the keys) and the
-// rows' log-sums; an entry with more rows than the call said has no scores, and its threads take the products themselves.
+// rows' log-sums.
 constexpr int kStepRows = 16;
 template <typename T, int FMT, int D>
 __device__ __forceinline__ void step_mass(const AttnArgs& a, const MassArgs& w, int e, int head, const RowSpan& rows, int start, int z, int ways, float (&s_lse)[kStepRows]) {
   const int len = a.c.tokens(e, start + rows.n), first_block = a.c.indptr[e], total = rows.n * a.group, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  if (total > a.score_rows) return rows_mass<T, FMT, D>(a, w, e, head, rows, start, z, ways);
   if (z * 256 >= len) return;
-  const bool scored = total <= a.score_rows;
   auto row_head = [&](int rr) { const QueryRow r = query_row(rr, total, a.group, rows, start, head); return (int64_t)r.row * a.heads + r.head; };
-  if (scored) {
-    for (int rr = wave; rr < total; rr += 4) {
-      const float x = a.n_split > 1 ? lse_of_splits(a, row_head(rr), lane) : a.lse[row_head(rr)];
-      if (lane == 0) s_lse[rr] = x;
-    }
-    __syncthreads();
+  for (int rr = wave; rr < total; rr += 4) {
+    const float x = a.n_split > 1 ? lse_of_splits(a, row_head(rr), lane) : a.lse[row_head(rr)];
+    if (lane == 0) s_lse[rr] = x;
   }
+  __syncthreads();
   for (int slot0 = z * 256; slot0 < len; slot0 += ways * 256) {
     const int slot = slot0 + threadIdx.x, block = slot / kKv8Page, t = slot % kKv8Page, page = slot < len ? a.c.page(e, block) : -1;
+    if (page < 0) continue;
+    const float* s = a.scores + (((int64_t)first_block + block) * a.c.kv_heads + head) * a.score_rows * kKv8Page + t;
     float x = 0.f;
-    if (scored) {
-      if (page < 0) continue;
-      const float* s = a.scores + (((int64_t)first_block + block) * a.c.kv_heads + head) * a.score_rows * kKv8Page + t;
 #pragma unroll 4
-      for (int rr = 0; rr < total; ++rr) x += exp2_of(s[rr * kKv8Page] - s_lse[rr]);
-    } else {
-      const uint8_t* kb = a.c.block(max(page, 0), 0, head, D) + t * 64;
-      const float ks = *a.c.scale(max(page, 0), 0, head) * a.scale_log2;
-      for (int rr = 0; rr < total; ++rr) {             // all lanes walk all rows: a row's log-sum is a wave's work
-        const QueryRow r = query_row(rr, total, a.group, rows, start, head);
-        const int64_t rh = (int64_t)r.row * a.heads + r.head;
-        const float lse = a.n_split > 1 ? lse_of_splits(a, rh, lane) : a.lse[rh];
-        const T* q = static_cast<const T*>(a.q) + r.row * a.q_stride + (int64_t)r.head * D;
-        float dot = 0.f;
-#pragma unroll 1
-        for (int d = 0; d < D; d += 4) {
-          float k[4], y[4];
-          kv8_numbers<FMT>(*reinterpret_cast<const uint32_t*>(kb + d / 64 * 1024 + d % 64), k);
-          ld4(q + d, y);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) dot = fmaf(k[i], y[i], dot);
-        }
-        if (slot <= r.far) x += exp2_of(fmaf(dot, ks, -lse));
-      }
-    }
-    if (page >= 0) put_mass(w, page, head * kKv8Page + t, x);
+    for (int rr = 0; rr < total; ++rr) x += exp2_of(s[rr * kKv8Page] - s_lse[rr]);
+    put_mass(w, page, head * kKv8Page + t, x);
   }
 }
 
@@ -864,7 +911,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? 2 : 1)) void kv8_mass_kernel
 // The weights of steps over many tokens.  Where the keys were split, the first `merges` workgroups of an entry and head join its outputs and the others take the rows'
 // log-sums from the splits' states: one launch for both (16 x 4096 tokens: 29.7 -> 27.5 us).
 template <typename T, int FMT, int D>
-__global__ __launch_bounds__(256) void kv8_step_finish_kernel(AttnArgs a, MassArgs w, int merges) {
+__global__ __launch_bounds__(256, (D == 128 ? 7 : 6)) void kv8_step_finish_kernel(AttnArgs a, MassArgs w, int merges) {
   __shared__ float s_lse[kStepRows];
   const int e = blockIdx.y, head = blockIdx.x, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const RowSpan rows = row_span(a.row0, e, a.n_rows);

@@ -5,7 +5,8 @@ import torch
 
 from oracle import kv8_ref as R
 from pegainfer_amd import ops_blocks as B
-from kv8_common import Cache, TORCH, codes_of
+from kv8_common import Cache, codes_of
+from test_gpu_kv8_ops import attend
 
 pytestmark = pytest.mark.gpu
 TYPES = {"bf16": torch.bfloat16, "fp32": torch.float32}
@@ -113,3 +114,38 @@ def test_a_hint_of_no_rows_gives_what_any_gives():
     for x, y in zip(got[:2], got[2:]):
         assert all(torch.equal(i, j) for i, j in zip(x, y))
     assert torch.equal(a.pool, b.pool) and torch.equal(a.scales, b.scales) and torch.equal(a.mass, b.mass)
+
+
+# ---- entries of more rows than the call said ----
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("kv,group,dim", [(2, 1, 64), (1, 3, 128), (1, 2, 256)])
+def test_weights_of_more_rows_than_were_said(fmt, dtype, kv, group, dim):
+    """the weights of a step's call where an entry brings a portion: over few tokens, over a run of keys, over split ones; pages that are not there"""
+    c = Cache([40, 9, 0], [70, 1, 33], kv, dim, fmt, seed=dim, layers=2)
+    c.ids[c.indptr[0] + 1] = -1
+    for length in (300, 1000, 9000):
+        attend(c, kv * group, TYPES[dtype], weigh=True, keep=0.5, hints=(1, length))
+    attend(Cache([1100, 3], [20, 1], kv, dim, fmt, seed=dim + 1), kv * group, TYPES[dtype], weigh=True, hints=(1, 1200), keep=0.0)
+
+
+def test_a_portion_among_single_tokens_is_not_a_cliff():
+    """the default hint is the average of the rows: with weights, a portion that it does not fit takes a few times what it takes with a hint of its own, not 66 times"""
+    n, kv, dim, ctx = 256, 8, 128, 300
+    c = Cache([ctx] * 32, [n] + [1] * 31, kv, dim, "int8", seed=50, dirty=False)
+    d = c.device()
+    q = torch.randn(c.row0[-1], kv, dim, device="cuda").bfloat16()
+
+    def time(most):
+        run = lambda: B.kv8_attention(q, d.codes, d.scales, d.row0, d.starts, d.indptr, d.ids, 0.1, max_rows=most, max_len=600, mass=d.mass)  # noqa: E731
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        run()
+        a.record()
+        for _ in range(10):
+            run()
+        b.record()
+        torch.cuda.synchronize()
+        return a.elapsed_time(b)
+
+    best = {most: min(time(most) for _ in range(3)) for most in (None, n)}
+    assert best[None] < 12 * best[n], best
