@@ -1093,7 +1093,7 @@ def kv8_evict(codes, scales, mass, lens, page_indptr, page_ids, dst_indptr, dst_
     entries = lens.numel()
     cache, kv, _, device = _kv8_cache(codes, scales, page_indptr, page_ids, entries)
     tables = _kv8_index(lens, entries, device, "lens"), _kv8_index(dst_indptr, entries + 1, device, "dst_indptr"), _kv8_index(dst_ids, None, device, "dst_ids")
-    _kv8_need(budget >= 1 and keep_first >= 0 and keep_last >= 0 and keep_first + keep_last <= budget, "budget of at least 1 token, keep_first + keep_last within it")
+    _kv8_need(1 <= budget < 2 ** 31 and keep_first >= 0 and keep_last >= 0 and keep_first + keep_last <= budget, "budget of 1 to 2^31 - 1 tokens, keep_first + keep_last within it")
     stride = _kv8_mass(mass, codes, "mass")
     kept = torch.empty((entries, kv, budget), dtype=torch.int32, device=codes.device)
     _chk(ffi.lib().pegainfer_kv8_evict(ctypes.addressof(cache), mass.data_ptr(), stride, *tables, dst_ids.numel(),

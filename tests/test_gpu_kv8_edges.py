@@ -149,3 +149,11 @@ def test_a_portion_among_single_tokens_is_not_a_cliff():
 
     best = {most: min(time(most) for _ in range(3)) for most in (None, n)}
     assert best[None] < 12 * best[n], best
+
+
+def test_a_budget_beyond_32_bits_is_refused():
+    c = Cache([20], [4], 1, 64, "e4m3")
+    d = c.device()
+    for budget, first in [(2 ** 31, 0), (2 ** 32 + 8, 0), (2 ** 32 + 8, 2 ** 32)]:
+        with pytest.raises(ValueError):
+            B.kv8_evict(d.codes, d.scales, d.mass, d.lens, d.indptr, d.ids, d.indptr, d.ids, budget, first)
