@@ -1097,8 +1097,8 @@ typedef struct {
 /* Rows of k, v [n_rows][kv_heads][dim] (rows of dtype at strides of 16 bytes) into the slots starts[e] ...  A block's scale is the least 2^e (e >= -100) whose
  * top reaches its largest finite value, and not below that of the tokens that were in the block before starts[e], which are rescaled where it grew; codes are
  * rounded to nearest, ties to even, but never to 2^128: what lies beyond the largest code * 2^e within fp32 (240 * 2^120, int8 127 * 2^121) becomes it; infinities
- * become the top, a NaN becomes 0.  Slots of a written block behind the entry's last row become 0.  Two entries
- * of a call must not write the same page. */
+ * become the top, a NaN becomes 0.  Slots of a written block behind the entry's last row become 0.  A call
+ * must not write a page twice, for two entries or for one whose table names it twice. */
 pegainfer_status_t pegainfer_kv8_append(const pegainfer_kv8_cache* cache, const void* k, const void* v, int64_t k_row_stride, int64_t v_row_stride,
                                         const int32_t* row0, const int32_t* starts, int32_t n_rows, int32_t max_rows, int32_t dtype, pegainfer_stream_t stream);
 /* The same into a cache whose tokens are weighed: mass [page][kv_heads][16] (fp32, pages mass_page_stride values apart) becomes 0 for the tokens that the rows bring and
@@ -1117,9 +1117,9 @@ pegainfer_status_t pegainfer_kv8_read(const pegainfer_kv8_cache* cache, const in
  * weight beside about the row's largest.  Entries may share pages (a common prompt).  out is not q.
  * mass_out given: mass_out[page][kv head][16] (fp32, pages mass_out_page_stride values apart) = mass_keep * mass + the weight that the call's rows and the kv
  * head's query heads gave to the token, for every slot of an entry that has rows, its new tokens among them (pegainfer_kv8_append_weighed sets theirs to 0; mass_out may
- * be mass; mass_keep 0: mass is not read and may be NULL).  Every
- * sum has one order: results do not change from run to run.  Entries of such a call must not share a page (both would write its weights): those of a common prompt
- * go in calls of their own, one after the other.
+ * be mass; mass_keep 0: mass is not read and may be NULL).  Every sum has one order: results do not change from run to run.  Entries of such a call must not share a
+ * page (both would write its weights, and one would be lost): those of a common prompt go in calls of their own, one after the other, with mass_keep 1 over weights
+ * that were scaled before.
  * workspace: fp32 scratch on 16 bytes of pegainfer_kv8_attention_workspace(...) values, of this call alone until it is done (0: NULL). */
 typedef struct {
   const void* q;

@@ -1055,10 +1055,10 @@ def kv8_read(codes, scales, row0, starts, page_indptr, page_ids, n_rows, dtype=t
 
 def kv8_attention(q, codes, scales, row0, starts, page_indptr, page_ids, scale, max_rows=None, max_len=None, out=None, mass=None, mass_out=None, mass_keep=1.0):
     """-> out [rows, heads, dim]: causal attention of q's rows (their own tokens are in the cache already).  max_rows / max_len: about the most rows / tokens of an
-    entry (None: the average of the rows, twice that of the pages); they choose how the call is cut, results are right for any, but two to
-    four times as late where a few rows are said and an entry has hundreds.  mass fp32 [pages, kv_heads, 16]:
-    mass_out (None: mass itself) becomes mass_keep * mass + the weight that every token got, the call's own among them (kv8_append(mass=) sets theirs to 0);
-    mass_out alone with mass_keep 0: the weight of this call.  Entries may share pages, but not where a call writes weights."""
+    entry (None: the average of the rows, twice that of the pages); they choose how the call is cut, results are right for any, but two to four times as late where a
+    few rows are said and an entry has hundreds.  mass fp32 [pages, kv_heads, 16]: mass_out (None: mass itself) becomes mass_keep * mass + the weight that every token
+    got, the call's own among them (kv8_append(mass=) sets theirs to 0); mass_out alone with mass_keep 0: the weight of this call.  Entries may share pages, but not
+    where a call writes weights (one entry's would be lost): then an entry a call, with mass_keep 1 over weights that were scaled before."""
     entries = row0.numel() - 1
     cache, kv, dim, device = _kv8_cache(codes, scales, page_indptr, page_ids, entries)
     row0_at, starts_at = _kv8_index(row0, entries + 1, device, "row0"), _kv8_index(starts, entries, device, "starts")

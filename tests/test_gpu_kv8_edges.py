@@ -5,7 +5,7 @@ import torch
 
 from oracle import kv8_ref as R
 from pegainfer_amd import ops_blocks as B
-from kv8_common import Cache, codes_of
+from kv8_common import Cache, attention_bound, codes_of, mass_bound
 from test_gpu_kv8_ops import attend
 
 pytestmark = pytest.mark.gpu
@@ -157,3 +157,29 @@ def test_a_budget_beyond_32_bits_is_refused():
     for budget, first in [(2 ** 31, 0), (2 ** 32 + 8, 0), (2 ** 32 + 8, 2 ** 32)]:
         with pytest.raises(ValueError):
             B.kv8_evict(d.codes, d.scales, d.mass, d.lens, d.indptr, d.ids, d.indptr, d.ids, budget, first)
+
+
+@pytest.mark.parametrize("rows", [[1, 1, 1], [40, 33, 3]])
+def test_weights_behind_a_common_prompt(rows):
+    """entries that share the pages of a prompt, one call each over weights that were scaled before: every page has the sum of all"""
+    kv, H, dim, keep = 2, 6, 64, 0.5
+    c = Cache([70, 64, 90], rows, kv, dim, "int8", seed=60, dirty=False)
+    for e in (1, 2):
+        c.ids[c.indptr[e]:c.indptr[e] + 4] = c.ids[:4]                   # 64 tokens
+    d = c.device()
+    d.mass *= keep
+    q = torch.randn(c.row0[-1], H, dim, device="cuda").bfloat16()
+    out = torch.zeros_like(q)
+    for e in range(3):
+        mine = slice(c.row0[e], c.row0[e + 1])
+        B.kv8_attention(q[mine], d.codes, d.scales, i32(0, rows[e]), d.starts[e:e + 1], i32(0, c.indptr[e + 1] - c.indptr[e]), d.ids[c.indptr[e]:c.indptr[e + 1]], 0.125, out=out[mine],
+                        mass=d.mass)
+    answer, mass, spread, reach = R.attention(q.float().cpu().numpy(), c.codes, c.scales, c.fmt, c.row0, c.starts, c.tables, 0.125)
+    assert (np.abs(out.double().cpu().numpy() - answer) <= attention_bound(spread, reach, answer, dim, 140, torch.bfloat16)).all()
+    want, most = keep * c.mass.astype(np.float64), np.zeros(c.mass.shape)
+    for e in range(3):
+        for s in range(mass[e].shape[1]):
+            p = c.ids[c.indptr[e] + s // 16]
+            want[p, :, s % 16] += mass[e][:, s]
+            most[p, :, s % 16] += mass_bound(mass[e][:, s], reach.max(), dim, 140, rows[e] * 3)
+    assert (np.abs(d.mass.cpu().numpy() - want) <= most + 2.0 ** -22 * want).all()
