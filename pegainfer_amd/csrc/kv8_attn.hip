@@ -42,8 +42,9 @@ __device__ __forceinline__ float across_quad(float v, Op op) {
 __device__ __forceinline__ float quad_max(float v) { return across_quad(v, [](float x, float y) { return fmaxf(x, y); }); }
 __device__ __forceinline__ float quad_sum(float v) { return across_quad(v, [](float x, float y) { return x + y; }); }
 // The maximum that a row's weights are taken against moves only when a score passes it by a factor of 2^kSlack, so that most steps need no exchange between lanes
-// and no rescaling.  Not by more: the maximum's own key has a weight of exactly 1 and a key above it at most 2, so no key whose weight is rounded to bf16 has over
-// two thirds of a row, and one with almost all of it gives its values.  16 rows x 500 keys to 256 rows x 20000: outputs off by 1.64 to 1.73e-3 of their norm, 1.62
+// and no rescaling.  Not by more: the maximum's own key has a weight of 1 (in prompts' unmasked steps but for the rounding of its score, 2^-24 of it, which bf16 takes
+// off again for scores below 2^15) and a key above it at most 2, so no key whose weight is rounded to bf16 has over two thirds of a row, and one with almost all of it
+// gives its values.  16 rows x 500 keys to 256 rows x 20000: outputs off by 1.64 to 1.73e-3 of their norm, 1.62
 // to 1.71e-3 with none, 1.72 to 1.97e-3 with 8; 2048 rows over 8192 tokens 255 us, 258 with none, 251 with 8.
 constexpr float kSlack = 1.f;
 
@@ -194,7 +195,8 @@ __device__ __forceinline__ void rows_mass(const AttnArgs& a, const MassArgs& w, 
 }
 
 // What an entry's tokens weigh in a step, a thread a token, by workgroup z of `ways`, from the scores that the attention left (4 bytes a row beside D of the keys) and the
-// rows' log-sums.
+// rows' log-sums.  Of up to 16 rows whatever the head, against keys and rows multiplied again (kv8_mass_kernel), 16 rows of each: 16 entries x 4096 tokens of 64 values 40 us
+// and 57, of 128 53 and 69, of 256 43 and 62; x 1000 tokens 19, 23, 32 and 20, 24, 29; a single row 25, 35, 31 and 56, 68, 60.
 constexpr int kStepRows = 16;
 template <typename T, int FMT, int D>
 __device__ __forceinline__ void step_mass(const AttnArgs& a, const MassArgs& w, int e, int head, const RowSpan& rows, int start, int z, int ways, float (&s_lse)[kStepRows]) {
@@ -231,8 +233,8 @@ template <typename T, int D, int NT> constexpr int attn_waves() {
 // keys' scores of one row, exactly what the second product wants from it.  The next keys are on their way while the weights are made, the next values while
 // the next scores are.
 // ONCE: the rows are one tile, so nobody reads the keys again and they pass the caches by (32 x 8192 tokens int8: 78 -> 70 us, 4.8 TB/s).
-// FEW: a step over so few tokens that the workgroup, which has seen them all, gives them their weights as well, without a second launch (100 tokens: 9.5 -> 8.2 us, of the
-// host 15.2 -> 12.4; over 1000 tokens the four walks through the scores take 1 us more than the launch).  An instance of its own: at its end the others lose 0.6 us.
+// FEW: a step over so few tokens that the workgroup, which has seen them all, gives them their weights as well, without a second launch (100 tokens: captured 9.5 -> 8.4 us,
+// called one by one 14.2 -> 12.0; over 1024 tokens the four walks through the scores take 1.5 us more than the launch).  An instance of its own: at its end the others lose 0.6 us.
 template <typename T, int FMT, int D, int NT, bool ONCE, bool FEW>
 __global__ __launch_bounds__(256, (attn_waves<T, D, NT>())) void kv8_attn_kernel(AttnArgs a, MassArgs w) {
   constexpr int NP = kv8_parts<T>(), C = D / 64, KB = attn_kb<T, D, NT>(), W = 4;
@@ -765,7 +767,7 @@ __global__ __launch_bounds__(256) void kv8_merge_rows_kernel(AttnArgs a) {
 // the rows that see them, MT tiles of sixteen a step, which its four waves (each with keys of its own) fetch together, two steps ahead, into shared memory: a
 // token's sum is one wave's, in the rows' order.  n_slice > 1, where that leaves too few workgroups: every slice of the rows leaves its sums in part,
 // kv8_mass_sum_kernel adds them in order.  Bound by shared memory's reads (one for four products, of 256 values for two) and the exponentials: 8000 rows of 32 / 8 heads of
-// 128 over themselves 382 us, 0.69 PFLOP/s; 3 prompts of up to 2000 of 16 / 4 x 256: 78.
+// 128 over themselves 350 us, 0.75 PFLOP/s of the scores; 3 prompts of up to 2000 of 16 / 4 x 256: 72.
 template <int D> constexpr int mass_blocks() { return D == 256 ? 2 : 4; }   // of keys, a wave
 template <typename T, int D> constexpr int mass_tiles() { return sizeof(T) == 2 ? 2 : 1; }   // fp32: three parts of every query
 
@@ -955,7 +957,9 @@ inline AttnPlan attn_plan(const pegainfer_kv8_cache* cache, int n_rows, int max_
   const int64_t want = 2 * device_cus();
   auto cut = [&](int64_t groups, int64_t most) { return (int)std::max<int64_t>(1, std::min((want + groups - 1) / groups, most)); };
   const int64_t groups = p.tiles * pairs;
-  // Whole over a run of 64 blocks (a step over 1024 tokens: 9.8 us; cut, 8.7 with a merge, whose launch costs the host 4).  Steps over more: runs of 16 blocks at least.
+  // Whole over a run of 64 blocks.  Steps over 1024 tokens of 8 heads of 128, called one by one: one entry 11.2 us whole, 13.5 cut with a merge, whose launch and workspace are
+  // the host's; 32 entries 14.5 and 18.  Captured the cut is faster for few entries (11.1 and 8.5; 16 entries 13.2 and 11.6; 32 14.5 and 17.9).  Steps over more: runs of 16 blocks
+  // at least.
   // Prompts: cut where they leave compute units without one (8 entries of 64 rows over 4000 tokens: 52 us in four, 64 in two), into runs of 32 blocks at least; a
   // split of 128 rows leaves 1 KB of sums a value of the head (32 entries of 32 rows over 1000 tokens, a workgroup a compute unit: 34 us whole, 46 halved).
   p.n_split = blocks <= kWholeBlocks ? 1
@@ -963,7 +967,7 @@ inline AttnPlan attn_plan(const pegainfer_kv8_cache* cache, int n_rows, int max_
               : groups >= device_cus() ? 1
                                        : (int)std::max<int64_t>(1, std::min<int64_t>({want / groups, blocks / 32, 256}));
   p.split_blocks = ceil_div(blocks, p.n_split);
-  p.few = blocks <= 32;                    // a step's weights by the attention's workgroups: two tokens a thread
+  p.few = blocks <= 32;                    // a step's weights by the attention's workgroups: two tokens a thread (500 tokens: 12.1 -> 11.8 us captured, 1024: 16.4 -> 17.9)
   p.round = (int)std::max<int64_t>(1, device_cus() / pairs);
   p.snake = p.n_split == 1 && p.tiles > p.round && p.tiles <= 2 * p.round;
   p.score_rows = rows <= kStepRows ? (int)rows : 0;

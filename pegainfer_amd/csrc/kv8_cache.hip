@@ -6,7 +6,7 @@
 
 namespace pk {
 
-// Rows pass the caches by, in and out: they are used once here (prompts written and read back 61 -> 54 us, 62 000 tokens read in fp32 158 -> 148).
+// Rows pass the caches by, in and out: they are used once here (prompts written and read back 61 -> 54 us, 62 000 tokens read in fp32 158 -> 151).
 // N = 4 or 8 values of a row at 8 or 16 bytes (fp32: 16)
 template <int N, typename T>
 __device__ __forceinline__ void rows_in(const T* p, float* x) {
@@ -63,9 +63,10 @@ __device__ __forceinline__ int unit_token(int side, int n, int q, int i) { retur
 
 // Rows into the cache.  One workgroup of two waves a (block, head): the rows' largest value, the exponent it wants (not below that of the tokens in front of
 // them in the block), their codes, and the older tokens' codes again where the exponent grew.  Bound by bytes: the rows are read once
-// (20 000 tokens of 8 x 128 from bf16: 34 us, 3.6 TB/s; 16 single tokens 5 us, a launch).  mass: given, the tokens that the rows bring weigh nothing yet, and the
+// (20 000 tokens of 8 x 128 from bf16: 36 us, 3.4 TB/s; 23 600 from fp32 60, 4.1; 16 single tokens 5 us, a launch).  mass: given, the tokens that the rows bring weigh nothing yet, and the
 // slots behind them neither, whatever a page's last owner left there.
-template <int D> constexpr int append_waves() { return D == 64 ? 8 : D == 128 ? 6 : 4; }   // of a SIMD, that the registers hold (8 x 128, prompts of up to 8000 rows in int8, with what is read back: 53 us with six or seven, 57 with five)
+// Waves of a SIMD that the registers hold (prompts of up to 8000 rows of 8 x 128 in int8, with what is read back: 53 us with seven, 57 with five)
+template <int D> constexpr int append_waves() { return D == 64 ? 8 : D == 128 ? 6 : 4; }
 template <typename T, int FMT, int D>
 __global__ __launch_bounds__(128, append_waves<D>()) void kv8_append_kernel(Kv8 c, float* mass, int64_t mass_stride, const T* k, const T* v, int64_t k_stride, int64_t v_stride,
                                                          const int32_t* row0, const int32_t* starts, int n_rows) {
@@ -119,7 +120,7 @@ __global__ __launch_bounds__(128, append_waves<D>()) void kv8_append_kernel(Kv8 
   }
 }
 
-// Tokens out of the cache: code * scale, exact in either type.  Bound by bytes, most of them written (62 000 tokens of 8 x 128 to fp32: 154 us, 4.0 TB/s).  Lanes are laid
+// Tokens out of the cache: code * scale, exact in either type.  Bound by bytes, most of them written (62 000 tokens of 8 x 128 to fp32: 151 us, 4.1 TB/s).  Lanes are laid
 // over the rows that leave, not over the blocks, so that whole lines do.
 template <typename T, int FMT, int D>
 __global__ __launch_bounds__(128) void kv8_read_kernel(Kv8 c, T* k, T* v, const int32_t* row0, const int32_t* starts, int n_rows) {
@@ -207,7 +208,7 @@ __device__ __forceinline__ int lanes_before(uint64_t mask, int n) { return __bui
 // lowest slots.  11 bits reach into the mantissa: weights share few exponents, and counts of one address are taken in turn.  Bound by what few workgroups issue, so the
 // weights are fetched once, through their pages, 16 bytes a lane, and kept in shared memory where they fit (36 864 tokens; of those beyond, every pass fetches
 // them again), and no pass asks where the first and last tokens are.  8 entries of up to 32 000 tokens and 8 heads: 24 us, 8 of them until the weights are there and
-// counted; 2000 tokens 8 us, 1 of them a histogram's barriers.
+// counted; 2000 tokens 8.6 us, 1 of them a histogram's barriers.
 constexpr int kPickThreads = 1024, kPickWaves = kPickThreads / 64, kPickCached = 36864;
 constexpr uint32_t kAlways = 0xFFFFFFFFu;   // in the place of a weight's order, which never has it: the first and last tokens, and what lies behind the last
 __global__ __launch_bounds__(kPickThreads) void kv8_pick_kernel(Kv8 c, const float* mass, int64_t mass_stride, const int32_t* lens, int budget, int keep_first,
