@@ -1111,7 +1111,8 @@ pegainfer_status_t pegainfer_kv8_append_weighed(const pegainfer_kv8_cache* cache
 pegainfer_status_t pegainfer_kv8_read(const pegainfer_kv8_cache* cache, const int32_t* row0, const int32_t* starts, void* k, void* v, int32_t n_rows, int32_t max_rows,
                                       int32_t dtype, pegainfer_stream_t stream);
 /* Causal softmax attention: row i of entry e sees the slots up to starts[e] + i (its own token is in the cache already), query head h reads kv head
- * h / (heads / kv_heads);  scale >= 0;  out[row, h] = sum_j softmax_j(scale q . k_j) v_j, zeros where a row sees nothing.  q, out: rows [heads][dim] of dtype at strides of
+ * h / (heads / kv_heads);  scale >= 0;  out[row, h] = sum_j softmax_j(scale q . k_j) v_j, zeros where a row sees nothing, or no score
+ * above -infinity.  q, out: rows [heads][dim] of dtype at strides of
  * 16 bytes.  Scores, softmax state and sums are fp32; bf16: the softmax weights are rounded to bf16 where they enter the matrix cores (their sum is not); fp32:
  * queries and weights enter as three bf16 parts, nothing is rounded.  Sums are divided at the end: values near fp32's largest must add up below it, each by its
  * weight beside about the row's largest.  Entries may share pages (a common prompt).  out is not q.

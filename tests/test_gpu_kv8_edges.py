@@ -183,3 +183,18 @@ def test_weights_behind_a_common_prompt(rows):
             want[p, :, s % 16] += mass[e][:, s]
             most[p, :, s % 16] += mass_bound(mass[e][:, s], reach.max(), dim, 140, rows[e] * 3)
     assert (np.abs(d.mass.cpu().numpy() - want) <= most + 2.0 ** -22 * want).all()
+
+
+@pytest.mark.parametrize("rows", [1, 8, 40])
+@pytest.mark.parametrize("length", [64, 2000])
+def test_a_row_without_a_score_above_minus_infinity(rows, length):
+    """zeros, and no weight: by steps, two row tiles and prompts, whole and split"""
+    c = Cache([200], [rows], 1, 64, "int8", seed=70, dirty=False)
+    c.codes[:, 0] = 3                                                    # every key is above 0
+    d = c.device()
+    q = torch.randn(rows, 4, 64, device="cuda").bfloat16()
+    q[0, 1] = -torch.inf
+    out = B.kv8_attention(q, d.codes, d.scales, d.row0, d.starts, d.indptr, d.ids, 0.125, max_len=length, mass=d.mass, mass_keep=0.0)
+    assert (out[0, 1] == 0).all() and torch.isfinite(out).all()
+    total = sum(d.mass[c.ids[s // 16], 0, s % 16] for s in range(200 + rows)).item()
+    assert abs(total - (4 * rows - 1)) <= 4 * rows * (200 + rows + 16) * 2.0 ** -22
